@@ -33,6 +33,7 @@ extern "C" {
 /* Device status word values (noise_read_status). */
 #define NOISE_DEVICE_OK 0
 #define NOISE_DEVICE_TIMEOUT 1     /* a bounded mbarrier/flag wait gave up; outputs are invalid */
+#define NOISE_DEVICE_BAD_INDEX 2   /* a sequence, position or page of a key / value cache call is out of range */
 
 /* Model dimensions of the fixed GPT (reference utils/model.py:34-43). */
 #define NOISE_N_LAYER 8
@@ -710,6 +711,121 @@ int noise_gemm_tf32_tn(const float* a, const float* b, float* d, int m, int n, i
  * Replaces autocast's per-call weight casts inside the reference's linears (eggroll.py:58 under
  * torch.autocast, eggroll.py:144). */
 int noise_pack_bf16(const float* src, void* dst, int64_t n, void* stream);
+
+/* ---- Answering: the operators of a generation step of several tokens (no counterpart in the reference, which trains
+ * only; they continue its block, utils/model.py:81-97, and head, :202-209, past a prompt). A sequence's step is a tree
+ * of `nodes` tokens, the last sampled one as its root and drafted ones under it; one node is plain decoding. ---- */
+
+/* [tokens, heads, dim] rows of a projection, the last dimension contiguous (strides in elements). */
+typedef struct {
+  const void* data;
+  int64_t token_stride;
+  int64_t head_stride;
+  int heads;
+} noise_heads_t;
+
+/* Head norm and rotation of queries and keys in one pass: per row x of dim values a = w x rsqrt(mean x^2 + eps), then
+ * over its halves y1 = a1 c + a2 s, y2 = a2 c - a1 s with the table rows c, s of the token's position (utils/model.py:
+ * 46-47, 55-58, 93-94; without a weight the order of norm and rotation does not matter).
+ *   dtype, table_dtype: NOISE_DTYPE_*, of q / k / weights / outputs and of the tables [table_rows, dim / 2]; positions
+ *   int32 [tokens] (one outside the tables gives NaN); weights [dim] or NULL; q_out [tokens, q->heads, dim] and k_out
+ *   contiguous. dim even, at most 256. Rows, strides and tables on 16-byte boundaries take wide loads, others do not. */
+int noise_head_norm_rope(const noise_heads_t* q, const noise_heads_t* k, const void* cos, const void* sin,
+                         int table_dtype, int table_rows, const int* positions, int tokens, int dim, int dtype,
+                         const void* q_weight, const void* k_weight, float eps, void* q_out, void* k_out,
+                         void* stream);
+
+/* Its gradient: dq, dk are the outputs' (any strides), q, k the inputs; dq_in [tokens, heads, dim] and dk_in receive the
+ * inputs' gradients (contiguous, dtype), dq_weight and dk_weight (fp32 [dim], or NULL) the weights', summed over tokens
+ * and heads in an order that does not change. workspace: noise_head_norm_rope_backward_workspace_bytes(dim) bytes,
+ * 16-byte aligned (no status block), needed where a weight's gradient is. */
+size_t noise_head_norm_rope_backward_workspace_bytes(int dim);
+int noise_head_norm_rope_backward(const noise_heads_t* dq, const noise_heads_t* dk, const noise_heads_t* q,
+                                  const noise_heads_t* k, const void* cos, const void* sin, int table_dtype,
+                                  int table_rows, const int* positions, int tokens, int dim, int dtype,
+                                  const void* q_weight, const void* k_weight, float eps, void* dq_in, void* dk_in,
+                                  float* dq_weight, float* dk_weight, void* workspace, size_t workspace_bytes,
+                                  void* stream);
+
+/* A paged key / value cache. k [layers, pages, heads, page_size, dim], v [layers, pages, heads, page_size / 4, dim, 4]
+ * (four tokens side by side), in bf16 or in 8-bit codes; k_scale, v_scale uint8 [layers, pages, heads, page_size]
+ * (8-bit kinds, else NULL): value = code * 2^(byte - 127), byte 255: the row held a NaN or an infinity and reads as NaN.
+ * status: an int32 on the device, zero at first, that a call which meets an index out of range sets to
+ * NOISE_DEVICE_BAD_INDEX (noise_read_status reads it). All 16-byte aligned but status. page_size a power of two from 16 to
+ * 4096; dim a multiple of 16 from 16 to 256 (attention: 64 or 128). */
+#define NOISE_KV_BF16 0
+#define NOISE_KV_E4M3 1
+#define NOISE_KV_INT8 2
+typedef struct {
+  void* k;
+  void* v;
+  uint8_t* k_scale;
+  uint8_t* v_scale;
+  int* status;
+  int layers;
+  int pages;
+  int heads;
+  int page_size;
+  int dim;
+  int kind;
+} noise_kv_cache_t;
+
+/* Write `tokens` rows of keys and values into layers [layer, layer + layers): entry i takes source row rows[i] (rows
+ * NULL: i) to position pos[i] of sequence seq[i], page table[seq, pos / page_size]. A negative seq, pos or row skips
+ * the entry; one past seqs, width * page_size, source_rows or pages is skipped and reported in status. k, v
+ * [layers, source_rows, heads, dim] of dtype, the last dimension contiguous; seq, pos, rows int32 [tokens]; table int32
+ * [seqs, width]. Two entries of a call for one place leave either. 8-bit kinds: the scale is the least power of two (not
+ * under 2^-126) with max|x| <= scale * 448 (e4m3) or 127 (int8), code = round(x / scale), ties to even. */
+int noise_kv_write(const noise_kv_cache_t* cache, int layer, int layers, const void* k, int64_t k_layer_stride,
+                   int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_layer_stride,
+                   int64_t v_token_stride, int64_t v_head_stride, int source_rows, int dtype, int tokens,
+                   const int* seq, const int* pos, const int* rows, const int* table, int seqs, int width,
+                   void* stream);
+
+/* Read positions back: k, v [layers, tokens, heads, dim] of dtype, contiguous, 16-byte aligned (bf16 holds every value
+ * of every kind exactly). Skipped entries give zeros, entries out of range NaN (and the status). */
+int noise_kv_read(const noise_kv_cache_t* cache, int layer, int layers, void* k, void* v, int dtype, int tokens,
+                  const int* seq, const int* pos, const int* table, int seqs, int width, void* stream);
+
+/* A tree's plan from its parents int32 [seqs, nodes] (-1: a root; else an earlier node; anything else, and what hangs
+ * from it, is padding): mask int64 [seqs, nodes], bit j of node i: i sees j (its ancestors and itself; padding 0), and
+ * depth int32 [seqs, nodes], the distance from the root (padding -1). nodes at most 64. */
+int noise_tree_plan(const int* parents, int seqs, int nodes, int64_t* mask, int* depth, void* stream);
+
+/* Attention of each sequence's tree over its cached tokens and over the tree. Node n of sequence b stands at position
+ * lengths[b] + depth[b, n]; with scale * (q . k) as its scores it sees cached positions below lengths[b] and the nodes in
+ * mask[b, n], those at most `window` positions back (window < 0: all). depth >= 0 for a real node; a depth below 0
+ * marks padding, whose output is 0; so is that of a row that sees nothing.
+ *   q [seqs, nodes, q_heads, dim], k, v [seqs, nodes, heads, dim] bf16, the last dimension contiguous (strides in
+ *   elements, of q and k multiples of 4; q 16-byte, k 8-byte aligned); q_heads a multiple of the cache's heads; table int32
+ *   [seqs, width]; lengths int32 [seqs] (taken as between 0 and width * page_size); out bf16 [seqs, nodes, q_heads,
+ *   dim]. nodes at most 64, seqs at most 4096, q_heads / heads at most 64, scale from 1e-18 to 1e18. A page out of
+ *   range makes its sequence's outputs NaN and sets the cache's status. workspace:
+ *   noise_tree_attention_workspace_bytes bytes, 16-byte aligned (no status block). */
+size_t noise_tree_attention_workspace_bytes(int seqs, int nodes, int q_heads, int heads, int dim);
+int noise_tree_attention(const noise_kv_cache_t* cache, int layer, const void* q, int64_t q_seq_stride,
+                         int64_t q_node_stride, int64_t q_head_stride, int q_heads, const void* k,
+                         int64_t k_seq_stride, int64_t k_node_stride, int64_t k_head_stride, const void* v,
+                         int64_t v_seq_stride, int64_t v_node_stride, int64_t v_head_stride, int seqs, int nodes,
+                         const int* table, int width, const int* lengths, const int64_t* mask, const int* depth,
+                         int window, float scale, void* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Verify drafted tokens against the target's logits [seqs, nodes, vocab] (dtype, last dimension contiguous) and name
+ * the next token. From the root on, a node's children (in their order) are tried: with p = softmax(cap(logits) /
+ * temperature), cap(z) = softcap tanh(z / softcap) (softcap 0: z), r = p and S = 1 at first, child c of token x is
+ * accepted if u[c] S q(x) < r(x), else r = max(r / S - q, 0), S = sum r; q = probs of the node (fp32 [seqs, nodes,
+ * vocab]; NULL: drafts picked without drawing, q = 1 at x). From an accepted child the walk goes on; where none is, the
+ * next token is the v with the largest r_v / race_v (S = 0: p_v / race_v), the lowest of equals. temperature 0: a child
+ * is accepted if its token is the largest logit's, which is the next token too; u, race and probs are not read.
+ *   tokens int64, parents int32, u fp32 [seqs, nodes]; race fp32 [seqs, vocab], positive; count int32 [seqs] accepted
+ *   drafts; path int32 [seqs, nodes] the nodes gone through from the root, then -1; token int64 [seqs] (-1 where the
+ *   logits name none). A token outside the vocabulary is never accepted; children follow their parent (a
+ *   node with an earlier index is none). nodes at most 64, vocab at most 393,216. */
+int noise_verify_tree(const void* logits, int logits_dtype, int64_t seq_stride, int64_t node_stride,
+                      const int64_t* tokens, const int* parents, const float* u, const float* race,
+                      const float* probs, int64_t probs_seq_stride, int64_t probs_node_stride, int seqs, int nodes,
+                      int vocab, float temperature, float softcap, int* count, int* path, int64_t* token,
+                      void* stream);
 
 /* Copy the device status word at the head of `workspace` to *status (synchronises `stream`). */
 int noise_read_status(const void* workspace, int* status, void* stream);

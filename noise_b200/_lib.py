@@ -72,6 +72,18 @@ class HeadPrep(ctypes.Structure):
                                                'hub_out', 'sq_q', 'sq_k', 'steps_q', 'steps_k')]
 
 
+class Heads(ctypes.Structure):
+    """noise_heads_t."""
+    _fields_ = [('data', ctypes.c_void_p), ('token_stride', ctypes.c_int64), ('head_stride', ctypes.c_int64),
+                ('heads', ctypes.c_int)]
+
+
+class KVCache(ctypes.Structure):
+    """noise_kv_cache_t."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ('k', 'v', 'k_scale', 'v_scale', 'status')] + \
+               [(n, ctypes.c_int) for n in ('layers', 'pages', 'heads', 'page_size', 'dim', 'kind')]
+
+
 class NoiseError(RuntimeError):
     pass
 
@@ -250,6 +262,30 @@ SIGNATURES = [
     ('noise_head_error_chunk', ctypes.c_int,
      [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64] + [ctypes.c_void_p] * 6 + [ctypes.c_int] * 4 +
      [ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p]),
+    ('noise_head_norm_rope', ctypes.c_int,
+     [ctypes.POINTER(Heads)] * 2 + [ctypes.c_void_p] * 2 + [ctypes.c_int] * 2 + [ctypes.c_void_p] + [ctypes.c_int] * 3 +
+     [ctypes.c_void_p] * 2 + [ctypes.c_float] + [ctypes.c_void_p] * 3),
+    ('noise_head_norm_rope_backward_workspace_bytes', ctypes.c_size_t, [ctypes.c_int]),
+    ('noise_head_norm_rope_backward', ctypes.c_int,
+     [ctypes.POINTER(Heads)] * 4 + [ctypes.c_void_p] * 2 + [ctypes.c_int] * 2 + [ctypes.c_void_p] + [ctypes.c_int] * 3 +
+     [ctypes.c_void_p] * 2 + [ctypes.c_float] + [ctypes.c_void_p] * 5 + [ctypes.c_size_t, ctypes.c_void_p]),
+    ('noise_kv_write', ctypes.c_int,
+     [ctypes.POINTER(KVCache), ctypes.c_int, ctypes.c_int, ctypes.c_void_p] + [ctypes.c_int64] * 3 +
+     [ctypes.c_void_p] + [ctypes.c_int64] * 3 + [ctypes.c_int] * 3 + [ctypes.c_void_p] * 4 + [ctypes.c_int] * 2 +
+     [ctypes.c_void_p]),
+    ('noise_kv_read', ctypes.c_int,
+     [ctypes.POINTER(KVCache), ctypes.c_int, ctypes.c_int] + [ctypes.c_void_p] * 2 + [ctypes.c_int] * 2 +
+     [ctypes.c_void_p] * 3 + [ctypes.c_int] * 2 + [ctypes.c_void_p]),
+    ('noise_tree_plan', ctypes.c_int,
+     [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    ('noise_tree_attention_workspace_bytes', ctypes.c_size_t, [ctypes.c_int] * 5),
+    ('noise_tree_attention', ctypes.c_int,
+     [ctypes.POINTER(KVCache), ctypes.c_int, ctypes.c_void_p] + [ctypes.c_int64] * 3 + [ctypes.c_int] +
+     ([ctypes.c_void_p] + [ctypes.c_int64] * 3) * 2 + [ctypes.c_int] * 2 + [ctypes.c_void_p, ctypes.c_int] +
+     [ctypes.c_void_p] * 3 + [ctypes.c_int, ctypes.c_float] + [ctypes.c_void_p] * 2 + [ctypes.c_size_t, ctypes.c_void_p]),
+    ('noise_verify_tree', ctypes.c_int,
+     [ctypes.c_void_p, ctypes.c_int] + [ctypes.c_int64] * 2 + [ctypes.c_void_p] * 5 + [ctypes.c_int64] * 2 +
+     [ctypes.c_int] * 3 + [ctypes.c_float] * 2 + [ctypes.c_void_p] * 4),
     ('noise_read_status', ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_int), ctypes.c_void_p]),
     ('noise_clear_status', ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     ('noise_status_string', ctypes.c_char_p, [ctypes.c_int]),

@@ -1,0 +1,150 @@
+"""CPU restatement, in 64 bits, of the operators that let the trained GPT answer — test infrastructure only.
+
+Head norm with rotation and its gradient, the cache's quantisation, attention of a tree of drafted tokens over a prefix,
+and the drafts' verification (definitions: include/noise_b200.h). Written plainly, one row or sequence at a time."""
+import math
+
+import torch
+
+QMAX = {'e4m3': 448.0, 'int8': 127.0}
+
+
+def head_norm_rope(x, cos, sin, positions, weight=None, eps=None):
+    """x [tokens, heads, D] -> fp64. eps: finfo(x.dtype).eps."""
+    eps = torch.finfo(x.dtype).eps if eps is None else eps
+    x = x.double()
+    a = x / torch.sqrt(x.square().mean(-1, keepdim=True) + eps)
+    if weight is not None:
+        a = a * weight.double()
+    c, s = cos.double()[positions.long()][:, None], sin.double()[positions.long()][:, None]
+    h = x.shape[-1] // 2
+    return torch.cat([a[..., :h] * c + a[..., h:] * s, a[..., h:] * c - a[..., :h] * s], -1)
+
+
+def head_norm_rope_backward(dy, x, cos, sin, positions, weight=None, eps=None):
+    """(dx, dw) in fp64 by the formula (dw None without a weight)."""
+    eps = torch.finfo(x.dtype).eps if eps is None else eps
+    x, dy = x.double(), dy.double()
+    r = 1 / torch.sqrt(x.square().mean(-1, keepdim=True) + eps)
+    c, s = cos.double()[positions.long()][:, None], sin.double()[positions.long()][:, None]
+    h = x.shape[-1] // 2
+    g = torch.cat([dy[..., :h] * c - dy[..., h:] * s, dy[..., :h] * s + dy[..., h:] * c], -1)
+    w = 1.0 if weight is None else weight.double()
+    xh = x * r
+    dx = r * (w * g - xh * (w * g * xh).mean(-1, keepdim=True))
+    return dx, None if weight is None else (g * xh).sum((0, 1))
+
+
+def scale_exponent(top, kind):
+    """The least e >= -126 with top <= 2^e * qmax, by trial."""
+    if top == 0:
+        return -126
+    e = max(-126, math.frexp(top / QMAX[kind])[1] - 2)
+    while math.ldexp(QMAX[kind], e) < top:
+        e += 1
+    return e
+
+
+def quantised(x, kind):
+    """The values (fp64) that rows x [..., D] read back as."""
+    flat = x.double().reshape(-1, x.shape[-1])
+    if kind == 'bf16':
+        return x.double().to(torch.bfloat16).double()
+    out = torch.empty_like(flat)
+    for i, row in enumerate(flat):
+        if not torch.isfinite(row).all():
+            out[i] = math.nan
+            continue
+        scale = math.ldexp(1.0, scale_exponent(row.abs().max().item(), kind))
+        y = row / scale
+        if kind == 'int8':
+            out[i] = torch.round(y) * scale
+        else:  # 1 + 3 bits from 2^-6 up, steps of 2^-9 below
+            e = torch.clamp(torch.frexp(y)[1] - 1, min=-6)
+            step = torch.ldexp(torch.ones_like(y), e - 3)
+            out[i] = torch.round(y / step) * step * scale
+    return out.reshape(x.shape)
+
+
+def tree_plan(parents):
+    """(mask, depth) as lists of one tree's parents."""
+    mask, depth = [], []
+    for i, p in enumerate(parents):
+        real = p == -1 or (0 <= p < i and depth[p] >= 0)
+        mask.append((1 << i) | (mask[p] if p >= 0 else 0) if real else 0)
+        depth.append(-1 if not real else 0 if p == -1 else depth[p] + 1)
+    return mask, depth
+
+
+def tree_attention(q, k, v, past_k, past_v, mask, depth, window=-1, scale=None):
+    """One sequence: q [N, heads, D], k, v [N, k heads, D], past_k, past_v [len, k heads, D] (what the cache reads as);
+    mask, depth lists -> (o, a) fp64 [N, heads, D]: the outputs and the same averages of |v|."""
+    n, heads, d = q.shape
+    group, length = heads // k.shape[1], past_k.shape[0]
+    scale = d ** -0.5 if scale is None else scale
+    out, size = torch.zeros(n, heads, d, dtype=torch.float64), torch.zeros(n, heads, d, dtype=torch.float64)
+    for i in range(n):
+        if depth[i] < 0:
+            continue
+        at = length + depth[i]
+        past = [j for j in range(length) if window < 0 or at - j <= window]
+        nodes = [j for j in range(n) if mask[i] >> j & 1 and (window < 0 or depth[i] - depth[j] <= window)]
+        if not past and not nodes:
+            continue
+        for h in range(heads):
+            kk = torch.cat([past_k[past, h // group].double(), k[nodes, h // group].double()])
+            vv = torch.cat([past_v[past, h // group].double(), v[nodes, h // group].double()])
+            p = (kk @ q[i, h].double() * scale).softmax(0)
+            out[i, h] = (p[:, None] * vv).sum(0)
+            size[i, h] = (p[:, None] * vv.abs()).sum(0)
+    return out, size
+
+
+def target(z, temperature, softcap):
+    z = z.double()
+    if softcap > 0:
+        z = softcap * torch.tanh(z / softcap)
+    return z if temperature == 0 else (z / temperature).softmax(-1)
+
+
+def verify_tree(logits, tokens, parents, u, race, probs=None, temperature=1.0, softcap=0.0):
+    """One sequence -> (count, path, token, margin): margin is how far, relatively, the closest decision was from going
+    the other way."""
+    n, vocab = logits.shape
+    at, path, margin = 0, [0], math.inf
+    while True:
+        p = target(logits[at], temperature, softcap)
+        kids = [c for c in range(at + 1, n) if parents[c] == at]
+        nxt = None
+        if temperature == 0:
+            best = int(p.argmax())
+            nxt = next((c for c in kids if tokens[c] == best), None)
+        else:
+            r, mass = p.clone(), 1.0
+            for c in kids:
+                x = int(tokens[c])
+                if 0 <= x < vocab:
+                    q = 1.0 if probs is None else float(probs[at, x])
+                    test, value = float(u[c]) * mass * q, float(r[x])
+                    margin = min(margin, abs(test - value) / max(test, value, 1e-300))
+                    if test < value:
+                        nxt = c
+                        break
+                draft = torch.zeros(vocab, dtype=torch.float64) if probs is None else probs[at].double()
+                if probs is None and 0 <= x < vocab:
+                    draft[x] = 1.0
+                r = (r / (mass if mass > 0 else 1.0) - draft).clamp(min=0)
+                mass = float(r.sum())
+        if nxt is None:
+            break
+        at = nxt
+        path.append(at)
+    if temperature == 0:
+        token = best
+    else:
+        score = (r if mass > 0 else p) / race.double()
+        top = score.topk(min(2, vocab)).values
+        if vocab > 1:
+            margin = min(margin, float((top[0] - top[1]) / top[0]))
+        token = int(score.argmax())
+    return len(path) - 1, path + [-1] * (n - len(path)), token, margin

@@ -1,0 +1,597 @@
+"""The operators that let the trained GPT answer (noise_b200.decode) against the oracle in 64 bits: head norm with rotation
+and its gradient, the quantised cache, tree attention and verification.
+
+Tolerances, from the roundings the kernels make:
+- head norm in fp32: the row's sum, rsqrt, two products and a sum of two, each within 2^-23 of its terms: a dozen times
+  2^-23 of |a1| + |a2|; in bf16 half a last place more (8 bits: 2^-8 of the
+  result at most).
+- the cache: none. A power of two as the scale makes every step but the rounding exact, so the codes are the oracle's.
+- attention: bf16 outputs, 2^-8 of the result; P in bf16 at worst, 2^-8 of the average a of |v|, and 2^-12 of a for the
+  scores' and sums' fp32 roundings.
+- verification: whole numbers, equal wherever no decision is closer than 1e-4 (relative) to going the other way."""
+import math
+
+import pytest
+import torch
+
+from oracle import decode as oracle
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device('cuda', 0) if torch.cuda.is_available() else None
+
+
+def _tables(n, dim, dtype=torch.bfloat16):
+    angle = torch.outer(torch.arange(n).float(), 1e4 ** (-torch.arange(0, dim, 2).float() / dim))
+    return angle.cos().to(dtype).to(DEV), angle.sin().to(dtype).to(DEV)
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+# ---- head norm and rotation -----------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('tokens,qh,kh,dim,weights,offset', [
+    (1, 8, 8, 64, False, 0), (7, 32, 8, 128, True, 0), (130, 5, 1, 96, True, 0), (3, 3, 2, 256, False, 0),
+    (9, 2, 7, 6, True, 0), (33, 4, 4, 64, True, 1), (5, 9, 1, 16, False, 0), (2, 1, 1, 250, True, 3)])
+def test_head_norm_rope(dtype, tokens, qh, kh, dim, weights, offset):
+    """Views of one projection's rows, even and odd sizes, addresses off the 16-byte grid (offset values)."""
+    from noise_b200 import decode
+    g = _gen(tokens * dim)
+    flat = torch.randn(tokens * (qh + kh + 1) * dim + offset, generator=g).to(dtype)
+    flat[: dim // 2] = 0
+    qkv = flat.to(DEV)[offset:].view(tokens, qh + kh + 1, dim)
+    q, k = qkv[:, :qh], qkv[:, qh:qh + kh]
+    cos, sin = _tables(300, dim, torch.float32 if dim == 96 else torch.bfloat16)
+    pos = torch.randint(0, 300, (tokens,), generator=g, dtype=torch.int32).to(DEV)
+    w = [(1 + 0.3 * torch.randn(dim, generator=g)).to(dtype).to(DEV) if weights else None for _ in range(2)]
+    got = decode.head_norm_rope(q, k, cos, sin, pos, *w)
+    dq, dk = (torch.randn(x.shape, generator=g).to(dtype).to(DEV) for x in (q, k))
+    grads = decode.head_norm_rope_backward(dq, dk, q, k, cos, sin, pos, *w)
+    cpu = lambda t: None if t is None else t.cpu()  # noqa: E731
+    for i, (x, d) in enumerate(((q, dq), (k, dk))):
+        args = (cos.cpu(), sin.cpu(), pos.cpu(), cpu(w[i]))
+        ref = oracle.head_norm_rope(x.cpu(), *args)
+        half = dim // 2
+        a = ref.abs()
+        size = (a[..., :half] + a[..., half:]).repeat(1, 1, 2) + 1e-30  # |a1| + |a2| is at most sqrt 2 of this
+        last = 2.0 ** -8 if dtype == torch.bfloat16 else 0.0
+        assert got[i].shape == x.shape and got[i].is_contiguous()
+        err = (got[i].cpu().double() - ref).abs()
+        assert (err <= 12 * 2.0 ** -23 * size + last * a).all(), (err / size).max()
+        dx, dw = oracle.head_norm_rope_backward(d.cpu(), x.cpu(), *args)
+        # every term is within a few 2^-23 of r |w g| or of r |xh| mean |h xh|: bounded by the row's largest h
+        r = 1 / torch.sqrt(x.cpu().double().square().mean(-1, keepdim=True) + torch.finfo(dtype).eps)
+        wmax = 1.0 if w[i] is None else w[i].abs().max().item()
+        xh = (x.cpu().double() * r).abs().amax(-1, keepdim=True)
+        size = r * wmax * d.cpu().double().abs().amax(-1, keepdim=True) * 1.5 * (1 + xh)
+        err = (grads[i].cpu().double() - dx).abs()
+        assert (err <= (16 + dim / 16) * 2.0 ** -23 * size + last * dx.abs()).all(), (err / size).max()
+        if w[i] is None:
+            assert grads[2 + i] is None
+        else:
+            terms = tokens * x.shape[1]
+            size = 2 * d.cpu().double().abs().max() * xh.max()
+            err = (grads[2 + i].cpu().double() - dw).abs().max()
+            assert err <= 2.0 ** -23 * size * terms * 4, err  # each term a few last places, the sums no more
+
+
+def test_head_norm_rope_gradient_against_differences():
+    """(L(x + t d) - L(x - t d)) / 2t in the kernel's own fp32 forward, along random directions; truncation t^2 and
+    rounding 2^-23 |L| / t are both below 1e-3 of |grad||d| for t = 2^-7."""
+    from noise_b200 import decode
+    g = _gen(5)
+    q, k = torch.randn(6, 4, 64, generator=g).to(DEV), torch.randn(6, 2, 64, generator=g).to(DEV)
+    w = [(1 + 0.2 * torch.randn(64, generator=g)).to(DEV) for _ in range(2)]
+    cos, sin = _tables(32, 64, torch.float32)
+    pos = torch.arange(6, dtype=torch.int32, device=DEV)
+    cq, ck = torch.randn(q.shape, generator=g).to(DEV), torch.randn(k.shape, generator=g).to(DEV)
+    leaves = [x.clone().requires_grad_() for x in (q, k, *w)]
+
+    def loss(q, k, qw, kw):
+        a, b = decode.head_norm_rope(q, k, cos, sin, pos, qw, kw)
+        return (a.double() * cq).sum() + (b.double() * ck).sum()
+    grads = torch.autograd.grad(loss(*leaves), leaves)
+    for i in range(4):
+        d = torch.randn(leaves[i].shape, generator=g).to(DEV)
+        t = 2.0 ** -7
+        moved = [[x + s * t * d if j == i else x for j, x in enumerate((q, k, *w))] for s in (1, -1)]
+        diff = (loss(*moved[0]) - loss(*moved[1])).item() / (2 * t)
+        want = (grads[i].double() * d).sum().item()
+        assert abs(diff - want) <= 2e-3 * grads[i].double().norm().item() * d.double().norm().item()
+
+
+def test_head_norm_rope_agrees_with_the_reference_order():
+    """norm(rope(x)), as the framework's model has it, is the same without a weight."""
+    from noise_b200 import decode
+    from oracle import gpt
+    x = torch.randn(50, 8, 64, generator=_gen(3))
+    cos, sin = (t[:50] for t in gpt.rotary())
+    ref = gpt.norm(gpt.apply_rotary_emb(x, cos.float(), sin.float()))
+    got, _ = decode.head_norm_rope(x.to(DEV), x.to(DEV), cos.to(DEV), sin.to(DEV),
+                                   torch.arange(50, dtype=torch.int32, device=DEV))
+    # bf16 cos and sin are no exact rotation: c^2 + s^2 is within 2^-8 of 1, and so are the two norms
+    assert ((got.cpu() - ref).abs() <= 2.0 ** -7 * ref.abs() + 1e-5).all()
+
+
+def test_head_norm_rope_edges():
+    from noise_b200 import decode
+    cos, sin = _tables(4, 64)
+    q = torch.randn(3, 2, 64, generator=_gen(1)).to(DEV)
+    q[0, 0] = 0
+    pos = torch.tensor([0, 4, -1], dtype=torch.int32, device=DEV)  # two positions without a table row
+    out, _ = decode.head_norm_rope(q, q, cos, sin, pos)
+    assert (out[0, 0] == 0).all() and torch.isfinite(out[0]).all() and torch.isnan(out[1:]).all()
+    none = q[:0]
+    a, b = decode.head_norm_rope(none, none, cos, sin, pos[:0])
+    assert a.shape == b.shape == (0, 2, 64)
+    w = torch.ones(64, device=DEV)
+    grads = decode.head_norm_rope_backward(none, none, none, none, cos, sin, pos[:0], w, w)
+    assert (grads[2] == 0).all() and (grads[3] == 0).all()
+
+
+# ---- the cache ------------------------------------------------------------------------------------------------
+
+
+def _cache(kind, dim, heads, page, seqs, room, layers=1, seed=0):
+    """A cache of shuffled pages and its table."""
+    from noise_b200.decode import KVCache
+    width = -(-room // page)
+    pages = seqs * width + 2
+    cache = KVCache(layers, pages, heads, dim, kind, page, DEV)
+    table = torch.randperm(pages, generator=_gen(seed))[:seqs * width].int().view(seqs, width).to(DEV)
+    return cache, table
+
+
+@pytest.mark.parametrize('kind', ['bf16', 'e4m3', 'int8'])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('dim,heads,page,offset', [(64, 8, 64, 0), (128, 2, 16, 0), (16, 1, 16, 0), (96, 3, 32, 1),
+                                                   (256, 2, 16, 0)])
+def test_cache_holds_the_rounded_values(kind, dtype, dim, heads, page, offset):
+    g = _gen(dim)
+    lens = [page + 3, 1, 2 * page]
+    cache, table = _cache(kind, dim, heads, page, 3, 2 * page)
+    seq = torch.cat([torch.full((n,), i) for i, n in enumerate(lens)]).int()
+    pos = torch.cat([torch.arange(n) for n in lens]).int()
+    order = torch.randperm(len(seq), generator=g)
+    seq, pos = seq[order].to(DEV), pos[order].to(DEV)
+    t = len(order)
+    # rows of every size, to the ends of the range; ties of the codes' grid among them
+    spread = torch.exp2(torch.randint(-12, 12, (t, heads, 1), generator=g).float())
+    spread[0], spread[1], spread[2] = 2.0 ** -130, 2.0 ** 100, 2.0 ** -100
+    flat = torch.empty(2 * t * heads * dim + offset).normal_(generator=g).to(dtype)
+    kv = (flat[offset:].view(t, 2, heads, dim) * spread[:, None].to(dtype))
+    kv[3, 0, 0] = 0
+    kv[4] = torch.arange(dim).to(dtype) * 0.5 - 8
+    kv[5, 1, 0, 3], kv[6, 0, 0, 5], kv[7, 1, 0, 0] = math.nan, math.inf, -math.inf
+    buf = torch.empty_like(flat).to(DEV)
+    buf[offset:] = kv.reshape(-1).to(DEV)
+    kv_dev = buf[offset:].view(t, 2, heads, dim)
+    cache.write(kv_dev[:, 0], kv_dev[:, 1], seq, pos, table)
+    for out in (torch.float32, torch.bfloat16):
+        got = cache.read(seq, pos, table, dtype=out)
+        for i in range(2):
+            ref = oracle.quantised(kv[:, i], kind)
+            a = got[i].cpu().double()
+            assert torch.equal(torch.isnan(a), torch.isnan(ref))
+            if kind == 'bf16':
+                assert torch.equal(a.nan_to_num(), ref.nan_to_num())
+            else:  # values below fp32's smallest normal ones may be flushed
+                tiny = ref.abs() < 2.0 ** -126
+                assert torch.equal(torch.where(tiny, 0.0, a).nan_to_num(), torch.where(tiny, 0.0, ref).nan_to_num())
+    # what was read back, written again, reads as the same values (e4m3 may take half the scale and twice the codes: a
+    # largest value just above 224 scales rounds down to it)
+    k, v = cache.read(seq, pos, table, dtype=torch.float32)
+    fine = torch.isfinite(kv.double()).all(-1).all(-1).all(-1).to(DEV)
+    cache.write(k, v, torch.where(fine, seq, -1), pos, table)
+    again = cache.read(seq, pos, table, dtype=torch.float32)
+    assert all(torch.equal(x[fine], y[fine]) for x, y in zip((k, v), again))
+    cache.check()
+
+
+def test_cache_rows_layers_and_bad_places():
+    from noise_b200._lib import NoiseError
+    cache, table = _cache('int8', 64, 2, 16, 2, 48, layers=3)
+    g = _gen(8)
+    k, v = (torch.randn(3, 5, 2, 64, generator=g).to(DEV) for _ in range(2))
+    seq = torch.tensor([0, 1, 1, -1, 0], dtype=torch.int32, device=DEV)
+    pos = torch.tensor([5, 47, 0, 3, -1], dtype=torch.int32, device=DEV)
+    rows = torch.tensor([4, 0, -1, 1, 2], dtype=torch.int32, device=DEV)
+    cache.write(k, v, seq, pos, table, layer=None, rows=rows)  # all layers; entries 2, 3 and 4 are skipped
+    got = cache.read(seq, pos, table, layer=None)
+    for x, y in zip((k, v), got):
+        for layer in range(3):
+            for entry, row in ((0, 4), (1, 0)):
+                assert torch.equal(oracle.quantised(x[layer, row].cpu(), 'int8'), y[layer, entry].cpu().double())
+        assert (y[:, 2:] == 0).all()  # entry 2's place was never written, the others are no places
+    cache.check()
+    assert torch.equal(cache.read(seq, pos, table, layer=1)[0], got[0][1])
+    untouched = cache.k.clone()
+    bad = torch.tensor([2, 0, 0], dtype=torch.int32, device=DEV), torch.tensor([0, 48, 0], dtype=torch.int32, device=DEV)
+    for s, p, r in [(bad[0][:1], bad[1][:1], None), (bad[0][1:2], bad[1][1:2], None),
+                    (bad[0][2:], bad[1][2:], torch.tensor([5], dtype=torch.int32, device=DEV))]:
+        cache.write(k[0], v[0], s, p, table, rows=r)
+        with pytest.raises(NoiseError, match='out of range'):
+            cache.check()
+        cache.check()  # the report is given once
+    broken = table.clone()
+    broken[0, 0] = cache.pages
+    cache.write(k[0], v[0], bad[0][2:], bad[1][2:], broken)
+    got, _ = cache.read(bad[0][2:], bad[1][2:], broken)
+    assert torch.isnan(got).all() and torch.equal(untouched, cache.k)
+    with pytest.raises(NoiseError, match='out of range'):
+        cache.check()
+
+
+# ---- tree attention -------------------------------------------------------------------------------------------
+
+
+def _fill(cache, table, lens, g):
+    """Random keys and values at positions below lens; what they read back as, [seq][len, heads, D] on the CPU."""
+    past = []
+    for b, n in enumerate(lens):
+        k, v = (torch.randn(n, cache.heads, cache.dim, generator=g).to(torch.bfloat16).to(DEV) for _ in range(2))
+        v = v * torch.exp2(torch.randint(-3, 4, (n, 1, 1), generator=g).float().to(DEV)).bfloat16()
+        seq, pos = torch.full((n,), b, dtype=torch.int32, device=DEV), torch.arange(n, dtype=torch.int32, device=DEV)
+        cache.write(k, v, seq, pos, table)
+        past.append([x.cpu() for x in cache.read(seq, pos, table, dtype=torch.float32)])
+    return past
+
+
+def _random_tree(n, g):
+    parents = [-1] + [int(torch.randint(max(0, i - 5), i, (1,), generator=g)) for i in range(1, n)]
+    if n > 3:
+        parents[n // 2] = -2  # padding, with whatever hangs from it
+    return parents
+
+
+def _check(got, q, k, v, past, plan, window=-1, scale=None):
+    for b, (mask, depth) in enumerate(plan):
+        ref, a = oracle.tree_attention(q[b].cpu(), k[b].cpu(), v[b].cpu(), *past[b], mask, depth, window, scale)
+        err = (got[b].cpu().double() - ref).abs()
+        assert torch.isfinite(got[b]).all()
+        assert (err <= 2.0 ** -8 * ref.abs() + (2.0 ** -8 + 2.0 ** -12) * a).all(), (b, (err / (a + 1e-30)).max().item())
+
+
+@pytest.mark.parametrize('kind', ['bf16', 'e4m3', 'int8'])
+@pytest.mark.parametrize('dim', [64, 128])
+@pytest.mark.parametrize('nodes,heads,group,page,window', [
+    (1, 2, 1, 64, -1), (1, 2, 4, 16, 100), (5, 1, 3, 16, -1), (16, 2, 1, 32, 30), (17, 1, 2, 64, 17), (64, 1, 1, 16, -1),
+    (33, 1, 8, 64, 64), (3, 1, 32, 128, 0), (64, 2, 4, 64, 5)])
+def test_tree_attention(kind, dim, nodes, heads, group, page, window):
+    """Lengths from none to several units, trees with padding, grouped heads, windows that end inside a page and inside
+    the tree; q, k and v views of one projection's rows."""
+    from noise_b200 import decode
+    g = _gen(nodes * dim + group)
+    lens = [0, 1, 15, 16, 17, 63, 64, 65, 127, 200, 331]
+    cache, table = _cache(kind, dim, heads, page, len(lens), 384, seed=nodes)
+    past = _fill(cache, table, lens, g)
+    parents = torch.tensor([_random_tree(nodes, g) for _ in lens], dtype=torch.int32, device=DEV)
+    mask, depth = decode.tree_plan(parents)
+    plan = [oracle.tree_plan(p) for p in parents.tolist()]
+    assert [[m & (1 << 64) - 1 for m in row] for row in mask.tolist()] == [m for m, _ in plan]
+    assert depth.tolist() == [d for _, d in plan]
+    qkv = torch.randn(len(lens), nodes, heads * (group + 2), dim, generator=g).to(torch.bfloat16).to(DEV)
+    q, k, v = qkv[:, :, :heads * group] * 2, qkv[:, :, heads * group:-heads], qkv[:, :, -heads:]
+    lengths = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    got = decode.tree_attention(q, k, v, cache, table, lengths, mask, depth, window=window)
+    _check(got, q, k, v, past, plan, window)
+    assert torch.equal(got, decode.tree_attention(q, k, v, cache, table, lengths, mask, depth, window=window))
+    cache.check()
+
+
+@pytest.mark.parametrize('kind', ['bf16', 'int8'])
+def test_tree_attention_long_and_layers(kind):
+    """A row split over many CTAs and joined, in the last layer of a cache."""
+    from noise_b200 import decode
+    g = _gen(4)
+    cache, table = _cache(kind, 64, 2, 64, 3, 5000, layers=2)
+    lens = [4999, 0, 2500]
+    full, cache_k = cache, cache.k
+    last = decode.KVCache.of(cache.k[1:], cache.v[1:], *(None if s is None else s[1:]
+                                                         for s in (cache.k_scale, cache.v_scale)))
+    past = _fill(last, table, lens, g)
+    q, k, v = (torch.randn(3, 1, h, 64, generator=g).to(torch.bfloat16).to(DEV) for h in (4, 2, 2))
+    mask, depth = decode.tree_plan(torch.full((3, 1), -1, dtype=torch.int32, device=DEV))
+    lengths = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    got = decode.tree_attention(q, k, v, full, table, lengths, mask, depth, layer=1)
+    _check(got, q, k, v, past, [oracle.tree_plan([-1])] * 3)
+    assert (cache_k[0].float() == 0).all()
+    # a large scale: all weight on one key
+    got = decode.tree_attention(q, k, v, full, table, lengths, mask, depth, layer=1, scale=4.0)
+    _check(got, q, k, v, past, [oracle.tree_plan([-1])] * 3, scale=4.0)
+
+
+@pytest.mark.parametrize('kind', ['bf16', 'e4m3', 'int8'])
+def test_tree_attention_ignores_what_is_masked(kind):
+    """NaN and infinities past the sequence's end, before the window, in padding nodes and in branches not seen."""
+    from noise_b200 import decode
+    g = _gen(11)
+    cache, table = _cache(kind, 64, 1, 16, 3, 160)
+    lens, window = [133, 90, 7], 40
+    past = _fill(cache, table, lens, g)
+    every = torch.arange(160, dtype=torch.int32, device=DEV)
+    for b, n in enumerate(lens):  # the rest of the pages, and what lies before the window of even the root
+        at = torch.cat([every[n:], every[:max(0, n - window - 1)]])
+        junk = torch.full((len(at), 1, 64), math.nan, device=DEV)
+        junk[::2] = math.inf
+        cache.write(junk, junk, torch.full_like(at, b), at, table)
+    if kind != 'bf16':  # codes and scales that no write leaves, past the end of sequence 2
+        page = table[2, 1]
+        cache.k.view(torch.uint8)[:, page] = 0x7f
+        cache.v.view(torch.uint8)[:, page] = 0xff
+        cache.v_scale[:, page] = 254
+    # the window's edge differs between the nodes: position 93 - 40 is the root's last, not its children's
+    parents = [[-1, 0, 0, 1, -2, 2, 5, 6]] * 3
+    plan = [oracle.tree_plan(p) for p in parents]
+    mask, depth = decode.tree_plan(torch.tensor(parents, dtype=torch.int32, device=DEV))
+    q, k, v = (torch.randn(3, 8, h, 64, generator=g).to(torch.bfloat16) for h in (2, 1, 1))
+    k[:, 4], v[:, 4] = math.nan, math.inf  # the padding node
+    lengths = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    got = decode.tree_attention(q.to(DEV), k.to(DEV), v.to(DEV), cache, table, lengths, mask, depth, window=window)
+    _check(got, q, k, v, past, plan, window)
+    # a NaN in one branch (node 1) and an infinity in its child reach the rows that see them, and no others
+    v2 = v.clone()
+    v2[:, 1, 0, 5], v2[:, 3, 0, 9] = math.nan, -math.inf
+    got2 = decode.tree_attention(q.to(DEV), k.to(DEV), v2.to(DEV), cache, table, lengths, mask, depth, window=window)
+    same = torch.ones_like(got, dtype=torch.bool)
+    same[:, [1, 3], :, 5] = same[:, 3, :, 9] = False
+    assert torch.equal(got[same], got2[same])
+    assert torch.isnan(got2[:, [1, 3], :, 5]).all() and (got2[:, 3, :, 9] == -math.inf).all()
+    # a cached row at the window's edge: the root sees it, its children do not
+    at = torch.tensor([lens[0] - window], dtype=torch.int32, device=DEV)
+    bad = torch.full((1, 1, 64), math.nan, device=DEV)
+    cache.write(torch.zeros_like(bad), bad, torch.zeros_like(at), at, table)
+    got3 = decode.tree_attention(q.to(DEV), k.to(DEV), v.to(DEV), cache, table, lengths, mask, depth, window=window)
+    assert torch.isnan(got3[0, 0]).all() and torch.equal(got3[1:], got[1:])
+    # (fp16 steps are relative to the largest scale among a step's keys, the masked one's too: a last place may move)
+    assert torch.allclose(got3[0, 1:].float(), got[0, 1:].float(), rtol=2.0 ** -7, atol=2.0 ** -9)
+
+
+def test_tree_attention_rows_that_see_nothing():
+    from noise_b200 import decode
+    cache, table = _cache('e4m3', 64, 1, 16, 2, 32)
+    q, k, v = (torch.randn(2, 2, 1, 64, generator=_gen(h)).to(torch.bfloat16).to(DEV) for h in range(3))
+    mask = torch.tensor([[0, 2], [1, 0]], device=DEV)
+    depth = torch.zeros(2, 2, dtype=torch.int32, device=DEV)
+    got = decode.tree_attention(q, k, v, cache, table, torch.tensor([0, -5], dtype=torch.int32, device=DEV), mask, depth)
+    assert (got[0, 0] == 0).all() and (got[1, 1] == 0).all()
+    assert torch.equal(got[0, 1], v[0, 1]) and torch.equal(got[1, 0], v[1, 0])
+    none = decode.tree_attention(q[:0], k[:0], v[:0], cache, table[:0], torch.zeros(0, dtype=torch.int32, device=DEV),
+                                 mask[:0], depth[:0])
+    assert none.shape == (0, 2, 1, 64)
+
+
+def test_tree_attention_bad_page():
+    from noise_b200 import decode
+    from noise_b200._lib import NoiseError
+    cache, table = _cache('int8', 64, 1, 16, 2, 32)
+    q, k, v = (torch.randn(2, 1, 1, 64, generator=_gen(h)).to(torch.bfloat16).to(DEV) for h in range(3))
+    mask, depth = decode.tree_plan(torch.full((2, 1), -1, dtype=torch.int32, device=DEV))
+    table[1, 1] = -3
+    got = decode.tree_attention(q, k, v, cache, table, torch.tensor([32, 32], dtype=torch.int32, device=DEV), mask, depth)
+    assert torch.isfinite(got[0]).all() and torch.isnan(got[1]).all()
+    with pytest.raises(NoiseError, match='out of range'):
+        cache.check()
+
+
+@pytest.mark.parametrize('kind', ['e4m3', 'int8'])
+@pytest.mark.parametrize('size', [2.0 ** -60, 2.0 ** 60])
+def test_tree_attention_sizes_of_values(kind, size):
+    """V and Q of any size: the output scales with V, and the fp16 steps keep their precision."""
+    from noise_b200 import decode
+    g = _gen(2)
+    cache, table = _cache(kind, 64, 1, 16, 1, 320)
+    k, v = (torch.randn(300, 1, 64, generator=g).to(torch.bfloat16).to(DEV) for _ in range(2))
+    seq, pos = torch.zeros(300, dtype=torch.int32, device=DEV), torch.arange(300, dtype=torch.int32, device=DEV)
+    qt, kt, vt = (torch.randn(1, 2, 1, 64, generator=g).to(torch.bfloat16).to(DEV) for _ in range(3))
+    mask, depth = decode.tree_plan(torch.tensor([[-1, 0]], dtype=torch.int32, device=DEV))
+    lengths = torch.tensor([300], dtype=torch.int32, device=DEV)
+    # V alone large; Q small and K large by the same factor
+    for vs, qs in ((max(size, 2.0 ** -12), 1.0), (1.0, min(size, 2.0 ** 40))):
+        kk, vv = k / qs, v * vs
+        cache.write(kk, vv, seq, pos, table)
+        past = [x.cpu() for x in cache.read(seq, pos, table, dtype=torch.float32)]
+        got = decode.tree_attention(qt * qs, kt / qs, vt * vs, cache, table, lengths, mask, depth)
+        _check(got, qt * qs, kt / qs, vt * vs, [past], [oracle.tree_plan([-1, 0])])
+
+
+def test_offsets_past_32_bits():
+    """A cache of more than 2^32 bytes of codes: the last pages are written, read and attended over."""
+    from noise_b200 import decode
+    g = _gen(6)
+    cache = decode.KVCache(2, 2100, 16, 128, 'int8', 512, DEV)  # 2 x 2.2e9 codes each of K and V
+    assert cache.k.numel() > 2 ** 32
+    table = torch.tensor([[2099, 2098]], dtype=torch.int32, device=DEV)
+    n = 600
+    k, v = (torch.randn(n, 16, 128, generator=g).to(torch.bfloat16).to(DEV) for _ in range(2))
+    seq, pos = torch.zeros(n, dtype=torch.int32, device=DEV), torch.arange(n, dtype=torch.int32, device=DEV)
+    cache.write(k, v, seq, pos, table, layer=1)
+    got = cache.read(seq, pos, table, layer=1, dtype=torch.float32)
+    sample = torch.arange(0, n, 37)
+    for x, y in zip((k, v), got):
+        assert torch.equal(oracle.quantised(x[sample].cpu(), 'int8'), y[sample].cpu().double())
+    q, kt, vt = (torch.randn(1, 1, 16, 128, generator=g).to(torch.bfloat16).to(DEV) for _ in range(3))
+    mask, depth = decode.tree_plan(torch.full((1, 1), -1, dtype=torch.int32, device=DEV))
+    out = decode.tree_attention(q, kt, vt, cache, table, torch.tensor([n], dtype=torch.int32, device=DEV), mask, depth,
+                                layer=1)
+    _check(out, q, kt, vt, [[x.cpu() for x in got]], [oracle.tree_plan([-1])])
+    assert (cache.k[0, :2].view(torch.uint8) == 0).all()
+
+
+def test_other_stream_and_layouts():
+    """Calls on a side stream after work on it; q, k and v in a transposed order and off the 8-byte grid."""
+    from noise_b200 import decode
+    g = _gen(9)
+    cache, table = _cache('e4m3', 64, 2, 16, 2, 64)
+    past = _fill(cache, table, [50, 20], g)
+    mask, depth = decode.tree_plan(torch.tensor([[-1, 0, 1]] * 2, dtype=torch.int32, device=DEV))
+    lengths = torch.tensor([50, 20], dtype=torch.int32, device=DEV)
+    base = torch.randn(2, 2, 3, 67, generator=g).to(torch.bfloat16).to(DEV)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(2_000_000)
+        x = (base * 1.5)[..., 3:].transpose(1, 2)  # [B, N, heads, D]
+        got = decode.tree_attention(x, x, x, cache, table, lengths, mask, depth)
+    side.synchronize()
+    _check(got, x, x, x, past, [oracle.tree_plan([-1, 0, 1])] * 2)
+
+
+# ---- verification ---------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('nodes,vocab,branch,drawn,temperature,softcap', [
+    (1, 7, 1, True, 1.0, 0.0), (5, 4096, 1, True, 1.0, 15.0), (16, 1001, 3, True, 0.7, 0.0), (64, 50, 2, False, 1.3, 0.0),
+    (9, 9001, 2, True, 1.0, 0.0), (31, 33333, 3, False, 0.5, 15.0), (12, 70001, 2, True, 1.0, 0.0),
+    (20, 3000, 3, True, 0.0, 15.0), (7, 20001, 2, False, 0.0, 0.0), (4, 1, 2, True, 1.0, 0.0)])
+def test_verify_tree(dtype, nodes, vocab, branch, drawn, temperature, softcap):
+    from noise_b200 import decode
+    seqs, g = 40, _gen(nodes * vocab)
+    draft = 2 * torch.randn(seqs, nodes, vocab, generator=g)
+    logits = (draft + 0.5 * torch.randn(seqs, nodes, vocab, generator=g)).to(dtype)
+    probs = draft.softmax(-1)
+    parents = torch.tensor([[-1] + [(i - 1) // branch for i in range(1, nodes)]] * seqs, dtype=torch.int32)
+    if nodes > 6:
+        parents[3:6, 4] = -2
+        parents[7, 5] = 5  # not an earlier node: never reached
+    at = parents.clamp(min=0).long()
+    rows = torch.gather(probs if temperature > 0 else (logits.float() * 4).softmax(-1), 1, at[..., None].expand(-1, -1, vocab))
+    tokens = torch.multinomial(rows.reshape(-1, vocab), 1, generator=g).view(seqs, nodes)
+    if nodes > 6:
+        tokens[9, 1], tokens[10, 1] = -1, vocab  # no tokens: never accepted
+    u, race = torch.rand(seqs, nodes, generator=g), torch.empty(seqs, vocab).exponential_(generator=g)
+    dev = [x.to(DEV) for x in (logits, tokens, parents, u, race)]
+    count, path, token = decode.verify_tree(*dev, probs=probs.to(DEV) if drawn else None, temperature=temperature,
+                                            softcap=softcap)
+    close = 0
+    for b in range(seqs):
+        ref = oracle.verify_tree(logits[b], tokens[b], parents[b].tolist(), u[b], race[b], probs[b] if drawn else None,
+                                 temperature, softcap)
+        if ref[3] < 1e-4:
+            close += 1
+            continue
+        assert (count[b].item(), path[b].tolist(), token[b].item()) == ref[:3], b
+    assert close <= 4
+    again = decode.verify_tree(*dev, probs=probs.to(DEV) if drawn else None, temperature=temperature, softcap=softcap)
+    assert all(torch.equal(x, y) for x, y in zip((count, path, token), again))
+    # views: logits and probs inside wider rows
+    wide = torch.zeros(seqs, nodes, vocab + 3, dtype=dtype, device=DEV)
+    wide[..., 1:vocab + 1] = dev[0]
+    again = decode.verify_tree(wide[..., 1:vocab + 1], *dev[1:], probs=probs.to(DEV) if drawn else None,
+                               temperature=temperature, softcap=softcap)
+    assert all(torch.equal(x, y) for x, y in zip((count, path, token), again))
+
+
+@pytest.mark.parametrize('drawn', [True, False])
+def test_verified_tokens_are_distributed_as_the_targets(drawn):
+    """The first token of 2^16 walks over two drafts at the root: each frequency within 5 standard deviations."""
+    from noise_b200 import decode
+    n, vocab, g = 1 << 16, 6, torch.Generator(DEV).manual_seed(3)
+    logits = torch.tensor([1.0, -0.5, 0.3, -2.0, 0.0, 0.8], device=DEV).expand(n, 3, vocab)
+    q = torch.tensor([0.05, 0.4, 0.1, 0.2, 0.05, 0.2], device=DEV).expand(n, 3, vocab)
+    if drawn:
+        kids = torch.multinomial(q[:, 0], 2, replacement=True, generator=g)
+    else:
+        kids = torch.tensor([[0, 5]], device=DEV).expand(n, 2)
+    tokens = torch.cat([torch.zeros(n, 1, dtype=torch.int64, device=DEV), kids], 1)
+    parents = torch.tensor([[-1, 0, 0]], dtype=torch.int32, device=DEV).repeat(n, 1)
+    u = torch.rand(n, 3, device=DEV, generator=g)
+    race = torch.empty(n, vocab, device=DEV).exponential_(generator=g)
+    count, path, token = decode.verify_tree(logits, tokens, parents, u, race, probs=q if drawn else None)
+    first = torch.where(count > 0, tokens.gather(1, path[:, 1:2].clamp(min=0).long())[:, 0], token)
+    p = logits[0, 0].double().softmax(-1).cpu()
+    share = torch.bincount(first, minlength=vocab).double().cpu() / n
+    assert ((share - p).abs() <= 5 * (p * (1 - p) / n).sqrt()).all(), (share, p)
+    assert 0.2 < (count > 0).double().mean().item() < 0.95
+
+
+def test_verify_special_logits():
+    """-inf logits are never drawn; nothing but -inf names token 0 when greedy; the draft's own distribution is accepted."""
+    from noise_b200 import decode
+    z = torch.full((3, 2, 300), -math.inf, device=DEV)
+    z[0, :, 17] = 1.0
+    z[1, :, :] = torch.randn(300, generator=_gen(1)).to(DEV)
+    tokens = torch.tensor([[0, 17], [0, 5], [0, 0]], device=DEV)
+    parents = torch.tensor([[-1, 0]] * 3, dtype=torch.int32, device=DEV)
+    probs = z.softmax(-1).nan_to_num()
+    u, race = torch.full((3, 2), 0.999, device=DEV), torch.ones(3, 300, device=DEV)
+    count, path, token = decode.verify_tree(z, tokens, parents, u, race, probs)
+    assert count[:2].tolist() == [1, 1] and path[:2].tolist() == [[0, 1], [0, 1]] and token[0].item() == 17
+    assert token[1].item() == z[1, 1].argmax().item()
+    count, _, token = decode.verify_tree(z, tokens, parents, None, None, temperature=0.0)
+    assert count[0].item() == 1 and token[2].item() == 0
+
+
+# ---- refusals -------------------------------------------------------------------------------------------------
+
+
+def test_refusals():
+    from noise_b200 import decode
+    from noise_b200._lib import NoiseError
+    cos, sin = _tables(4, 64)
+    q = torch.zeros(3, 2, 64, device=DEV)
+    pos = torch.zeros(3, dtype=torch.int32, device=DEV)
+    bad = [
+        (TypeError, lambda: decode.head_norm_rope(q.half(), q.half(), cos, sin, pos)),
+        (TypeError, lambda: decode.head_norm_rope(q, q, cos, sin, pos.long())),
+        (TypeError, lambda: decode.head_norm_rope(q, q, cos, sin, pos, q_weight=torch.ones(64, device=DEV).bfloat16())),
+        (ValueError, lambda: decode.head_norm_rope(q, q[:2], cos, sin, pos)),
+        (ValueError, lambda: decode.head_norm_rope(q, q, cos[:, :31], sin, pos)),
+        (ValueError, lambda: decode.head_norm_rope(q, q, cos, sin, pos, eps=-1.0)),
+        (ValueError, lambda: decode.head_norm_rope(q.transpose(1, 2), q, cos, sin, pos)),
+        (ValueError, lambda: decode.head_norm_rope(q, q, cos, sin, pos, k_weight=torch.ones(32, device=DEV))),
+        (NoiseError, lambda: decode.head_norm_rope(q.cpu(), q, cos, sin, pos)),
+        (ValueError, lambda: decode.head_norm_rope_backward(q, q[:, :1], q, q, cos, sin, pos)),
+        (ValueError, lambda: decode.KVCache(1, 4, 2, 64, 'fp4')),
+        (ValueError, lambda: decode.KVCache(1, 4, 2, 72)),
+        (ValueError, lambda: decode.KVCache(1, 4, 2, 64, page_size=48)),
+        (TypeError, lambda: decode.KVCache.of(torch.zeros(1, 1, 1, 16, 64, device=DEV), torch.zeros(1, 1, 1, 4, 64, 4, device=DEV))),
+        (ValueError, lambda: decode.KVCache.of(torch.zeros(1, 1, 1, 16, 64, dtype=torch.int8, device=DEV),
+                                               torch.zeros(1, 1, 1, 4, 64, 4, dtype=torch.int8, device=DEV))),
+    ]
+    cache, table = _cache('e4m3', 64, 2, 16, 3, 32)
+    kv = torch.zeros(3, 2, 64, device=DEV)
+    bad += [
+        (ValueError, lambda: cache.write(kv[:, :1], kv[:, :1], pos, pos, table)),
+        (ValueError, lambda: cache.write(kv[:2], kv[:2], pos, pos, table)),
+        (ValueError, lambda: cache.write(kv, kv, pos, pos, table, layer=1)),
+        (ValueError, lambda: cache.write(kv, kv, pos, pos, table, layer=None)),
+        (TypeError, lambda: cache.write(kv, kv, pos, pos.long(), table)),
+        (TypeError, lambda: cache.read(pos, pos, table, dtype=torch.float16)),
+        (ValueError, lambda: cache.read(pos, pos, table[0])),
+    ]
+    x = torch.zeros(3, 2, 2, 64, dtype=torch.bfloat16, device=DEV)
+    parents = torch.tensor([[-1, 0]] * 3, dtype=torch.int32, device=DEV)
+    mask, depth = decode.tree_plan(parents)
+    attend = lambda **kw: decode.tree_attention(**dict(dict(  # noqa: E731
+        q=x, k=x, v=x, cache=cache, table=table, lengths=pos, mask=mask, depth=depth), **kw))
+    bad += [
+        (TypeError, lambda: attend(q=x.float())),
+        (TypeError, lambda: attend(mask=mask.int())),
+        (ValueError, lambda: attend(q=torch.cat([x, x[:, :, :1]], 2))),
+        (ValueError, lambda: attend(k=x[:, :1])),
+        (ValueError, lambda: attend(table=table[:2])),
+        (ValueError, lambda: attend(layer=2)),
+        (ValueError, lambda: attend(lengths=pos[:2])),
+        (NoiseError, lambda: attend(scale=0.0)),
+        (NoiseError, lambda: attend(scale=math.nan)),
+        (ValueError, lambda: decode.tree_plan(torch.zeros(1, 65, dtype=torch.int32, device=DEV))),
+    ]
+    z = torch.zeros(3, 2, 9, device=DEV)
+    tokens, u, race = torch.zeros(3, 2, dtype=torch.int64, device=DEV), torch.zeros(3, 2, device=DEV), torch.ones(3, 9, device=DEV)
+    bad += [
+        (TypeError, lambda: decode.verify_tree(z.half(), tokens, parents, u, race)),
+        (TypeError, lambda: decode.verify_tree(z, tokens.int(), parents, u, race)),
+        (ValueError, lambda: decode.verify_tree(z, tokens, parents, u, race[:, :8])),
+        (ValueError, lambda: decode.verify_tree(z, tokens, parents, u, race, temperature=-1.0)),
+        (ValueError, lambda: decode.verify_tree(z, tokens, parents, u, race, softcap=math.inf)),
+        (ValueError, lambda: decode.verify_tree(z, tokens, parents, u, race, probs=z[:, :1])),
+    ]
+    for kind, call in bad:
+        with pytest.raises(kind):
+            call()
+    cache.check()

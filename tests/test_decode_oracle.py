@@ -1,0 +1,102 @@
+"""The decode operators on the CPU: the oracle against torch's own functions, and the C ABI's refusals before a launch."""
+import ctypes
+import math
+
+import torch
+
+from oracle import decode as oracle
+
+
+def test_head_norm_rope_gradient_is_the_forwards():
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(5, 3, 16, generator=g, dtype=torch.float64).requires_grad_()
+    w = (1 + 0.1 * torch.randn(16, generator=g, dtype=torch.float64)).requires_grad_()
+    angle = torch.randn(7, 8, generator=g, dtype=torch.float64)
+    pos = torch.tensor([0, 6, 3, 3, 1])
+    dy = torch.randn(x.shape, generator=g, dtype=torch.float64)
+    y = oracle.head_norm_rope(x, angle.cos(), angle.sin(), pos, w)
+    dx, dw = torch.autograd.grad((y * dy).sum(), (x, w))
+    got = oracle.head_norm_rope_backward(dy, x.detach(), angle.cos(), angle.sin(), pos, w.detach())
+    assert torch.allclose(got[0], dx, rtol=1e-12, atol=1e-13) and torch.allclose(got[1], dw, rtol=1e-12, atol=1e-13)
+
+
+def test_quantised_is_torchs_e4m3_under_the_scale():
+    x = torch.randn(20, 32, generator=torch.Generator().manual_seed(1)) * torch.exp2(torch.arange(-10, 10).float())[:, None]
+    for i, row in enumerate(x):
+        e = oracle.scale_exponent(row.abs().max().item(), 'e4m3')
+        assert row.abs().max().item() <= 448 * 2.0 ** e and row.abs().max().item() > 448 * 2.0 ** (e - 1)
+        ref = (row * 2.0 ** -e).to(torch.float8_e4m3fn).double() * 2.0 ** e
+        assert torch.equal(oracle.quantised(row[None], 'e4m3')[0], ref)
+    assert torch.isnan(oracle.quantised(torch.tensor([[1.0, math.nan]]), 'int8')).all()
+    assert oracle.scale_exponent(127.0, 'int8') == 0 and oracle.scale_exponent(127.5, 'int8') == 1
+
+
+def test_tree_attention_of_a_chain_is_causal_attention():
+    from oracle import gpt
+    g = torch.Generator().manual_seed(2)
+    q, k, v = (torch.randn(12, 2, 64, generator=g, dtype=torch.float64) for _ in range(3))
+    mask, depth = oracle.tree_plan([-1, 0, 1, 2, 3])
+    for window in (4, 100):
+        ref = gpt.attention(q[None], k[None], v[None], window)[0, 7:]
+        got, _ = oracle.tree_attention(q[7:], k[7:], v[7:], k[:7], v[:7], mask, depth, window)
+        assert torch.allclose(got, ref, atol=1e-12)
+
+
+def test_verification_keeps_the_targets_distribution():
+    """Over a grid of random numbers the first token's shares are the target's."""
+    z = torch.tensor([0.3, -1.0, 0.9])
+    p, q = z.double().softmax(-1), torch.tensor([0.6, 0.3, 0.1])
+    share = torch.zeros(3, dtype=torch.float64)
+    g = torch.Generator().manual_seed(4)
+    n = 4000
+    for _ in range(n):
+        kid = int(torch.multinomial(q, 1, generator=g))
+        count, path, token, _ = oracle.verify_tree(z.expand(2, 3), [0, kid], [-1, 0], torch.rand(2, generator=g),
+                                                   torch.empty(3).exponential_(generator=g), q.expand(2, 3))
+        share[kid if count else token] += 1 / n
+    assert ((share - p).abs() < 5 * (p * (1 - p) / n).sqrt()).all()
+
+
+def test_the_abi_refuses_before_a_launch():
+    from noise_b200 import _lib
+    L, fake = _lib.lib(), 256  # never dereferenced
+    heads = ctypes.byref(_lib.Heads(fake, 128, 64, 2))
+    norm = lambda dim=64, dtype=1, tokens=4, rows=8, eps=1e-6, q=heads: L.noise_head_norm_rope(  # noqa: E731
+        q, heads, fake, fake, 1, rows, fake, tokens, dim, dtype, None, None, eps, fake, fake, None)
+    assert norm(dim=63) == 1 and norm(dim=258) == 1 and norm(tokens=-1) == 1 and norm(rows=0) == 1
+    assert norm(dtype=2) == 4 and norm(eps=math.nan) == 4 and norm(q=None) == 4
+    assert norm(tokens=0) == 0
+    assert norm(q=ctypes.byref(_lib.Heads(None, 128, 64, 2))) == 4
+    back = lambda ws, n, dk=heads: L.noise_head_norm_rope_backward(  # noqa: E731
+        heads, dk, heads, heads, fake, fake, 1, 8, fake, 4, 64, 1, fake, None, 1e-6, fake, fake, fake, None, ws, n, None)
+    assert L.noise_head_norm_rope_backward_workspace_bytes(64) > 0
+    assert L.noise_head_norm_rope_backward_workspace_bytes(300) == 0
+    assert back(None, 1 << 30) == 3 and back(fake, 16) == 3 and back(fake + 4, 1 << 30) == 2
+    assert back(fake, 1 << 30, ctypes.byref(_lib.Heads(fake, 128, 64, 3))) == 4  # dk has other heads than k
+    def cache(**kw):
+        f = dict(k=fake, v=fake, k_scale=fake, v_scale=fake, status=fake, layers=2, pages=4, heads=2, page_size=64, dim=64,
+                 kind=1)
+        f.update(kw)
+        return ctypes.byref(_lib.KVCache(**f))
+    write = lambda c, layer=0, layers=1, tokens=4, dtype=1: L.noise_kv_write(  # noqa: E731
+        c, layer, layers, fake, 0, 128, 64, fake, 0, 128, 64, 4, dtype, tokens, fake, fake, None, fake, 2, 3, None)
+    assert write(cache(kind=3)) == 4 and write(cache(k_scale=None)) == 4 and write(cache(status=None)) == 4
+    assert write(cache(page_size=48)) == 1 and write(cache(dim=24)) == 1 and write(cache(v=fake + 8)) == 2
+    assert write(cache(), layer=1, layers=2) == 1 and write(cache(), layer=-1) == 1 and write(cache(), tokens=-1) == 1
+    assert write(cache(), dtype=5) == 4 and write(cache(), tokens=0) == 0
+    read = lambda c, out=fake: L.noise_kv_read(c, 0, 1, out, out, 1, 4, fake, fake, fake, 2, 3, None)  # noqa: E731
+    assert read(cache(), None) == 4 and read(cache(), fake + 2) == 2
+    attend = lambda c, layer=0, nodes=4, qh=4, scale=0.1, ws=fake, n=16, stride=64, q=fake, seqs=2: (  # noqa: E731
+        L.noise_tree_attention(c, layer, q, 1024, 256, stride, qh, fake, 512, 128, 64, fake, 512, 128, 64, seqs, nodes,
+                               fake, 3, fake, fake, fake, -1, scale, fake, ws, n, None))
+    assert attend(cache(dim=32)) == 1 and attend(cache(), layer=2) == 1 and attend(cache(), nodes=65) == 1
+    assert attend(cache(), qh=3) == 1 and attend(cache(), scale=-1.0) == 4 and attend(cache(), scale=math.inf) == 4
+    assert attend(cache(), ws=None) == 3 and attend(cache(), stride=66) == 2
+    assert attend(cache(), q=fake + 4) == 2 and attend(cache(), seqs=0) == 0 and attend(cache(), seqs=5000) == 1
+    assert L.noise_tree_attention_workspace_bytes(2, 4, 4, 2, 64) > 0
+    assert L.noise_tree_attention_workspace_bytes(2, 4, 4, 2, 32) == 0
+    assert L.noise_tree_plan(fake, 2, 65, fake, fake, None) == 1 and L.noise_tree_plan(None, 2, 4, fake, fake, None) == 4
+    verify = lambda vocab=100, nodes=4, t=1.0, cap=0.0, u=fake, seqs=2: L.noise_verify_tree(  # noqa: E731
+        fake, 0, 400, 100, fake, fake, u, fake, None, 0, 0, seqs, nodes, vocab, t, cap, fake, fake, fake, None)
+    assert verify(vocab=0) == 1 and verify(vocab=400000) == 1 and verify(nodes=65) == 1 and verify(t=-1.0) == 4
+    assert verify(t=math.nan) == 4 and verify(cap=-2.0) == 4 and verify(u=None) == 4 and verify(seqs=0) == 0
