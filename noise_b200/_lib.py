@@ -316,7 +316,10 @@ def check(status, what):
 
 
 def stream_handle(device=None):
-    return torch.cuda.current_stream(device).cuda_stream
+    index = getattr(device, 'index', None)
+    if index is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(index)  # the same handle, without the Stream object around it
 
 
 def require_cuda(*tensors):

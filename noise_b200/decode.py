@@ -15,7 +15,7 @@ prompt. A step takes a tree of up to 64 tokens a sequence: the last sampled toke
 Each call runs on the current stream of its tensors' device, allocates with torch and reads nothing back. Arguments are
 checked before a pointer reaches the library (TypeError for a dtype, ValueError for a shape, layout or device).
 """
-import ctypes
+import functools
 import math
 
 import torch
@@ -23,9 +23,11 @@ import torch
 from . import _lib
 
 MAX_NODES = 64
+MAX_VOCAB = 393216
 KINDS = {'bf16': 0, 'e4m3': 1, 'int8': 2}
 CODES = {'bf16': torch.bfloat16, 'e4m3': torch.float8_e4m3fn, 'int8': torch.int8}
 DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+EPS = {t: torch.finfo(t).eps for t in DTYPES}  # F.rms_norm's
 
 
 def _need(ok, message):
@@ -33,74 +35,76 @@ def _need(ok, message):
         raise ValueError(message)
 
 
-def _rows(name, t, dims, device=None):
+def _rows(name, t, dims, device):
     """The checks every floating operand of ``dims`` dimensions gets; the last dimension is contiguous."""
     if t.dim() != dims or (t.stride(-1) != 1 and t.shape[-1] > 1):
         raise ValueError(f'{name}: {dims} dimensions, the last one contiguous; got {tuple(t.shape)}, strides {t.stride()}')
-    if device is not None and t.device != device:
+    if t.device != device:
         raise ValueError(f'{name}: on {t.device}, expected {device}')
 
 
 def _ints(name, t, dtype, shape, device):
     if t.dtype != dtype:
         raise TypeError(f'{name}: {dtype}, got {t.dtype}')
-    if tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
-        raise ValueError(f'{name}: contiguous {shape} on {device}, got {tuple(t.shape)} on {t.device}')
+    if t.shape != shape or not t.is_contiguous() or t.device != device:
+        raise ValueError(f'{name}: contiguous {tuple(shape)} on {device}, got {tuple(t.shape)} on {t.device}')
 
 
-class _On:
-    """The device's current stream handle, with the device current while the call is made."""
-
-    def __init__(self, device):
-        self.device = device
-        self.guard = torch.cuda.device(device) if torch.cuda.current_device() != device.index else None
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return _lib.stream_handle(self.device)
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-        return False
+def _call(name, device, *args):
+    """The entry point on the device's current stream, with the device current."""
+    fn = getattr(_lib.lib(), name)
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, _lib.stream_handle(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, _lib.stream_handle(device))
+    if rc:
+        _lib.check(rc, name)
 
 
 # ---- head norm and rotation -----------------------------------------------------------------------------------
 
 
 def _head_args(q, k, cos, sin, positions, q_weight, k_weight, eps):
+    """The checks of both directions; (tokens, D, the arguments that both calls share)."""
     _lib.require_cuda(q, k, cos, sin, positions)
-    dev = q.device
-    if q.dtype not in DTYPES or k.dtype != q.dtype:
-        raise TypeError(f'q and k: fp32 or bf16, alike; got {q.dtype}, {k.dtype}')
-    if cos.dtype not in DTYPES or sin.dtype != cos.dtype:
-        raise TypeError(f'cos and sin: fp32 or bf16, alike; got {cos.dtype}, {sin.dtype}')
-    _rows('q', q, 3)
+    dev, dtype, table = q.device, q.dtype, cos.dtype
+    if dtype not in DTYPES or k.dtype != dtype:
+        raise TypeError(f'q and k: fp32 or bf16, alike; got {dtype}, {k.dtype}')
+    if table not in DTYPES or sin.dtype != table:
+        raise TypeError(f'cos and sin: fp32 or bf16, alike; got {table}, {sin.dtype}')
+    _rows('q', q, 3, dev)
     _rows('k', k, 3, dev)
-    tokens, heads, dim = q.shape
-    _need(k.shape[0] == tokens and k.shape[2] == dim, f'q [tokens, heads, D] and k [tokens, k heads, D]: got '
-          f'{tuple(q.shape)}, {tuple(k.shape)}')
-    _need(2 <= dim <= 256 and dim % 2 == 0, f'D: even, 2 to 256; got {dim}')
-    _need(0 < heads <= 4096 and 0 < k.shape[1] <= 4096, 'heads: 1 to 4096')
-    _need(cos.dim() == 2 and cos.shape == sin.shape and cos.shape[1] == dim // 2 and cos.shape[0] > 0 and
-          cos.is_contiguous() and sin.is_contiguous() and cos.device == dev and sin.device == dev,
-          f'cos, sin: contiguous [positions, {dim // 2}] on {dev}, got {tuple(cos.shape)}, {tuple(sin.shape)}')
+    (tokens, heads, dim), (k_tokens, k_heads, k_dim) = q.shape, k.shape
+    if k_tokens != tokens or k_dim != dim:
+        raise ValueError(f'q [tokens, heads, D], k [tokens, k heads, D]: got {tuple(q.shape)}, {tuple(k.shape)}')
+    if dim < 2 or dim > 256 or dim % 2:
+        raise ValueError(f'D: even, 2 to 256; got {dim}')
+    if not (0 < heads <= 4096 and 0 < k_heads <= 4096):
+        raise ValueError(f'heads: 1 to 4096; got {heads}, {k_heads}')
+    shape = cos.shape
+    if (len(shape) != 2 or shape[1] * 2 != dim or shape[0] < 1 or sin.shape != shape or not cos.is_contiguous() or
+            not sin.is_contiguous() or cos.device != dev or sin.device != dev):
+        raise ValueError(f'cos, sin: contiguous [positions, {dim // 2}] on {dev}, got {tuple(shape)}, {tuple(sin.shape)}')
     _ints('positions', positions, torch.int32, (tokens,), dev)
-    for name, w in (('q_weight', q_weight), ('k_weight', k_weight)):
+    weights = [None, None]
+    for i, w in enumerate((q_weight, k_weight)):
         if w is not None:
-            if w.dtype != q.dtype:
-                raise TypeError(f'{name}: {q.dtype}, got {w.dtype}')
-            _need(tuple(w.shape) == (dim,) and w.is_contiguous() and w.device == dev,
-                  f'{name}: contiguous [{dim}] on {dev}, got {tuple(w.shape)}')
-    if eps is None:
-        eps = torch.finfo(q.dtype).eps
-    _need(math.isfinite(eps) and eps >= 0, f'eps: {eps}')
-    return tokens, dim, float(eps)
+            name = 'qk'[i] + '_weight'
+            if w.dtype != dtype:
+                raise TypeError(f'{name}: {dtype}, got {w.dtype}')
+            if w.shape != (dim,) or not w.is_contiguous() or w.device != dev:
+                raise ValueError(f'{name}: contiguous [{dim}] on {dev}, got {tuple(w.shape)} on {w.device}')
+            weights[i] = w.data_ptr()
+    eps = EPS[dtype] if eps is None else float(eps)
+    if not 0 <= eps < math.inf:
+        raise ValueError(f'eps: {eps}')
+    return (_heads(q), _heads(k), cos.data_ptr(), sin.data_ptr(), DTYPES[table], shape[0], positions.data_ptr(),
+            tokens, dim, DTYPES[dtype], *weights, eps)
 
 
 def _heads(t):
-    return ctypes.byref(_lib.Heads(t.data_ptr(), t.stride(0), t.stride(1), t.shape[1]))
+    return _lib.Heads(t.data_ptr(), t.stride(0), t.stride(1), t.shape[1])
 
 
 def _ptr(t):
@@ -108,41 +112,33 @@ def _ptr(t):
 
 
 def _head_forward(q, k, cos, sin, positions, q_weight, k_weight, eps):
-    tokens, dim, eps = _head_args(q, k, cos, sin, positions, q_weight, k_weight, eps)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = torch.empty(k.shape, dtype=q.dtype, device=q.device)
-    with _On(q.device) as stream:
-        _lib.check(_lib.lib().noise_head_norm_rope(
-            _heads(q), _heads(k), cos.data_ptr(), sin.data_ptr(), DTYPES[cos.dtype], cos.shape[0],
-            positions.data_ptr(), tokens, dim, DTYPES[q.dtype], _ptr(q_weight), _ptr(k_weight), eps,
-            q_out.data_ptr(), k_out.data_ptr(), stream), 'noise_head_norm_rope')
+    args = _head_args(q, k, cos, sin, positions, q_weight, k_weight, eps)
+    q_out, k_out = q.new_empty(q.shape), k.new_empty(k.shape)
+    _call('noise_head_norm_rope', q.device, *args, q_out.data_ptr(), k_out.data_ptr())
     return q_out, k_out
 
 
 def head_norm_rope_backward(dq, dk, q, k, cos, sin, positions, q_weight=None, k_weight=None, eps=None):
     """Gradient of ``head_norm_rope``: (q's, k's, q_weight's, k_weight's) from the outputs' gradients dq, dk and the call's
     own arguments. The weights' are fp32 [D], summed over tokens and heads in a fixed order, None without a weight."""
-    tokens, dim, eps = _head_args(q, k, cos, sin, positions, q_weight, k_weight, eps)
-    dev = q.device
-    for name, d, x in (('dq', dq, q), ('dk', dk, k)):
-        if d.dtype != q.dtype:
-            raise TypeError(f'{name}: {q.dtype}, got {d.dtype}')
-        _rows(name, d, 3, dev)
-        _need(d.shape == x.shape, f'{name}: {tuple(x.shape)}, got {tuple(d.shape)}')
-    gq = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    gk = torch.empty(k.shape, dtype=q.dtype, device=dev)
+    args = _head_args(q, k, cos, sin, positions, q_weight, k_weight, eps)
+    _lib.require_cuda(dq, dk)
+    dev, dim = q.device, q.shape[2]
+    if dq.dtype != q.dtype or dk.dtype != q.dtype:
+        raise TypeError(f'dq and dk: {q.dtype}, got {dq.dtype}, {dk.dtype}')
+    _rows('dq', dq, 3, dev)
+    _rows('dk', dk, 3, dev)
+    if dq.shape != q.shape or dk.shape != k.shape:
+        raise ValueError(f'dq, dk: {tuple(q.shape)}, {tuple(k.shape)}; got {tuple(dq.shape)}, {tuple(dk.shape)}')
+    gq, gk = q.new_empty(q.shape), k.new_empty(k.shape)
     gqw = None if q_weight is None else torch.empty(dim, dtype=torch.float32, device=dev)
     gkw = None if k_weight is None else torch.empty(dim, dtype=torch.float32, device=dev)
-    L, nbytes, ws = _lib.lib(), 0, None
+    nbytes, ws = 0, None
     if gqw is not None or gkw is not None:
-        nbytes = L.noise_head_norm_rope_backward_workspace_bytes(dim)
+        nbytes = _lib.lib().noise_head_norm_rope_backward_workspace_bytes(dim)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    with _On(dev) as stream:
-        _lib.check(L.noise_head_norm_rope_backward(
-            _heads(dq), _heads(dk), _heads(q), _heads(k), cos.data_ptr(), sin.data_ptr(), DTYPES[cos.dtype],
-            cos.shape[0], positions.data_ptr(), tokens, dim, DTYPES[q.dtype], _ptr(q_weight), _ptr(k_weight), eps,
-            gq.data_ptr(), gk.data_ptr(), _ptr(gqw), _ptr(gkw), _ptr(ws), nbytes, stream),
-            'noise_head_norm_rope_backward')
+    _call('noise_head_norm_rope_backward', dev, _heads(dq), _heads(dk), *args, gq.data_ptr(), gk.data_ptr(),
+          _ptr(gqw), _ptr(gkw), _ptr(ws), nbytes)
     return gq, gk, gqw, gkw
 
 
@@ -235,66 +231,68 @@ class KVCache:
             _need(t.data_ptr() % 16 == 0, 'the cache\'s tensors: on 16-byte boundaries')
         self._struct = _lib.KVCache(k.data_ptr(), v.data_ptr(), _ptr(k_scale), _ptr(v_scale), self.status.data_ptr(),
                                     layers, pages, heads, page, dim, KINDS[self.kind])
-        self._ref = ctypes.byref(self._struct)
 
     def _places(self, seq, pos, table, layer):
-        tokens = seq.shape[0]
-        _ints('seq', seq, torch.int32, (tokens,), self.device)
-        _ints('pos', pos, torch.int32, (tokens,), self.device)
-        _need(table.dim() == 2, f'table: [sequences, pages], got {tuple(table.shape)}')
-        _ints('table', table, torch.int32, tuple(table.shape), self.device)
-        _need(layer is None or 0 <= layer < self.layers, f'layer: 0 to {self.layers - 1}, or None for all')
-        return tokens, (0, self.layers) if layer is None else (layer, 1)
+        _lib.require_cuda(seq, pos, table)
+        shape = seq.shape
+        if len(shape) != 1 or table.dim() != 2:
+            raise ValueError(f'seq [tokens], table [sequences, pages]: got {tuple(shape)}, {tuple(table.shape)}')
+        _ints('seq', seq, torch.int32, shape, self.device)
+        _ints('pos', pos, torch.int32, shape, self.device)
+        _ints('table', table, torch.int32, table.shape, self.device)
+        if layer is None:
+            return shape[0], 0, self.layers
+        if not 0 <= layer < self.layers:
+            raise ValueError(f'layer: 0 to {self.layers - 1}, or None for all; got {layer}')
+        return shape[0], layer, 1
 
     def write(self, k, v, seq, pos, table, layer=0, rows=None):
         """Write keys and values of token i at position pos[i] of sequence seq[i] (int32 [tokens]; negative: skipped).
 
         k, v [source rows, heads, D], fp32 or bf16, any strides but the last; entry i takes row rows[i] (int32 [tokens];
-        negative: skipped), or row i. layer None: all layers at once, k, v [layers, source rows, heads, D]. An entry out of range is
-        skipped and reported by ``check()``."""
-        _lib.require_cuda(k, v, seq, pos, table)
-        tokens, (first, layers) = self._places(seq, pos, table, layer)
+        negative: skipped), or row i. layer None: all layers at once, k, v [layers, source rows, heads, D]. An entry out
+        of range is skipped and reported by ``check()``."""
+        _lib.require_cuda(k, v)
+        tokens, first, layers = self._places(seq, pos, table, layer)
         if k.dtype not in DTYPES or v.dtype != k.dtype:
             raise TypeError(f'k and v: fp32 or bf16, alike; got {k.dtype}, {v.dtype}')
         dims = 4 if layer is None else 3
         _rows('k', k, dims, self.device)
         _rows('v', v, dims, self.device)
         source = k.shape[-3]
-        want = ((self.layers,) if layer is None else ()) + (source, self.heads, self.dim)
-        _need(tuple(k.shape) == want and tuple(v.shape) == want, f'k, v: {want}, got {tuple(k.shape)}, {tuple(v.shape)}')
-        if rows is None:
-            _need(source >= tokens, f'{tokens} tokens, but {source} rows')
-        else:
-            _ints('rows', rows, torch.int32, (tokens,), self.device)
-        with _On(self.device) as stream:
-            _lib.check(_lib.lib().noise_kv_write(
-                self._ref, first, layers, k.data_ptr(), k.stride(0) if dims == 4 else 0, k.stride(-3), k.stride(-2),
-                v.data_ptr(), v.stride(0) if dims == 4 else 0, v.stride(-3), v.stride(-2), source, DTYPES[k.dtype],
-                tokens, seq.data_ptr(), pos.data_ptr(), _ptr(rows), table.data_ptr(), table.shape[0], table.shape[1],
-                stream), 'noise_kv_write')
+        want = (self.layers, source, self.heads, self.dim) if layer is None else (source, self.heads, self.dim)
+        if k.shape != want or v.shape != want:
+            raise ValueError(f'k, v: {want}, got {tuple(k.shape)}, {tuple(v.shape)}')
+        if rows is not None:
+            _lib.require_cuda(rows)
+            _ints('rows', rows, torch.int32, seq.shape, self.device)
+            rows = rows.data_ptr()
+        elif source < tokens:
+            raise ValueError(f'{tokens} tokens, but {source} rows')
+        _call('noise_kv_write', self.device, self._struct, first, layers, k.data_ptr(), k.stride(0), k.stride(-3),
+              k.stride(-2), v.data_ptr(), v.stride(0), v.stride(-3), v.stride(-2), source, DTYPES[k.dtype], tokens,
+              seq.data_ptr(), pos.data_ptr(), rows, table.data_ptr(), table.shape[0], table.shape[1])
 
     def read(self, seq, pos, table, layer=0, dtype=torch.bfloat16):
         """(k, v) [tokens, heads, D] at those places, or [layers, ...] for layer None. bf16 holds every value of every kind
         exactly. Negative seq or pos: zeros; out of range: NaN."""
-        _lib.require_cuda(seq, pos, table)
-        tokens, (first, layers) = self._places(seq, pos, table, layer)
+        tokens, first, layers = self._places(seq, pos, table, layer)
         if dtype not in DTYPES:
             raise TypeError(f'dtype: fp32 or bf16, got {dtype}')
-        shape = ((layers,) if layer is None else ()) + (tokens, self.heads, self.dim)
-        k, v = (torch.empty(shape, dtype=dtype, device=self.device) for _ in range(2))
-        with _On(self.device) as stream:
-            _lib.check(_lib.lib().noise_kv_read(
-                self._ref, first, layers, k.data_ptr(), v.data_ptr(), DTYPES[dtype], tokens, seq.data_ptr(),
-                pos.data_ptr(), table.data_ptr(), table.shape[0], table.shape[1], stream), 'noise_kv_read')
+        shape = (layers, tokens, self.heads, self.dim) if layer is None else (tokens, self.heads, self.dim)
+        k = torch.empty(shape, dtype=dtype, device=self.device)
+        v = torch.empty(shape, dtype=dtype, device=self.device)
+        _call('noise_kv_read', self.device, self._struct, first, layers, k.data_ptr(), v.data_ptr(), DTYPES[dtype],
+              tokens, seq.data_ptr(), pos.data_ptr(), table.data_ptr(), table.shape[0], table.shape[1])
         return k, v
 
     def check(self):
         """Raise if a call since the last check met an index out of range (synchronises the current stream)."""
-        with _On(self.device) as stream:
+        with torch.cuda.device(self.device):
             code = _lib.read_status(self.status)
-            if code:
-                _lib.check(_lib.lib().noise_clear_status(self.status.data_ptr(), stream), 'noise_clear_status')
-                raise _lib.NoiseError(f'a cache call met a sequence, position, row or page out of range (status {code})')
+        if code:
+            _call('noise_clear_status', self.device, self.status.data_ptr())
+            raise _lib.NoiseError(f'a cache call met a sequence, position, row or page out of range (status {code})')
 
 
 # ---- the tree -------------------------------------------------------------------------------------------------
@@ -310,10 +308,13 @@ def tree_plan(parents):
     _ints('parents', parents, torch.int32, tuple(parents.shape), parents.device)
     mask = torch.empty(parents.shape, dtype=torch.int64, device=parents.device)
     depth = torch.empty(parents.shape, dtype=torch.int32, device=parents.device)
-    with _On(parents.device) as stream:
-        _lib.check(_lib.lib().noise_tree_plan(parents.data_ptr(), parents.shape[0], parents.shape[1],
-                                              mask.data_ptr(), depth.data_ptr(), stream), 'noise_tree_plan')
+    _call('noise_tree_plan', parents.device, parents.data_ptr(), *parents.shape, mask.data_ptr(), depth.data_ptr())
     return mask, depth
+
+
+@functools.lru_cache(maxsize=256)
+def _attention_bytes(*sizes):
+    return max(_lib.lib().noise_tree_attention_workspace_bytes(*sizes), 16)
 
 
 def tree_attention(q, k, v, cache, table, lengths, mask, depth, layer=0, window=-1, scale=None):
@@ -326,39 +327,44 @@ def tree_attention(q, k, v, cache, table, lengths, mask, depth, layer=0, window=
     (depth below 0) and of nodes that see nothing are 0."""
     _lib.require_cuda(q, k, v, table, lengths, mask, depth)
     dev = cache.device
-    for name, t in (('q', q), ('k', k), ('v', v)):
-        if t.dtype != torch.bfloat16:
-            raise TypeError(f'{name}: bf16, got {t.dtype}')
-        _rows(name, t, 4, dev)
-    seqs, nodes, heads, dim = q.shape
-    want = (seqs, nodes, cache.heads, cache.dim)
-    _need(dim == cache.dim and dim in (64, 128), f'D: the cache\'s, 64 or 128; got {dim}, the cache has {cache.dim}')
-    _need(tuple(k.shape) == want and tuple(v.shape) == want, f'k, v: {want}, got {tuple(k.shape)}, {tuple(v.shape)}')
-    _need(1 <= nodes <= MAX_NODES, f'nodes: 1 to {MAX_NODES}, got {nodes}')
-    _need(heads >= cache.heads and heads % cache.heads == 0 and heads // cache.heads <= 64,
-          f'q heads: a multiple of the cache\'s {cache.heads}, at most 64 times it; got {heads}')
-    _need(table.dim() == 2 and table.shape[0] == seqs, f'table: [{seqs}, pages], got {tuple(table.shape)}')
-    _ints('table', table, torch.int32, tuple(table.shape), dev)
+    if not q.dtype == k.dtype == v.dtype == torch.bfloat16:
+        raise TypeError(f'q, k, v: bf16, got {q.dtype}, {k.dtype}, {v.dtype}')
+    _rows('q', q, 4, dev)
+    _rows('k', k, 4, dev)
+    _rows('v', v, 4, dev)
+    (seqs, nodes, heads, dim), k_heads = q.shape, cache.heads
+    if dim != cache.dim or dim not in (64, 128):
+        raise ValueError(f'D: the cache\'s, 64 or 128; got {dim}, the cache has {cache.dim}')
+    want = (seqs, nodes, k_heads, dim)
+    if k.shape != want or v.shape != want:
+        raise ValueError(f'k, v: {want}, got {tuple(k.shape)}, {tuple(v.shape)}')
+    if not 1 <= nodes <= MAX_NODES:
+        raise ValueError(f'nodes: 1 to {MAX_NODES}, got {nodes}')
+    if heads < k_heads or heads % k_heads or heads // k_heads > 64:
+        raise ValueError(f'q heads: a multiple of the cache\'s {k_heads}, at most 64 times it; got {heads}')
+    if table.dim() != 2 or table.shape[0] != seqs:
+        raise ValueError(f'table: [{seqs}, pages], got {tuple(table.shape)}')
+    _ints('table', table, torch.int32, table.shape, dev)
     _ints('lengths', lengths, torch.int32, (seqs,), dev)
     _ints('mask', mask, torch.int64, (seqs, nodes), dev)
     _ints('depth', depth, torch.int32, (seqs, nodes), dev)
-    _need(0 <= layer < cache.layers, f'layer: 0 to {cache.layers - 1}, got {layer}')
+    if not 0 <= layer < cache.layers:
+        raise ValueError(f'layer: 0 to {cache.layers - 1}, got {layer}')
     # the kernel loads four values of q and of k at once
-    if q.data_ptr() % 16 or any(x % 4 for x in q.stride()[:3]):
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    if q.data_ptr() % 16 or (qs[0] | qs[1] | qs[2]) % 4:
         q = q.contiguous()
-    if k.data_ptr() % 8 or any(x % 4 for x in k.stride()[:3]):
+        qs = q.stride()
+    if k.data_ptr() % 8 or (ks[0] | ks[1] | ks[2]) % 4:
         k = k.contiguous()
+        ks = k.stride()
     out = torch.empty((seqs, nodes, heads, dim), dtype=torch.bfloat16, device=dev)
-    L = _lib.lib()
-    nbytes = L.noise_tree_attention_workspace_bytes(seqs, nodes, heads, cache.heads, dim)
-    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
-    with _On(dev) as stream:
-        _lib.check(L.noise_tree_attention(
-            cache._ref, layer, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), heads, k.data_ptr(), k.stride(0),
-            k.stride(1), k.stride(2), v.data_ptr(), v.stride(0), v.stride(1), v.stride(2), seqs, nodes,
-            table.data_ptr(), table.shape[1], lengths.data_ptr(), mask.data_ptr(), depth.data_ptr(), window,
-            dim ** -0.5 if scale is None else scale, out.data_ptr(), ws.data_ptr(), nbytes, stream),
-            'noise_tree_attention')
+    nbytes = _attention_bytes(seqs, nodes, heads, k_heads, dim)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _call('noise_tree_attention', dev, cache._struct, layer, q.data_ptr(), qs[0], qs[1], qs[2], heads, k.data_ptr(),
+          ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], seqs, nodes, table.data_ptr(), table.shape[1],
+          lengths.data_ptr(), mask.data_ptr(), depth.data_ptr(), window, dim ** -0.5 if scale is None else scale,
+          out.data_ptr(), ws.data_ptr(), nbytes)
     return out
 
 
@@ -372,34 +378,39 @@ def verify_tree(logits, tokens, parents, u, race, probs=None, temperature=1.0, s
     [B, V] exponential; probs fp32 [B, N, V]: the draft's distribution at each node, from which its children were
     drawn, or None for drafts that were picked."""
     _lib.require_cuda(logits, tokens, parents)
-    dev = logits.device
-    if logits.dtype not in DTYPES:
-        raise TypeError(f'logits: fp32 or bf16, got {logits.dtype}')
-    _rows('logits', logits, 3)
+    dev, dtype = logits.device, logits.dtype
+    if dtype not in DTYPES:
+        raise TypeError(f'logits: fp32 or bf16, got {dtype}')
+    _rows('logits', logits, 3, dev)
     seqs, nodes, vocab = logits.shape
-    _need(1 <= nodes <= MAX_NODES, f'nodes: 1 to {MAX_NODES}, got {nodes}')
-    _need(1 <= vocab <= 393216, f'vocabulary: 1 to 393216, got {vocab}')
-    _need(math.isfinite(temperature) and temperature >= 0, f'temperature: {temperature}')
-    _need(math.isfinite(softcap) and softcap >= 0, f'softcap: {softcap}')
-    _ints('tokens', tokens, torch.int64, (seqs, nodes), dev)
-    _ints('parents', parents, torch.int32, (seqs, nodes), dev)
+    if not 1 <= nodes <= MAX_NODES:
+        raise ValueError(f'nodes: 1 to {MAX_NODES}, got {nodes}')
+    if not 1 <= vocab <= MAX_VOCAB:
+        raise ValueError(f'vocabulary: 1 to {MAX_VOCAB}, got {vocab}')
+    if not (0 <= temperature < math.inf and 0 <= softcap < math.inf):
+        raise ValueError(f'temperature and softcap: at least 0; got {temperature}, {softcap}')
+    shape = (seqs, nodes)
+    _ints('tokens', tokens, torch.int64, shape, dev)
+    _ints('parents', parents, torch.int32, shape, dev)
+    u_ptr = race_ptr = q_ptr = None
+    q_seq = q_node = 0
     if temperature > 0:
-        _ints('u', u, torch.float32, (seqs, nodes), dev)
+        _lib.require_cuda(u, race)
+        _ints('u', u, torch.float32, shape, dev)
         _ints('race', race, torch.float32, (seqs, vocab), dev)
+        u_ptr, race_ptr = u.data_ptr(), race.data_ptr()
         if probs is not None:
+            _lib.require_cuda(probs)
             if probs.dtype != torch.float32:
                 raise TypeError(f'probs: fp32, got {probs.dtype}')
             _rows('probs', probs, 3, dev)
-            _need(probs.shape == logits.shape, f'probs: {tuple(logits.shape)}, got {tuple(probs.shape)}')
-    else:
-        u = race = probs = None
+            if probs.shape != logits.shape:
+                raise ValueError(f'probs: {tuple(logits.shape)}, got {tuple(probs.shape)}')
+            q_ptr, q_seq, q_node = probs.data_ptr(), probs.stride(0), probs.stride(1)
     count = torch.empty(seqs, dtype=torch.int32, device=dev)
-    path = torch.empty((seqs, nodes), dtype=torch.int32, device=dev)
+    path = torch.empty(shape, dtype=torch.int32, device=dev)
     token = torch.empty(seqs, dtype=torch.int64, device=dev)
-    with _On(dev) as stream:
-        _lib.check(_lib.lib().noise_verify_tree(
-            logits.data_ptr(), DTYPES[logits.dtype], logits.stride(0), logits.stride(1), tokens.data_ptr(),
-            parents.data_ptr(), _ptr(u), _ptr(race), _ptr(probs), 0 if probs is None else probs.stride(0),
-            0 if probs is None else probs.stride(1), seqs, nodes, vocab, temperature, softcap, count.data_ptr(),
-            path.data_ptr(), token.data_ptr(), stream), 'noise_verify_tree')
+    _call('noise_verify_tree', dev, logits.data_ptr(), DTYPES[dtype], logits.stride(0), logits.stride(1),
+          tokens.data_ptr(), parents.data_ptr(), u_ptr, race_ptr, q_ptr, q_seq, q_node, seqs, nodes, vocab, temperature,
+          softcap, count.data_ptr(), path.data_ptr(), token.data_ptr())
     return count, path, token
