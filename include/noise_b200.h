@@ -774,7 +774,7 @@ typedef struct {
  * NULL: i) to position pos[i] of sequence seq[i], page table[seq, pos / page_size]. A negative seq, pos or row skips
  * the entry; one past seqs, width * page_size, source_rows or pages is skipped and reported in status. k, v
  * [layers, source_rows, heads, dim] of dtype, the last dimension contiguous; seq, pos, rows int32 [tokens]; table int32
- * [seqs, width]. Two entries of a call for one place leave either. 8-bit kinds: the scale is the least power of two (not
+ * [seqs, width]. No two entries of a call may share a place (their codes and scales could mix). 8-bit kinds: the scale is the least power of two (not
  * under 2^-126) with max|x| <= scale * 448 (e4m3) or 127 (int8), code = round(x / scale), ties to even. */
 int noise_kv_write(const noise_kv_cache_t* cache, int layer, int layers, const void* k, int64_t k_layer_stride,
                    int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_layer_stride,

@@ -43,52 +43,96 @@ struct Args {
   float* partial;          // [blocks, D] weight gradients
 };
 
+// N values as they lie in memory, unpacked one at a time: half the registers of fp32 for bf16 rows in flight.
 template <int N, typename T>
-__device__ __forceinline__ void load(const T* p, float (&v)[N]) {
-  constexpr int BYTES = N * sizeof(T);
-  if constexpr (BYTES % 4 == 0) {
-    uint32_t w[BYTES / 4];
+struct Raw {
+  static constexpr int BYTES = N * sizeof(T), WORDS = BYTES < 4 ? 1 : BYTES / 4;
+  uint32_t w[WORDS];
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) w[i] = 0;
+  }
+  __device__ __forceinline__ void ones() {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) w[i] = sizeof(T) == 4 ? 0x3f800000u : 0x3f803f80u;
+  }
+  __device__ __forceinline__ void load(const T* p) {
     if constexpr (BYTES % 16 == 0) {
 #pragma unroll
-      for (int i = 0; i < BYTES / 16; ++i) reinterpret_cast<uint4*>(w)[i] = reinterpret_cast<const uint4*>(p)[i];
-    } else if constexpr (BYTES == 8) {
-      *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(p);
-    } else {
-      w[0] = *reinterpret_cast<const uint32_t*>(p);
-    }
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = __uint_as_float(w[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < N / 2; ++i) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      for (int i = 0; i < BYTES / 16; ++i) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p) + i);
+        w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
       }
+    } else if constexpr (BYTES == 8) {
+      const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
+      w[0] = u.x, w[1] = u.y;
+    } else if constexpr (BYTES == 4) {
+      w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+    } else {
+      static_assert(N == 1 && sizeof(T) == 2, "one 16-bit value");
+      w[0] = __ldg(reinterpret_cast<const unsigned short*>(p));
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = static_cast<float>(p[i]);
   }
+  __device__ __forceinline__ float operator[](int e) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
+    else return __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+  }
+};
+
+// Two fp32 values in a register pair: sm_100a multiplies and adds them in one instruction.
+struct F2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F2 pair(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ F2 both(float a) { return pair(a, a); }
+__device__ __forceinline__ float2 parts(F2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 negative(F2 a) { return {a.v ^ 0x8000000080000000ull}; }
+
+// Pairs of N values (N 1: the second is 0).
+template <int N, typename T>
+__device__ __forceinline__ F2 get2(const Raw<N, T>& r, int p) {
+  if constexpr (N == 1) return pair(r[0], 0.f);
+  else return pair(r[2 * p], r[2 * p + 1]);
 }
 
 template <int N, typename T>
-__device__ __forceinline__ void store(T* p, const float (&v)[N]) {
-  if constexpr (sizeof(T) == 4 && N % 4 == 0) {
+__device__ __forceinline__ void store(T* p, const F2 (&v)[(N + 1) / 2]) {
+  if constexpr (N == 1) {
+    *p = static_cast<T>(parts(v[0]).x);
+  } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < N / 4; ++i)
-      reinterpret_cast<float4*>(p)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-  } else if constexpr (sizeof(T) == 2 && N == 8) {
+    for (int i = 0; i < N / 4; ++i) {
+      const float2 a = parts(v[2 * i]), b = parts(v[2 * i + 1]);
+      reinterpret_cast<float4*>(p)[i] = make_float4(a.x, a.y, b.x, b.y);
+    }
+  } else {
+    static_assert(N == 8, "16 bytes");
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      const float2 a = parts(v[i]);
+      const __nv_bfloat162 h = __floats2bfloat162_rn(a.x, a.y);
       w[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
     *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) p[i] = static_cast<T>(v[i]);
   }
 }
 
@@ -99,79 +143,83 @@ __device__ __forceinline__ float row_sum(float v) {
   return v;
 }
 
-// T: the rows' type; TT: the tables'; a row is LPR lanes with VEC values of each half ITER times. U rows a lane are
-// loaded before the first is used.
-template <typename T, typename TT, int VEC, int LPR, int ITER, int U>
+// T: the rows' type; TT: the tables'; a row is LPR lanes with VEC values of each half ITER times; W: there are weights.
+// A warp takes U (32 / LPR) heads of one token (blockIdx.y: which), all its loads issued before the first is used.
+template <typename T, typename TT, int VEC, int LPR, int ITER, int U, bool W>
 __global__ void __launch_bounds__(32 * WARPS) forward_kernel(const Args a) {
-  const int lane = threadIdx.x & 31, sub = lane % LPR, grp = lane / LPR;
-  const int half = a.dim / 2, chunks = a.q_chunks + a.k_chunks;
-  const int64_t item = blockIdx.x * static_cast<int64_t>(WARPS) + (threadIdx.x >> 5);
-  const int token = static_cast<int>(item / chunks);
+  constexpr int P = (VEC + 1) / 2;
+  const int lane = threadIdx.x & 31, sub = lane % LPR, grp = lane / LPR, half = a.dim / 2;
+  const int token = blockIdx.x * WARPS + (threadIdx.x >> 5);
   if (token >= a.tokens) return;
-  const int chunk = static_cast<int>(item - static_cast<int64_t>(token) * chunks);
+  const int chunk = blockIdx.y;
   const bool is_k = chunk >= a.q_chunks;
   const Rows& r = is_k ? a.k : a.q;
   const int h0 = (is_k ? chunk - a.q_chunks : chunk) * (32 / LPR) * U + grp;
   const T* src = static_cast<const T*>(r.x) + token * r.token;
-  float x[U][ITER][2][VEC];
+  const int pos = __ldg(a.positions + token);
+  Raw<VEC, T> x[U][ITER][2];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int h = h0 + u * (32 / LPR);
 #pragma unroll
     for (int it = 0; it < ITER; ++it) {
       const int i = (it * LPR + sub) * VEC;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) x[u][it][0][e] = x[u][it][1][e] = 0.f;
+      x[u][it][0].zero();
+      x[u][it][1].zero();
       if (h < r.heads && i < half) {
-        load<VEC>(src + h * r.head + i, x[u][it][0]);
-        load<VEC>(src + h * r.head + half + i, x[u][it][1]);
+        x[u][it][0].load(src + h * r.head + i);
+        x[u][it][1].load(src + h * r.head + half + i);
       }
     }
   }
-  const int pos = a.positions[token];
   const bool known = pos >= 0 && pos < a.table_rows;  // a position without a table row gives NaN
-  float c[ITER][VEC], s[ITER][VEC];
+  Raw<VEC, TT> c[ITER], s[ITER];
+  Raw<VEC, T> w[W ? ITER : 1][2];
 #pragma unroll
   for (int it = 0; it < ITER; ++it) {
     const int i = (it * LPR + sub) * VEC;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) c[it][e] = s[it][e] = __int_as_float(0x7fc00000);
+    c[it].zero();
+    s[it].zero();
     if (known && i < half) {
-      load<VEC>(static_cast<const TT*>(a.cos) + static_cast<int64_t>(pos) * half + i, c[it]);
-      load<VEC>(static_cast<const TT*>(a.sin) + static_cast<int64_t>(pos) * half + i, s[it]);
+      c[it].load(static_cast<const TT*>(a.cos) + static_cast<int64_t>(pos) * half + i);
+      s[it].load(static_cast<const TT*>(a.sin) + static_cast<int64_t>(pos) * half + i);
     }
-  }
-  float w[ITER][2][VEC];
-#pragma unroll
-  for (int it = 0; it < ITER; ++it) {
-    const int i = (it * LPR + sub) * VEC;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) w[it][0][e] = w[it][1][e] = 1.f;
-    if (r.weight && i < half) {
-      load<VEC>(static_cast<const T*>(r.weight) + i, w[it][0]);
-      load<VEC>(static_cast<const T*>(r.weight) + half + i, w[it][1]);
+    if constexpr (W) {
+      w[it][0].ones();
+      w[it][1].ones();
+      if (r.weight && i < half) {
+        w[it][0].load(static_cast<const T*>(r.weight) + i);
+        w[it][1].load(static_cast<const T*>(r.weight) + half + i);
+      }
     }
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    float sq = 0.f;
+    F2 sq = both(0.f);
 #pragma unroll
     for (int it = 0; it < ITER; ++it)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) sq += x[u][it][0][e] * x[u][it][0][e] + x[u][it][1][e] * x[u][it][1][e];
-    const float rr = rsqrtf(row_sum<LPR>(sq) / a.dim + a.eps);
+      for (int e = 0; e < P; ++e) {
+        const F2 x1 = get2(x[u][it][0], e), x2 = get2(x[u][it][1], e);
+        sq = fma2(x1, x1, fma2(x2, x2, sq));
+      }
+    const float2 sums = parts(sq);
+    float rr = rsqrtf(row_sum<LPR>(sums.x + sums.y) / a.dim + a.eps);
+    if (!known) rr = __int_as_float(0x7fc00000);
     const int h = h0 + u * (32 / LPR);
     if (h >= r.heads) continue;
     T* dst = static_cast<T*>(r.out) + (static_cast<int64_t>(token) * r.heads + h) * a.dim;
 #pragma unroll
     for (int it = 0; it < ITER; ++it) {
       const int i = (it * LPR + sub) * VEC;
-      float y1[VEC], y2[VEC];
+      F2 y1[P], y2[P];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float a1 = x[u][it][0][e] * rr * w[it][0][e], a2 = x[u][it][1][e] * rr * w[it][1][e];
-        y1[e] = a1 * c[it][e] + a2 * s[it][e];
-        y2[e] = a2 * c[it][e] - a1 * s[it][e];
+      for (int e = 0; e < P; ++e) {
+        F2 a1 = get2(x[u][it][0], e) * both(rr), a2 = get2(x[u][it][1], e) * both(rr);
+        if constexpr (W) a1 = a1 * get2(w[it][0], e), a2 = a2 * get2(w[it][1], e);
+        const F2 cc = get2(c[it], e), ss = get2(s[it], e);
+        y1[e] = fma2(a1, cc, a2 * ss);
+        y2[e] = fma2(a2, cc, negative(a1) * ss);
       }
       if (i < half) {
         store<VEC>(dst + i, y1);
@@ -182,115 +230,143 @@ __global__ void __launch_bounds__(32 * WARPS) forward_kernel(const Args a) {
 }
 
 // Blocks [0, q_blocks) take the queries, the others the keys, so a lane sums one weight's gradient over all its rows;
-// a block's sums go to partial[block] (no atomics: the order is the same from call to call).
-template <typename T, typename TT, int VEC, int LPR, int ITER>
+// a block's sums go to partial[block] (no atomics: the order is the same from call to call). A warp walks over its
+// (token, heads) items with the next one's rows on their way while it computes.
+template <typename T, typename TT, int VEC, int LPR, int ITER, bool W>
 __global__ void __launch_bounds__(32 * WARPS) backward_kernel(const Args a) {
-  __shared__ float sums[WARPS][2 * LPR * VEC * ITER];
+  __shared__ float sums[W ? WARPS : 1][2 * LPR * VEC * ITER];
+  constexpr int P = (VEC + 1) / 2;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % LPR, grp = lane / LPR;
   const int half = a.dim / 2;
   const bool is_k = blockIdx.x >= a.q_blocks;
   const Rows& r = is_k ? a.k : a.q;
-  const int chunks = is_k ? a.k_chunks : a.q_chunks;
-  const int block = is_k ? blockIdx.x - a.q_blocks : blockIdx.x;
-  const int blocks = is_k ? gridDim.x - a.q_blocks : a.q_blocks;
-  float w[ITER][2][VEC], dw[ITER][2][VEC];
+  const unsigned chunks = is_k ? a.k_chunks : a.q_chunks;
+  const unsigned block = is_k ? blockIdx.x - a.q_blocks : blockIdx.x;
+  const unsigned step = (is_k ? gridDim.x - a.q_blocks : a.q_blocks) * WARPS;
+  const unsigned items = a.tokens * chunks;
+  Raw<VEC, T> w[W ? ITER : 1][2];
+  F2 dw[W ? ITER : 1][2][P];
+  if constexpr (W) {
 #pragma unroll
-  for (int it = 0; it < ITER; ++it) {
-    const int i = (it * LPR + sub) * VEC;
+    for (int it = 0; it < ITER; ++it) {
+      const int i = (it * LPR + sub) * VEC;
+      w[it][0].ones();
+      w[it][1].ones();
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      w[it][0][e] = w[it][1][e] = 1.f;
-      dw[it][0][e] = dw[it][1][e] = 0.f;
-    }
-    if (r.weight && i < half) {
-      load<VEC>(static_cast<const T*>(r.weight) + i, w[it][0]);
-      load<VEC>(static_cast<const T*>(r.weight) + half + i, w[it][1]);
+      for (int e = 0; e < P; ++e) dw[it][0][e] = dw[it][1][e] = both(0.f);
+      if (r.weight && i < half) {
+        w[it][0].load(static_cast<const T*>(r.weight) + i);
+        w[it][1].load(static_cast<const T*>(r.weight) + half + i);
+      }
     }
   }
-  const int64_t items = static_cast<int64_t>(a.tokens) * chunks;
-  for (int64_t item = block * static_cast<int64_t>(WARPS) + warp; item < items;
-       item += static_cast<int64_t>(blocks) * WARPS) {
-    const int token = static_cast<int>(item / chunks);
-    const int h = static_cast<int>(item - static_cast<int64_t>(token) * chunks) * (32 / LPR) + grp;
-    const bool here = h < r.heads;
-    const T* src = static_cast<const T*>(r.x) + token * r.token + h * r.head;
-    const T* dsrc = static_cast<const T*>(r.dy) + token * r.dy_token + h * r.dy_head;
-    float x[ITER][2][VEC], g[ITER][2][VEC], c[ITER][VEC], s[ITER][VEC];
+  struct Item {
+    Raw<VEC, T> x[ITER][2], g[ITER][2];
+    int token, h, pos;
+  };
+  const auto fetch = [&](Item& n, unsigned item) {
+    n.token = static_cast<int>(item / chunks);
+    n.h = static_cast<int>(item - n.token * chunks) * (32 / LPR) + grp;
+    if (item >= items) n.h = r.heads;
+    n.pos = item < items ? __ldg(a.positions + n.token) : -1;
 #pragma unroll
     for (int it = 0; it < ITER; ++it) {
       const int i = (it * LPR + sub) * VEC;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) x[it][0][e] = x[it][1][e] = g[it][0][e] = g[it][1][e] = 0.f;
-      if (here && i < half) {
-        load<VEC>(src + i, x[it][0]);
-        load<VEC>(src + half + i, x[it][1]);
-        load<VEC>(dsrc + i, g[it][0]);
-        load<VEC>(dsrc + half + i, g[it][1]);
+      for (int p = 0; p < 2; ++p) {
+        n.x[it][p].zero();
+        n.g[it][p].zero();
+        if (n.h < r.heads && i < half) {
+          n.x[it][p].load(static_cast<const T*>(r.x) + n.token * r.token + n.h * r.head + p * half + i);
+          n.g[it][p].load(static_cast<const T*>(r.dy) + n.token * r.dy_token + n.h * r.dy_head + p * half + i);
+        }
       }
     }
-    const int pos = a.positions[token];
-    const bool known = pos >= 0 && pos < a.table_rows;
+  };
+  const unsigned first = block * WARPS + warp;
+  Item cur;
+  if (first < items) fetch(cur, first);
+  for (unsigned item = first; item < items; item += step) {
+    const bool known = cur.pos >= 0 && cur.pos < a.table_rows, here = cur.h < r.heads;
+    Raw<VEC, TT> c[ITER], s[ITER];
 #pragma unroll
     for (int it = 0; it < ITER; ++it) {
       const int i = (it * LPR + sub) * VEC;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) c[it][e] = s[it][e] = i < half ? __int_as_float(0x7fc00000) : 0.f;
+      c[it].zero();
+      s[it].zero();
       if (known && i < half) {
-        load<VEC>(static_cast<const TT*>(a.cos) + static_cast<int64_t>(pos) * half + i, c[it]);
-        load<VEC>(static_cast<const TT*>(a.sin) + static_cast<int64_t>(pos) * half + i, s[it]);
+        c[it].load(static_cast<const TT*>(a.cos) + static_cast<int64_t>(cur.pos) * half + i);
+        s[it].load(static_cast<const TT*>(a.sin) + static_cast<int64_t>(cur.pos) * half + i);
       }
     }
-    float sq = 0.f, dot = 0.f;  // dot: sum h x
+    Item next;
+    fetch(next, item + step);  // (tokens * chunks + step stays below 2^32)
+    F2 g[ITER][2][P];
+    F2 sq = both(0.f), dot = both(0.f);  // dot: sum h x
 #pragma unroll
     for (int it = 0; it < ITER; ++it)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float d1 = g[it][0][e], d2 = g[it][1][e];
-        g[it][0][e] = d1 * c[it][e] - d2 * s[it][e];
-        g[it][1][e] = d1 * s[it][e] + d2 * c[it][e];
-        sq += x[it][0][e] * x[it][0][e] + x[it][1][e] * x[it][1][e];
-        dot += g[it][0][e] * w[it][0][e] * x[it][0][e] + g[it][1][e] * w[it][1][e] * x[it][1][e];
+      for (int e = 0; e < P; ++e) {
+        const F2 d1 = get2(cur.g[it][0], e), d2 = get2(cur.g[it][1], e);
+        const F2 x1 = get2(cur.x[it][0], e), x2 = get2(cur.x[it][1], e);
+        const F2 cc = get2(c[it], e), ss = get2(s[it], e);
+        g[it][0][e] = fma2(d1, cc, negative(d2) * ss);
+        g[it][1][e] = fma2(d1, ss, d2 * cc);
+        sq = fma2(x1, x1, fma2(x2, x2, sq));
+        if constexpr (W)
+          dot = fma2(g[it][0][e] * get2(w[it][0], e), x1, fma2(g[it][1][e] * get2(w[it][1], e), x2, dot));
+        else
+          dot = fma2(g[it][0][e], x1, fma2(g[it][1][e], x2, dot));
       }
-    const float rr = rsqrtf(row_sum<LPR>(sq) / a.dim + a.eps);
-    const float m = row_sum<LPR>(dot) * rr / a.dim;  // mean(h xh)
-    T* dst = static_cast<T*>(r.out) + (static_cast<int64_t>(token) * r.heads + h) * a.dim;
+    const float2 sums_sq = parts(sq), sums_dot = parts(dot);
+    float rr = rsqrtf(row_sum<LPR>(sums_sq.x + sums_sq.y) / a.dim + a.eps);
+    if (!known) rr = __int_as_float(0x7fc00000);
+    const float m = row_sum<LPR>(sums_dot.x + sums_dot.y) * rr / a.dim;  // mean(h xh)
+    T* dst = static_cast<T*>(r.out) + (static_cast<int64_t>(cur.token) * r.heads + cur.h) * a.dim;
+    const F2 r2 = both(rr), m2 = both(-m * rr);
 #pragma unroll
     for (int it = 0; it < ITER; ++it) {
       const int i = (it * LPR + sub) * VEC;
-      float o[2][VEC];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        F2 o[P];
+#pragma unroll
+        for (int e = 0; e < P; ++e) {
+          const F2 xh = get2(cur.x[it][p], e) * r2;
+          F2 h = g[it][p][e];
+          if constexpr (W) {
+            if (here) dw[it][p][e] = fma2(h, xh, dw[it][p][e]);
+            h = h * get2(w[it][p], e);
+          }
+          o[e] = fma2(h, r2, xh * m2);  // r (h - xh m)
+        }
+        if (here && i < half) store<VEC>(dst + p * half + i, o);
+      }
+    }
+    cur = next;
+  }
+  if constexpr (W) {
+    if (!a.partial) return;
+#pragma unroll
+    for (int it = 0; it < ITER; ++it)
 #pragma unroll
       for (int p = 0; p < 2; ++p)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          const float xh = x[it][p][e] * rr;
-          o[p][e] = rr * (g[it][p][e] * w[it][p][e] - xh * m);
-          if (here) dw[it][p][e] += g[it][p][e] * xh;
+          const float2 two = parts(dw[it][p][e / 2]);
+          float v = e & 1 ? two.y : two.x;
+#pragma unroll
+          for (int o = 16; o >= LPR; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+          const int i = (it * LPR + sub) * VEC + e;
+          if (grp == 0 && i < half) sums[warp][p * half + i] = v;
         }
-      if (here && i < half) {
-        store<VEC>(dst + i, o[0]);
-        store<VEC>(dst + half + i, o[1]);
-      }
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.dim; i += 32 * WARPS) {
+      float v = 0.f;
+#pragma unroll
+      for (int k = 0; k < WARPS; ++k) v += sums[k][i];
+      a.partial[static_cast<int64_t>(blockIdx.x) * a.dim + i] = v;
     }
-  }
-  if (!a.partial) return;
-#pragma unroll
-  for (int it = 0; it < ITER; ++it)
-#pragma unroll
-    for (int p = 0; p < 2; ++p)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        float v = dw[it][p][e];
-#pragma unroll
-        for (int o = 16; o >= LPR; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        const int i = (it * LPR + sub) * VEC + e;
-        if (grp == 0 && i < half) sums[warp][p * half + i] = v;
-      }
-  __syncthreads();
-  for (int i = threadIdx.x; i < a.dim; i += 32 * WARPS) {
-    float v = 0.f;
-#pragma unroll
-    for (int k = 0; k < WARPS; ++k) v += sums[k][i];
-    a.partial[static_cast<int64_t>(blockIdx.x) * a.dim + i] = v;
   }
 }
 
@@ -316,7 +392,7 @@ __global__ void __launch_bounds__(1024) weight_kernel(const float* partial, int 
   }
 }
 
-constexpr int GRAD_BLOCKS = 148 * 3;  // three blocks of 8 warps fit an SM: one wave
+constexpr int GRAD_BLOCKS = 148 * 4;
 
 inline int lanes_of(int half, int vec) {
   int l = 1;
@@ -324,16 +400,15 @@ inline int lanes_of(int half, int vec) {
   return l;
 }
 
-template <typename T, typename TT, int VEC, int LPR, int ITER>
+template <typename T, typename TT, int VEC, int LPR, int ITER, bool W>
 cudaError_t run(Args a, bool backward, float* q_dw, float* k_dw, cudaStream_t s) {
   constexpr int U = ITER > 1 || LPR == 32 ? 1 : 2;
   if (!backward) {
     constexpr int HEADS = 32 / LPR * U;
     a.q_chunks = (a.q.heads + HEADS - 1) / HEADS;
     a.k_chunks = (a.k.heads + HEADS - 1) / HEADS;
-    const int64_t items = static_cast<int64_t>(a.tokens) * (a.q_chunks + a.k_chunks);
-    forward_kernel<T, TT, VEC, LPR, ITER, U>
-        <<<static_cast<unsigned>((items + WARPS - 1) / WARPS), 32 * WARPS, 0, s>>>(a);
+    forward_kernel<T, TT, VEC, LPR, ITER, U, W>
+        <<<dim3((a.tokens + WARPS - 1) / WARPS, a.q_chunks + a.k_chunks), 32 * WARPS, 0, s>>>(a);
     return cudaGetLastError();
   }
   constexpr int HEADS = 32 / LPR;
@@ -346,10 +421,9 @@ cudaError_t run(Args a, bool backward, float* q_dw, float* k_dw, cudaStream_t s)
   const int64_t k_most = GRAD_BLOCKS - q_most > 1 ? GRAD_BLOCKS - q_most : 1;
   a.q_blocks = static_cast<int>(q_need < q_most ? q_need : q_most);
   const int blocks = a.q_blocks + static_cast<int>(k_need < k_most ? k_need : k_most);
-  if (!q_dw && !k_dw) a.partial = nullptr;
-  backward_kernel<T, TT, VEC, LPR, ITER><<<blocks, 32 * WARPS, 0, s>>>(a);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || !a.partial) return e;
+  backward_kernel<T, TT, VEC, LPR, ITER, W><<<blocks, 32 * WARPS, 0, s>>>(a);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || (!q_dw && !k_dw)) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((a.dim + 31) / 32, 2);
   cfg.blockDim = dim3(1024);
@@ -363,18 +437,24 @@ cudaError_t run(Args a, bool backward, float* q_dw, float* k_dw, cudaStream_t s)
                             q_dw, k_dw);
 }
 
-template <typename T, typename TT>
+template <typename T, typename TT, bool W>
 cudaError_t by_lanes(const Args& a, bool wide, bool backward, float* q_dw, float* k_dw, cudaStream_t s) {
   constexpr int VEC = 16 / sizeof(T);
-  if (!wide) return run<T, TT, 1, 32, 4>(a, backward, q_dw, k_dw, s);  // any address: one value at a time
+  if (!wide) return run<T, TT, 1, 32, 4, W>(a, backward, q_dw, k_dw, s);  // any address: one value at a time
   switch (lanes_of(a.dim / 2, VEC)) {
-    case 1: return run<T, TT, VEC, 1, 1>(a, backward, q_dw, k_dw, s);
-    case 2: return run<T, TT, VEC, 2, 1>(a, backward, q_dw, k_dw, s);
-    case 4: return run<T, TT, VEC, 4, 1>(a, backward, q_dw, k_dw, s);
-    case 8: return run<T, TT, VEC, 8, 1>(a, backward, q_dw, k_dw, s);
-    case 16: return run<T, TT, VEC, 16, 1>(a, backward, q_dw, k_dw, s);
-    default: return run<T, TT, VEC, 32, 1>(a, backward, q_dw, k_dw, s);
+    case 1: return run<T, TT, VEC, 1, 1, W>(a, backward, q_dw, k_dw, s);
+    case 2: return run<T, TT, VEC, 2, 1, W>(a, backward, q_dw, k_dw, s);
+    case 4: return run<T, TT, VEC, 4, 1, W>(a, backward, q_dw, k_dw, s);
+    case 8: return run<T, TT, VEC, 8, 1, W>(a, backward, q_dw, k_dw, s);
+    case 16: return run<T, TT, VEC, 16, 1, W>(a, backward, q_dw, k_dw, s);
+    default: return run<T, TT, VEC, 32, 1, W>(a, backward, q_dw, k_dw, s);
   }
+}
+
+template <typename T, typename TT>
+cudaError_t by_weights(const Args& a, bool wide, bool backward, float* q_dw, float* k_dw, cudaStream_t s) {
+  return a.q.weight || a.k.weight ? by_lanes<T, TT, true>(a, wide, backward, q_dw, k_dw, s)
+                    : by_lanes<T, TT, false>(a, wide, backward, q_dw, k_dw, s);
 }
 
 template <typename T>
@@ -394,7 +474,8 @@ int launch(const noise_heads_t* q, const noise_heads_t* k, const noise_heads_t* 
       (table_dtype != NOISE_DTYPE_F32 && table_dtype != NOISE_DTYPE_BF16))
     return NOISE_ERR_ARGUMENT;
   if (tokens < 0 || dim < 2 || dim > 256 || dim % 2 || table_rows < 1 || q->heads < 1 || k->heads < 1 ||
-      q->heads > 4096 || k->heads > 4096)
+      q->heads > 4096 || k->heads > 4096 ||
+      static_cast<int64_t>(tokens) * (q->heads > k->heads ? q->heads : k->heads) > (1u << 31))
     return NOISE_ERR_SHAPE;
   if (!(eps >= 0.f)) return NOISE_ERR_ARGUMENT;
   if (tokens == 0) return NOISE_OK;
@@ -419,12 +500,12 @@ int launch(const noise_heads_t* q, const noise_heads_t* k, const noise_heads_t* 
   cudaError_t e;
   if (dtype == NOISE_DTYPE_F32) {
     const bool wide = tables && wide_rows<float>(a.q, dim) && wide_rows<float>(a.k, dim);
-    e = table_dtype == NOISE_DTYPE_F32 ? by_lanes<float, float>(a, wide, backward, q_dw, k_dw, s)
-                                       : by_lanes<float, __nv_bfloat16>(a, wide, backward, q_dw, k_dw, s);
+    e = table_dtype == NOISE_DTYPE_F32 ? by_weights<float, float>(a, wide, backward, q_dw, k_dw, s)
+                                       : by_weights<float, __nv_bfloat16>(a, wide, backward, q_dw, k_dw, s);
   } else {
     const bool wide = tables && wide_rows<__nv_bfloat16>(a.q, dim) && wide_rows<__nv_bfloat16>(a.k, dim);
-    e = table_dtype == NOISE_DTYPE_F32 ? by_lanes<__nv_bfloat16, float>(a, wide, backward, q_dw, k_dw, s)
-                                       : by_lanes<__nv_bfloat16, __nv_bfloat16>(a, wide, backward, q_dw, k_dw, s);
+    e = table_dtype == NOISE_DTYPE_F32 ? by_weights<__nv_bfloat16, float>(a, wide, backward, q_dw, k_dw, s)
+                                       : by_weights<__nv_bfloat16, __nv_bfloat16>(a, wide, backward, q_dw, k_dw, s);
   }
   return e == cudaSuccess ? NOISE_OK : NOISE_ERR_CUDA;
 }

@@ -38,8 +38,8 @@ __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) 
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
     return lo | hi << 16;
   } else {
-    return (__float2int_rn(a) & 0xff) | (__float2int_rn(b) & 0xff) << 8 | (__float2int_rn(c) & 0xff) << 16 |
-           (__float2int_rn(d) & 0xff) << 24;
+    const auto whole = [](float x) { return __float_as_uint(x + 12582912.f); };  // 1.5 * 2^23: rounds to the last bit
+    return __byte_perm(__byte_perm(whole(a), whole(b), 0x0040), __byte_perm(whole(c), whole(d), 0x0040), 0x5410);
   }
 }
 

@@ -251,7 +251,7 @@ class KVCache:
 
         k, v [source rows, heads, D], fp32 or bf16, any strides but the last; entry i takes row rows[i] (int32 [tokens];
         negative: skipped), or row i. layer None: all layers at once, k, v [layers, source rows, heads, D]. An entry out
-        of range is skipped and reported by ``check()``."""
+        of range is skipped and reported by ``check()``; no two entries of a call may share a place."""
         _lib.require_cuda(k, v)
         tokens, first, layers = self._places(seq, pos, table, layer)
         if k.dtype not in DTYPES or v.dtype != k.dtype:

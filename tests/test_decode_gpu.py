@@ -191,6 +191,35 @@ def test_cache_holds_the_rounded_values(kind, dtype, dim, heads, page, offset):
     cache.check()
 
 
+@pytest.mark.parametrize('kind', ['bf16', 'e4m3', 'int8'])
+@pytest.mark.parametrize('dim,heads', [(64, 3), (128, 1)])
+@pytest.mark.parametrize('runs', [[(0, 7, 40)], [(0, 0, 3), (1, 2, 5), (0, 3, 1), (1, 7, 30)], [(2, 61, 9), (0, 5, 2), (2, 1, 1)],
+                                  [(0, i, 1) for i in (9, 8, 7, 6, 5, 12, 13, 3, 2)]])
+def test_cache_runs_of_positions(kind, dim, heads, runs):
+    """Runs that begin and end anywhere (whole and broken quads), with skipped entries between them."""
+    g = _gen(len(runs))
+    cache, table = _cache(kind, dim, heads, 16, 3, 80)
+    seq, pos = [], []
+    for s, first, n in runs:
+        seq += [s] * n + [-1]
+        pos += list(range(first, first + n)) + [first + n]
+    seq, pos = (torch.tensor(x, dtype=torch.int32) for x in (seq, pos))
+    k, v = (torch.randn(len(seq), heads, dim, generator=g) for _ in range(2))
+    cache.write(k.to(DEV), v.to(DEV), seq.to(DEV), pos.to(DEV), table)
+    every = [(s, p) for s in range(3) for p in range(80)]
+    all_seq, all_pos = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in zip(*every))
+    for got, x in zip(cache.read(all_seq, all_pos, table), (k, v)):
+        want = torch.zeros(len(every), heads, dim, dtype=torch.float64)
+        for i, (s, p) in enumerate(zip(seq.tolist(), pos.tolist())):
+            if s >= 0:
+                want[s * 80 + p] = oracle.quantised(x[i], kind)
+        assert torch.equal(got.cpu().double(), want)
+    for got, x in zip(cache.read(seq.to(DEV), pos.to(DEV), table), (k, v)):
+        want = torch.where((seq >= 0)[:, None, None], oracle.quantised(x, kind), 0.0)
+        assert torch.equal(got.cpu().double(), want)
+    cache.check()
+
+
 def test_cache_rows_layers_and_bad_places():
     from noise_b200._lib import NoiseError
     cache, table = _cache('int8', 64, 2, 16, 2, 48, layers=3)
