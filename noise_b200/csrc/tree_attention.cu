@@ -11,9 +11,13 @@
 //  - Each warp walks the keys 16 at a time and keeps a running maximum, sum and output (32 bits) for its rows. A lane
 //    copies its own fragments (cp.async, 16 bytes each, a ring of STAGES steps) and reads back only what it copied
 //    itself: no barrier, and the loads of the next steps stay in flight while a step computes.
-//  - The order of a contraction's index is free, so it is chosen for the loads: for S = Q K^T a lane takes 16
-//    consecutive bytes of a key's row, for P V four neighbouring keys of one dimension, which lie in one word of V's
+//  - Keys are the products' 16 rows (S^T = K Q^T, O^T = V^T P^T) and query rows their 8 columns, so a decoding step of
+//    up to 8 rows wastes no more than its own rounding to 8. P passes from one product to the other by a transpose of
+//    8 x 8 tiles in registers.
+//  - The order of a contraction's index is free, so it is chosen for the loads: for K Q^T a lane takes 16
+//    consecutive bytes of a key's row, for V^T P^T four neighbouring keys of one dimension, which lie in one word of V's
 //    layout; codes become fp16 in registers.
+//  - The running maximum moves only when a score passes it by 2^8: a vote a step instead of a reduction over its keys.
 //  - The keys of all sequences, heads and row tiles form one line of units of 64 keys, cut into equal spans, one a
 //    CTA, whatever the lengths are. Parts of an item are joined by a second kernel.
 // Roundings: Q to fp16 under a power of two per row (an element loses bits only below 2^-14 of the row's largest),
@@ -65,14 +69,24 @@ __device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real) {
-  const int n = real ? 16 : 0;  // else zeros
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+template <bool BF>
+__device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  if constexpr (BF) mma_bf16(c, a[0], a[1], a[2], a[3], b0, b1);
+  else mma_f16(c, a, b0, b1);
 }
-__device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool real) {
-  const int n = real ? 4 : 0;
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+
+// An 8 x 8 tile of 16-bit values, a row's pairs in lanes 4 row .. 4 row + 3, transposed.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
@@ -146,158 +160,165 @@ struct Spans {  // CTA i takes units [cut(i), cut(i + 1))
 
 // ---- one item's part --------------------------------------------------------------------------------------------
 
-template <int KIND, int D, int MT, int RW>
+// NTL: tiles of 8 query rows a warp; RW: warps side by side that take other rows.
+template <int KIND, int D, int NTL, int RW>
 struct Shape {
   static constexpr bool BF = KIND == NOISE_KV_BF16;
-  static constexpr int KS = D / 16;                  // steps of Q K^T
-  static constexpr int NB = D / 8;                   // columns of 8 of the output
+  static constexpr int KS = D / 16;                  // steps of K Q^T
+  static constexpr int MB = D / 16;                  // tiles of 16 dimensions of the output
   static constexpr int NL = BF ? D / 16 : D / 32;    // 16-byte loads a lane of K, and of V
   static constexpr int NT = 32 * KW * RW;
-  static constexpr int RT = 16 * MT * RW;
+  static constexpr int RT = 8 * NTL * RW;
   static constexpr int STEP = 2 * NL * 512 + (BF ? 0 : 256);  // bytes of a warp's 16 keys
   static constexpr int STAGES = STEP <= 2500 ? 4 : 3;
-  static constexpr bool QREG = MT * KS <= 8;         // Q's fragments in registers, else in shared memory
+  static constexpr bool QREG = NTL * KS <= 16;       // Q's fragments in registers, else in shared memory
   static constexpr int RING = STAGES * STEP;
-  static constexpr int JOIN = 32 * (4 * MT * NB + 4 * MT) * 4;  // a warp's output, maxima and sums
-  static constexpr int QBYTES = QREG ? 0 : RW * MT * KS * 512;
+  static constexpr int JOIN = 32 * (4 * NTL * MB + 4 * NTL) * 4;  // a warp's output, maxima and sums
+  static constexpr int QBYTES = QREG ? 0 : RW * NTL * KS * 256;
   static constexpr int WORK = KW * RW * RING > 2 * RW * JOIN ? KW * RW * RING : 2 * RW * JOIN;
   static constexpr int SMEM = WORK + QBYTES;
-  // the dimension that word (ks) of lane t starts at in Q K^T: 16 consecutive bytes of a key's row a lane
+  // the dimension that word (ks) of lane t starts at in K Q^T: 16 consecutive bytes of a key's row a lane
   __device__ static __forceinline__ int dim_of(int ks, int t) {
     return BF ? (ks >> 1) * 32 + t * 8 + (ks & 1) * 4 : (ks >> 2) * 64 + t * 16 + (ks & 3) * 4;
   }
 };
 
-template <int KIND, int D, int MT, int RW>
-struct Part {
-  using S = Shape<KIND, D, MT, RW>;
-  float acc[MT][S::NB][4];
-  float m[MT][2], l[MT][2], rf[MT][2];  // maxima of the scores before the row's factor rf
-  int lo[MT][2];                        // the first cached position in the row's window
-  int vref;                             // acc holds the output in units of 2^(vref - 127) (8-bit kinds)
+constexpr float SLACK = 8.f;     // log2 of how far a probability may pass 1 before the maximum moves
+constexpr float NONE = 3e38f;    // off of a row that has seen no key
 
-  // Scores s (masked: -inf) to probabilities, the running maximum and sum and the output's rescaling.
-  __device__ __forceinline__ void soften(float (&s)[MT][2][4], int new_ref) {
-    bool up = new_ref != vref;
-    float top[MT][2];
+// A lane's part of a warp's rows: of rows 2t and 2t + 1 of each tile, the keys g and g + 8 of each step, and the
+// output's dimensions (below). Keys g and g + 8 of the products stand at key_of(g) and key_of(g) + 2 of the 16.
+__device__ __forceinline__ int key_of(int g) { return 4 * (g >> 1) + (g & 1); }
+
+template <int KIND, int D, int NTL, int RW>
+struct Part {
+  using S = Shape<KIND, D, NTL, RW>;
+  float acc[NTL][S::MB][4];
+  float l[NTL][2], rf[NTL][2];  // sums; the factor from a row's scores to powers of two
+  float off[NTL][2];            // less the running maximum, in powers of two
+  int vref;                     // acc holds the output in units of 2^(vref - 127) (8-bit kinds)
+
+  // The maximum and the output's unit moved; every lane of the warp calls it.
+  __device__ __forceinline__ void move(const float (&s)[NTL][4], int new_ref) {
+    const float unit = ex2(static_cast<float>(vref - new_ref));
+    vref = new_ref;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int nt = 0; nt < NTL; ++nt)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float x = fmaxf(fmaxf(s[mt][0][2 * h], s[mt][0][2 * h + 1]), fmaxf(s[mt][1][2 * h], s[mt][1][2 * h + 1]));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-        top[mt][h] = fmaxf(m[mt][h], x);
-        up |= top[mt][h] > m[mt][h];
-      }
-    if (__any_sync(0xffffffffu, up)) {
-      const float unit = ex2(static_cast<float>(vref - new_ref));
-      vref = new_ref;
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float f = top[mt][h] > m[mt][h] ? ex2((m[mt][h] - top[mt][h]) * rf[mt][h]) : 1.f;
-          m[mt][h] = top[mt][h];
-          l[mt][h] *= f;
-          const float g = f * unit;
-#pragma unroll
-          for (int nb = 0; nb < S::NB; ++nb) {
-            acc[mt][nb][2 * h] *= g;
-            acc[mt][nb][2 * h + 1] *= g;
-          }
+      for (int e = 0; e < 2; ++e) {
+        float x = fmaxf(s[nt][e], s[nt][2 + e]);
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16)) * rf[nt][e];
+        float f = 1.f;
+        if (x > -off[nt][e]) {
+          f = ex2(-off[nt][e] - x);
+          off[nt][e] = -x;
+          l[nt][e] *= f;
         }
+        f *= unit;
+#pragma unroll
+        for (int mb = 0; mb < S::MB; ++mb) {
+          acc[nt][mb][e] *= f;
+          acc[nt][mb][2 + e] *= f;
+        }
+      }
+  }
+
+  // Scores s (masked: -inf) to probabilities, their sums, and the running maximum; ref: the largest V scale there is.
+  __device__ __forceinline__ void soften(float (&s)[NTL][4], int ref) {
+    bool up = ref > vref;
+#pragma unroll
+    for (int nt = 0; nt < NTL; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) up |= fmaf(s[nt][e], rf[nt][e & 1], off[nt][e & 1]) > SLACK;
+    if (__any_sync(0xffffffffu, up)) {
+      ref = max(ref, __shfl_xor_sync(0xffffffffu, ref, 4));
+      ref = max(ref, __shfl_xor_sync(0xffffffffu, ref, 8));
+      ref = max(ref, __shfl_xor_sync(0xffffffffu, ref, 16));
+      move(s, max(ref, vref));
     }
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int nt = 0; nt < NTL; ++nt)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float off = m[mt][h] == NEG ? 0.f : -m[mt][h] * rf[mt][h];
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float& x = s[mt][j][2 * h + e];
-            x = ex2(fmaf(x, rf[mt][h], off));
-            l[mt][h] += x;
-          }
+      for (int e = 0; e < 4; ++e) {
+        s[nt][e] = ex2(fmaf(s[nt][e], rf[nt][e & 1], off[nt][e & 1]));
+        l[nt][e & 1] += s[nt][e];
       }
   }
 };
 
-// P's fragment of a 16 x 16 tile: columns 2t, 2t + 1 of both blocks of 8 are the lane's four keys 4t .. 4t + 3.
+// P^T's fragment of 16 keys x 8 rows from the lane's scores: keys g (factor f0) and g + 8 (f1).
 template <bool BF>
-__device__ __forceinline__ void p_fragment(const float (&s)[2][4], const float (&f)[4], uint32_t (&a)[4]) {
+__device__ __forceinline__ void p_fragment(const float (&s)[4], float f0, float f1, uint32_t (&b)[2]) {
   if constexpr (BF) {
-    a[0] = pack_bf16(s[0][0] * f[0], s[0][1] * f[1]);
-    a[1] = pack_bf16(s[0][2] * f[0], s[0][3] * f[1]);
-    a[2] = pack_bf16(s[1][0] * f[2], s[1][1] * f[3]);
-    a[3] = pack_bf16(s[1][2] * f[2], s[1][3] * f[3]);
+    b[0] = transposed(pack_bf16(s[0] * f0, s[1] * f0));
+    b[1] = transposed(pack_bf16(s[2] * f1, s[3] * f1));
   } else {
-    a[0] = pack_f16(s[0][0] * f[0], s[0][1] * f[1]);
-    a[1] = pack_f16(s[0][2] * f[0], s[0][3] * f[1]);
-    a[2] = pack_f16(s[1][0] * f[2], s[1][1] * f[3]);
-    a[3] = pack_f16(s[1][2] * f[2], s[1][3] * f[3]);
+    b[0] = transposed(pack_f16(s[0] * f0, s[1] * f0));
+    b[1] = transposed(pack_f16(s[2] * f1, s[3] * f1));
   }
 }
 
-// P V of bf16 values where a probability may be 0 because the key is masked: such a key's infinities and NaN must
+// V^T P^T of bf16 values where a probability may be 0 because the key is masked: such a key's infinities and NaN must
 // not count, a visible key's must. Values that are not finite are left out of the product and put in by hand: vis has
-// 1 for the keys that the row sees, and the products of vis with marks of +inf and of -inf (NaN: both) say what to add.
-template <int MT, int NB>
-__device__ __forceinline__ void pv_special(float (&acc)[MT][NB][4], int nb, const uint32_t (&a)[MT][4],
-                                           const uint32_t (&vis)[MT][4], uint32_t b0, uint32_t b1) {
-  const auto special = [](uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; };
-  if (!__any_sync(0xffffffffu, special(b0) || special(b1))) {
+// 1 for the keys that a row sees, and the products of vis with marks of +inf and of -inf (NaN: both) say what to add.
+template <int NTL, int MB>
+__device__ __forceinline__ void pv_special(float (&acc)[NTL][MB][4], int mb, const uint32_t (&v)[4],
+                                           const uint32_t (&p)[NTL][2], const uint32_t (&vis)[NTL][2]) {
+  bool special = false;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) mma_bf16(acc[mt][nb], a[mt][0], a[mt][1], a[mt][2], a[mt][3], b0, b1);
+  for (int i = 0; i < 4; ++i) special |= (v[i] & 0x7f80u) == 0x7f80u || (v[i] & 0x7f800000u) == 0x7f800000u;
+  if (!__any_sync(0xffffffffu, special)) {
+#pragma unroll
+    for (int nt = 0; nt < NTL; ++nt) mma<true>(acc[nt][mb], v, p[nt][0], p[nt][1]);
     return;
   }
-  uint32_t b[2] = {b0, b1}, plus[2] = {0, 0}, minus[2] = {0, 0};
+  uint32_t a[4], plus[4] = {0, 0, 0, 0}, minus[4] = {0, 0, 0, 0};
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < 4; ++i) {
+    a[i] = v[i];
 #pragma unroll
     for (int sh = 0; sh < 32; sh += 16) {
-      const uint32_t x = b[i] >> sh & 0xffffu;
+      const uint32_t x = v[i] >> sh & 0xffffu;
       if ((x & 0x7f80u) != 0x7f80u) continue;
       const bool nan = (x & 0x7fu) != 0;
       if (nan || !(x & 0x8000u)) plus[i] |= 0x3f80u << sh;
       if (nan || (x & 0x8000u)) minus[i] |= 0x3f80u << sh;
-      b[i] &= ~(0xffffu << sh);
+      a[i] &= ~(0xffffu << sh);
     }
+  }
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    mma_bf16(acc[mt][nb], a[mt][0], a[mt][1], a[mt][2], a[mt][3], b[0], b[1]);
+  for (int nt = 0; nt < NTL; ++nt) {
+    mma<true>(acc[nt][mb], a, p[nt][0], p[nt][1]);
     float up[4] = {0.f, 0.f, 0.f, 0.f}, down[4] = {0.f, 0.f, 0.f, 0.f};
-    mma_bf16(up, vis[mt][0], vis[mt][1], vis[mt][2], vis[mt][3], plus[0], plus[1]);
-    mma_bf16(down, vis[mt][0], vis[mt][1], vis[mt][2], vis[mt][3], minus[0], minus[1]);
+    mma<true>(up, plus, vis[nt][0], vis[nt][1]);
+    mma<true>(down, minus, vis[nt][0], vis[nt][1]);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      if (up[e] > 0.f) acc[mt][nb][e] += INFINITY;
-      if (down[e] > 0.f) acc[mt][nb][e] -= INFINITY;
+      if (up[e] > 0.f) acc[nt][mb][e] += INFINITY;
+      if (down[e] > 0.f) acc[nt][mb][e] -= INFINITY;
     }
   }
 }
 
-template <int MT>
-__device__ __forceinline__ void visible(const float (&s)[MT][2][4], uint32_t (&vis)[MT][4]) {  // scores, before soften
+template <int NTL>
+__device__ __forceinline__ void visible(const float (&s)[NTL][4], uint32_t (&vis)[NTL][2]) {  // scores, before soften
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+  for (int nt = 0; nt < NTL; ++nt)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int j = i >> 1, h = i & 1;
-      vis[mt][i] = (s[mt][j][2 * h] != NEG ? 0x3f80u : 0u) | (s[mt][j][2 * h + 1] != NEG ? 0x3f800000u : 0u);
-    }
+    for (int j = 0; j < 2; ++j)
+      vis[nt][j] = transposed((s[nt][2 * j] != NEG ? 0x3f80u : 0u) | (s[nt][2 * j + 1] != NEG ? 0x3f800000u : 0u));
 }
 
-template <int KIND, int D, int MT, int RW>
-__global__ void __launch_bounds__(Shape<KIND, D, MT, RW>::NT)
+template <int KIND, int D, int NTL, int RW>
+__global__ void __launch_bounds__(Shape<KIND, D, NTL, RW>::NT)
     attend_kernel(const Params p) {
-  using S = Shape<KIND, D, MT, RW>;
+  using S = Shape<KIND, D, NTL, RW>;
   constexpr bool BF = S::BF;
-  constexpr int NL = S::NL, KS = S::KS, NB = S::NB;
+  constexpr int NL = S::NL, KS = S::KS, MB = S::MB;
   extern __shared__ __align__(16) uint8_t smem[];
-  uint4* const qs = reinterpret_cast<uint4*>(smem + S::WORK);
+  uint2* const qs = reinterpret_cast<uint2*>(smem + S::WORK);
   int* const before = reinterpret_cast<int*>(smem + S::SMEM);
   cudaTriggerProgrammaticLaunchCompletion();
   line_of(p, before);
@@ -326,7 +347,7 @@ __global__ void __launch_bounds__(Shape<KIND, D, MT, RW>::NT)
     const int u0 = static_cast<int>(at - base - static_cast<int64_t>(item) * per);
     const int u1 = last - at < per - u0 ? u0 + static_cast<int>(last - at) : per;
     const int h = item / p.tiles, tile = item - h * p.tiles;
-    const int row0 = tile * S::RT + rw * 16 * MT;
+    const int row0 = tile * S::RT + rw * 8 * NTL;
     const int len = length_of(p, b);
     const int unit0 = first_unit(p, len) - 1;  // unit u holds the keys from (unit0 + u) * 64 on
 
@@ -337,6 +358,8 @@ __global__ void __launch_bounds__(Shape<KIND, D, MT, RW>::NT)
     const int chunk_end = min((unit0 + u1) * KW, (len + 15) >> 4);
     int ahead = chunk, page0 = -64, pages = 0;
     bool lost = false;
+    const uint8_t* const k_lane = static_cast<const uint8_t*>(p.c.k) + key_of(g) * D * (BF ? 2 : 1) + t * 16;
+    const uint8_t* const v_lane = static_cast<const uint8_t*>(p.c.v) + t * D * (BF ? 8 : 4) + g * 16;
     const auto fetch = [&](int stage) {
       if (ahead < chunk_end) {
         const int pi = ahead >> cshift;
@@ -352,22 +375,19 @@ __global__ void __launch_bounds__(Shape<KIND, D, MT, RW>::NT)
         const int64_t cell =
             (((p.layer_cell + page) * p.heads + h) << p.page_shift) + ((ahead & ((1 << cshift) - 1)) << 4);
         const uint32_t to = ring_at + stage * S::STEP;
-        const uint8_t* k = static_cast<const uint8_t*>(p.c.k) + cell * D * (BF ? 2 : 1);
-        const uint8_t* v = static_cast<const uint8_t*>(p.c.v) + cell * D * (BF ? 2 : 1);
+        const uint8_t* k = k_lane + cell * (D * (BF ? 2 : 1));
+        const uint8_t* v = v_lane + cell * (D * (BF ? 2 : 1));
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int key = 4 * (g >> 1) + (g & 1) + 2 * j;
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int c = 0; c < NL / 2; ++c)
-            copy16(to + (j * (NL / 2) + c) * 512, k + key * D * (BF ? 2 : 1) + c * 64 + t * 16, true);
-        }
+            copy16(to + (j * (NL / 2) + c) * 512, k + j * 2 * D * (BF ? 2 : 1) + c * 64);
 #pragma unroll
-        for (int c = 0; c < NL; ++c)
-          copy16(to + (NL + c) * 512, v + (t * D + c * (BF ? 16 : 32)) * (BF ? 8 : 4) + g * 16, true);
+        for (int c = 0; c < NL; ++c) copy16(to + (NL + c) * 512, v + c * 128);
         if constexpr (!BF) {
           const uint32_t s4 = smem_u32(ring) + stage * S::STEP + 2 * NL * 512 + lane * 4;
-          copy4(s4, p.c.k_scale + cell + 4 * t, true);
-          copy4(s4 + 128, p.c.v_scale + cell + 4 * t, true);
+          copy4(s4, p.c.k_scale + cell + (g & 6) * 2);
+          copy4(s4 + 128, p.c.v_scale + cell + (g & 6) * 2);
         }
       }
       cp_async_commit();
@@ -375,154 +395,135 @@ __global__ void __launch_bounds__(Shape<KIND, D, MT, RW>::NT)
     };
     for (int i = 0; i < S::STAGES - 1; ++i) fetch(i);
 
-    // ---- Q's fragments
-    Part<KIND, D, MT, RW> part;
-    uint32_t qr[S::QREG ? MT : 1][S::QREG ? KS : 1][4];
+    // ---- Q's fragments: row g of each tile
+    Part<KIND, D, NTL, RW> part;
+    uint32_t qr[S::QREG ? NTL : 1][S::QREG ? KS : 1][2];
     const __nv_bfloat16* qb = p.q + b * p.q_seq;
-    const auto q_row = [&](int mt, int hh, bool& real) {
-      const int r = row0 + mt * 16 + hh * 8 + g;
+    const auto depth_of = [&](int nt, int e) {  // of the node of row 2t + e
+      const int r = row0 + nt * 8 + 2 * t + e;
+      return p.depth[b * p.nodes + (r < rows ? r / p.group : 0)];
+    };
+    const auto q_row = [&](int nt, bool& real) {
+      const int r = row0 + nt * 8 + g;
       real = r < rows;
       const int node = real ? r / p.group : 0;
       return qb + node * p.q_node + (h * p.group + (real ? r - node * p.group : 0)) * p.q_head;
     };
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      uint32_t frag[KS][4];
+    for (int nt = 0; nt < NTL; ++nt) {
+      bool real;
+      const __nv_bfloat16* q = q_row(nt, real);
+      uint2 x[KS];
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        bool real;
-        const __nv_bfloat16* q = q_row(mt, hh, real);
-        uint2 x[KS];
+      for (int ks = 0; ks < KS; ++ks)
+        x[ks] = real ? *reinterpret_cast<const uint2*>(q + S::dim_of(ks, t)) : make_uint2(0, 0);
+      float scale = 1.f;
+      if constexpr (!BF) {  // fp16 under a power of two: the row's largest is brought to [1, 2)
+        uint32_t top = 0;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-          x[ks] = real ? *reinterpret_cast<const uint2*>(q + S::dim_of(ks, t)) : make_uint2(0, 0);
-        part.rf[mt][hh] = p.scale_log2;
-        if constexpr (!BF) {  // fp16 under a power of two: the row's largest is brought to [1, 2)
-          uint32_t top = 0;
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
-            top = max(top, max(x[ks].x & 0x7fffu, x[ks].x >> 16 & 0x7fffu));
-            top = max(top, max(x[ks].y & 0x7fffu, x[ks].y >> 16 & 0x7fffu));
-          }
-          top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          int e = static_cast<int>(top >> 7);
-          e = e == 255 || e < 1 ? 127 : e < 67 ? 67 : e > 253 ? 253 : e;  // (not finite or zero: as it is)
-          const float f = kv::power(254 - e);
-          part.rf[mt][hh] *= kv::power(e);
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
-            frag[ks][hh] = pack_f16(low_f(x[ks].x) * f, high_f(x[ks].x) * f);
-            frag[ks][2 + hh] = pack_f16(low_f(x[ks].y) * f, high_f(x[ks].y) * f);
-          }
-        } else {
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
-            frag[ks][hh] = x[ks].x;
-            frag[ks][2 + hh] = x[ks].y;
-          }
+        for (int ks = 0; ks < KS; ++ks) {
+          top = max(top, max(x[ks].x & 0x7fffu, x[ks].x >> 16 & 0x7fffu));
+          top = max(top, max(x[ks].y & 0x7fffu, x[ks].y >> 16 & 0x7fffu));
         }
-        const int r = row0 + mt * 16 + hh * 8 + g;
-        const int node = r < rows ? r / p.group : 0;
-        part.lo[mt][hh] = p.window < 0 ? 0 : len + p.depth[b * p.nodes + node] - p.window;
-        part.m[mt][hh] = NEG;
-        part.l[mt][hh] = 0.f;
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        int e = static_cast<int>(top >> 7);
+        e = e == 255 || e < 1 ? 127 : e < 67 ? 67 : e > 253 ? 253 : e;  // (not finite or zero: as it is)
+        const float f = kv::power(254 - e);
+        scale = kv::power(e);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          x[ks].x = pack_f16(low_f(x[ks].x) * f, high_f(x[ks].x) * f);
+          x[ks].y = pack_f16(low_f(x[ks].y) * f, high_f(x[ks].y) * f);
+        }
       }
-      if constexpr (S::QREG) {
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
+      for (int e = 0; e < 2; ++e) {
+        part.rf[nt][e] = p.scale_log2 * __shfl_sync(0xffffffffu, scale, 8 * t + 4 * e);  // of row 2t + e
+        part.l[nt][e] = 0.f;
+        part.off[nt][e] = NONE;
+      }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) qr[mt][ks][i] = frag[ks][i];
-      } else if (kw == 0) {
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-          qs[((rw * MT + mt) * KS + ks) * 32 + lane] = make_uint4(frag[ks][0], frag[ks][1], frag[ks][2], frag[ks][3]);
+      for (int ks = 0; ks < KS; ++ks) {
+        if constexpr (S::QREG) qr[nt][ks][0] = x[ks].x, qr[nt][ks][1] = x[ks].y;
+        else if (kw == 0) qs[((rw * NTL + nt) * KS + ks) * 32 + lane] = x[ks];
       }
     }
     if constexpr (!S::QREG) __syncthreads();
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int nt = 0; nt < NTL; ++nt)
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
+      for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) part.acc[mt][nb][e] = 0.f;
+        for (int e = 0; e < 4; ++e) part.acc[nt][mb][e] = 0.f;
     part.vref = BF ? 127 : VREF;
 
     // ---- the tree's own keys: 16 nodes a warp, unquantised, in bf16
     if (u0 == 0 && kw * 16 < p.nodes) {
-      float s[MT][2][4];
+      float s[NTL][4];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int nt = 0; nt < NTL; ++nt)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[mt][j][e] = 0.f;
+        for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
       const __nv_bfloat16* kb = p.k + b * p.k_seq + h * p.k_head;
       const __nv_bfloat16* vb = p.v + b * p.v_seq + h * p.v_head;
+      int node2[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) node2[j] = kw * 16 + key_of(g) + 2 * j;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         uint2 kk[2];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int node = kw * 16 + 4 * (g >> 1) + (g & 1) + 2 * j;
-          kk[j] = node < p.nodes ? *reinterpret_cast<const uint2*>(kb + node * p.k_node + S::dim_of(ks, t))
-                                 : make_uint2(0, 0);
-        }
+        for (int j = 0; j < 2; ++j)
+          kk[j] = node2[j] < p.nodes ? *reinterpret_cast<const uint2*>(kb + node2[j] * p.k_node + S::dim_of(ks, t))
+                                     : make_uint2(0, 0);
+        const uint32_t a[4] = {kk[0].x, kk[1].x, kk[0].y, kk[1].y};
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          uint32_t a[4];
-#pragma unroll
-          for (int hh = 0; hh < 2; ++hh) {
-            bool real;
-            const __nv_bfloat16* q = q_row(mt, hh, real);
-            const uint2 x = real ? *reinterpret_cast<const uint2*>(q + S::dim_of(ks, t)) : make_uint2(0, 0);
-            a[hh] = x.x;
-            a[2 + hh] = x.y;
-          }
-#pragma unroll
-          for (int j = 0; j < 2; ++j) mma_bf16(s[mt][j], a[0], a[1], a[2], a[3], kk[j].x, kk[j].y);
+        for (int nt = 0; nt < NTL; ++nt) {
+          bool real;
+          const __nv_bfloat16* q = q_row(nt, real);
+          const uint2 x = real ? *reinterpret_cast<const uint2*>(q + S::dim_of(ks, t)) : make_uint2(0, 0);
+          mma<true>(s[nt], a, x.x, x.y);
         }
       }
-      int dk[4];
+      int dk[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int node = kw * 16 + 4 * t + i;
-        dk[i] = node < p.nodes ? p.depth[b * p.nodes + node] : 0;
-      }
+      for (int j = 0; j < 2; ++j) dk[j] = node2[j] < p.nodes ? p.depth[b * p.nodes + node2[j]] : 0;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int nt = 0; nt < NTL; ++nt)
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-          const int r = row0 + mt * 16 + hh * 8 + g;
+        for (int e = 0; e < 2; ++e) {
+          const int r = row0 + nt * 8 + 2 * t + e;
           const int node = r < rows ? r / p.group : 0;
           const uint64_t mask = r < rows ? p.mask[b * p.nodes + node] : 0;
-          const float f = p.scale_log2 / part.rf[mt][hh];  // scores in the units of the cached keys' (a power of two)
+          const int reach = p.window < 0 ? 0 : depth_of(nt, e) - p.window;
+          const float f = p.scale_log2 / part.rf[nt][e];  // scores in the units of the cached keys' (a power of two)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int key = kw * 16 + 4 * t + i;
-            // lo - len = depth - window
-            const bool see = key < p.nodes && (mask >> key & 1) && (p.window < 0 || dk[i] >= part.lo[mt][hh] - len);
-            float& x = s[mt][i >> 1][2 * hh + (i & 1)];
-            x = see ? x * f : NEG;
+          for (int j = 0; j < 2; ++j) {
+            const bool see = node2[j] < p.nodes && (mask >> node2[j] & 1) && (p.window < 0 || dk[j] >= reach);
+            s[nt][2 * j + e] = see ? s[nt][2 * j + e] * f : NEG;
           }
         }
-      uint32_t vis[MT][4], a[MT][4];
-      visible<MT>(s, vis);
+      uint32_t vis[NTL][2], pf[NTL][2];
+      visible<NTL>(s, vis);
       part.soften(s, part.vref);
       constexpr float UNITS = BF ? 1.f : 1048576.f;  // 1 in units of 2^(VREF - 127)
-      const float one[4] = {UNITS, UNITS, UNITS, UNITS};
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) p_fragment<true>(s[mt], one, a[mt]);
+      for (int nt = 0; nt < NTL; ++nt) p_fragment<true>(s[nt], UNITS, UNITS, pf[nt]);
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const int d = BF ? (nb >> 1) * 16 + 2 * g + (nb & 1) : (nb >> 2) * 32 + 4 * g + (nb & 3);
-        uint32_t w[4];
+      for (int mb = 0; mb < MB; ++mb) {
+        const int d = BF ? mb * 16 + 2 * g : (mb >> 1) * 32 + 4 * g + (mb & 1) * 2;  // and d + 1
+        uint32_t w[2][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int node = kw * 16 + 4 * t + i;
-          w[i] = node < p.nodes ? __ldg(reinterpret_cast<const unsigned short*>(vb + node * p.v_node + d)) : 0u;
+          const unsigned short* from = reinterpret_cast<const unsigned short*>(vb + node * p.v_node + d);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) w[j][i] = node < p.nodes ? __ldg(from + j) : 0u;
         }
-        pv_special<MT, NB>(part.acc, nb, a, vis, w[0] | w[1] << 16, w[2] | w[3] << 16);
+        const uint32_t v4[4] = {w[0][0] | w[0][1] << 16, w[1][0] | w[1][1] << 16, w[0][2] | w[0][3] << 16,
+                                w[1][2] | w[1][3] << 16};
+        pv_special<NTL, MB>(part.acc, mb, v4, pf, vis);
       }
     }
 
@@ -533,13 +534,11 @@ __global__ void __launch_bounds__(Shape<KIND, D, MT, RW>::NT)
       fetch(stage == 0 ? S::STAGES - 1 : stage - 1);  // the step read last is free
       const uint8_t* step = ring + stage * S::STEP;
       const uint4* own = reinterpret_cast<const uint4*>(step) + lane;
-      float s[MT][2][4];
+      float s[NTL][4];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int nt = 0; nt < NTL; ++nt)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[mt][j][e] = 0.f;
+        for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
 #pragma unroll
       for (int c = 0; c < NL / 2; ++c) {
         constexpr int PER = BF ? 2 : 4;  // steps in 16 bytes
@@ -552,29 +551,20 @@ __global__ void __launch_bounds__(Shape<KIND, D, MT, RW>::NT)
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
           const int ks = c * PER + i;
-          uint32_t kk[2][2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            if constexpr (BF) {
-              kk[j][0] = w[j][2 * i], kk[j][1] = w[j][2 * i + 1];
-            } else {
-              kv::decode4<KIND>(w[j][i], kk[j][0], kk[j][1]);
-            }
+          uint32_t a[4];
+          if constexpr (BF) {
+            a[0] = w[0][2 * i], a[1] = w[1][2 * i], a[2] = w[0][2 * i + 1], a[3] = w[1][2 * i + 1];
+          } else {
+            kv::decode4<KIND>(w[0][i], a[0], a[2]);
+            kv::decode4<KIND>(w[1][i], a[1], a[3]);
           }
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            uint32_t a[4];
+          for (int nt = 0; nt < NTL; ++nt) {
             if constexpr (S::QREG) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) a[e] = qr[mt][ks][e];
+              mma<BF>(s[nt], a, qr[nt][ks][0], qr[nt][ks][1]);
             } else {
-              const uint4 u = qs[((rw * MT + mt) * KS + ks) * 32 + lane];
-              a[0] = u.x, a[1] = u.y, a[2] = u.z, a[3] = u.w;
-            }
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              if constexpr (BF) mma_bf16(s[mt][j], a[0], a[1], a[2], a[3], kk[j][0], kk[j][1]);
-              else mma_f16(s[mt][j], a, kk[j][0], kk[j][1]);
+              const uint2 x = qs[((rw * NTL + nt) * KS + ks) * 32 + lane];
+              mma<BF>(s[nt], a, x.x, x.y);
             }
           }
         }
@@ -582,106 +572,76 @@ __global__ void __launch_bounds__(Shape<KIND, D, MT, RW>::NT)
       const int key0 = chunk << 4;
       // some key is past the end, or before the window of the deepest node there could be
       const bool edge = key0 + 16 > len || (p.window >= 0 && key0 < len + p.nodes - p.window);
-      uint32_t vb4 = 0;
-      bool nan_v = false;
+      uint32_t vb0 = 0, vb1 = 0;  // V's scale bytes of keys g and g + 8
       if constexpr (!BF) {
-        const uint32_t kb4 = reinterpret_cast<const uint32_t*>(step + 2 * NL * 512)[lane];
-        vb4 = reinterpret_cast<const uint32_t*>(step + 2 * NL * 512)[32 + lane];
+        const uint32_t* sc = reinterpret_cast<const uint32_t*>(step + 2 * NL * 512) + lane;
+        const uint32_t kb = sc[0] >> (8 * (g & 1)), vb = sc[32] >> (8 * (g & 1));
+        vb0 = vb & 0xffu, vb1 = vb >> 16 & 0xffu;
+        // byte 255 gives infinity, times the row's zero codes NaN
+        const float f0 = __uint_as_float((kb & 0xffu) << 23), f1 = __uint_as_float((kb & 0xff0000u) << 7);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t kbyte = kb4 >> (8 * i) & 0xffu;
-          const float f = kbyte == 255 ? __int_as_float(0x7fc00000) : kv::power(kbyte);
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            s[mt][i >> 1][i & 1] *= f;
-            s[mt][i >> 1][2 + (i & 1)] *= f;
-          }
-        }
+        for (int nt = 0; nt < NTL; ++nt) s[nt][0] *= f0, s[nt][1] *= f0, s[nt][2] *= f1, s[nt][3] *= f1;
       }
-      uint32_t keep = 0xffffffffu;  // a byte for each of the lane's four keys that exist
+      uint32_t keep = 0xffffffffu;  // a byte for each of quad t's keys that exist
       if (edge) {
-        const int k0 = key0 + 4 * t, left = len - k0;
-        keep = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : 0xffffffffu >> (32 - 8 * left);
-        vb4 &= keep;
+        const int left4 = len - key0 - 4 * t, k0 = key0 + key_of(g);
+        keep = left4 >= 4 ? 0xffffffffu : left4 <= 0 ? 0u : 0xffffffffu >> (32 - 8 * left4);
+        if (k0 >= len) vb0 = 0;
+        if (k0 + 2 >= len) vb1 = 0;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int nt = 0; nt < NTL; ++nt)
 #pragma unroll
-          for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (i >= left || k0 + i < part.lo[mt][hh]) s[mt][i >> 1][2 * hh + (i & 1)] = NEG;
-      }
-      float f[4] = {1.f, 1.f, 1.f, 1.f};
-      int ref = part.vref;
-      if constexpr (!BF) {
-        uint32_t top = __vmaxu4(vb4, vb4 >> 16);
-        top = max(top & 0xffu, top >> 8 & 0xffu);
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        if (top == 255) {  // a row of V that reads as NaN: such keys are taken out here, and put into the sum below
-          nan_v = true;
-          top = 0;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t x = vb4 >> (8 * i) & 0xffu;
-            top = max(top, x == 255 ? 0u : x);
+          for (int e = 0; e < 2; ++e) {
+            const int low = p.window < 0 ? 0 : len + depth_of(nt, e) - p.window;
+            if (k0 >= len || k0 < low) s[nt][e] = NEG;
+            if (k0 + 2 >= len || k0 + 2 < low) s[nt][2 + e] = NEG;
           }
-          top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        }
-        ref = max(ref, static_cast<int>(top));
       }
-      uint32_t vis[BF ? MT : 1][4];
+      uint32_t vis[BF ? NTL : 1][2];
+      float f0 = 1.f, f1 = 1.f;
       if constexpr (BF) {
-        if (edge) visible<MT>(s, vis);
-      }
-      if (nan_v) {
+        if (edge) visible<NTL>(s, vis);
+        part.soften(s, part.vref);
+      } else {
+        if (__any_sync(0xffffffffu, vb0 == 255 || vb1 == 255)) {
+          // rows of V that read as NaN: taken out of the product (codes 0, factor 0) and put into the sums
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if ((vb4 >> (8 * i) & 0xffu) == 255) {
+          for (int nt = 0; nt < NTL; ++nt)
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-              for (int hh = 0; hh < 2; ++hh)
-                if (s[mt][i >> 1][2 * hh + (i & 1)] != NEG) part.l[mt][hh] = __int_as_float(0x7fc00000);
-          }
-      }
-      part.soften(s, ref);
-      if constexpr (!BF) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int x = static_cast<int>(vb4 >> (8 * i) & 0xffu), e = x - ref + 127;
-          f[i] = x == 255 || e <= 0 ? 0.f : kv::power(e);
+            for (int e = 0; e < 4; ++e)
+              if ((e & 2 ? vb1 : vb0) == 255 && s[nt][e] != NEG) part.l[nt][e & 1] = __int_as_float(0x7fc00000);
+          if (vb0 == 255) vb0 = 0;
+          if (vb1 == 255) vb1 = 0;
         }
+        part.soften(s, static_cast<int>(max(vb0, vb1)));
+        f0 = kv::power(max(static_cast<int>(vb0) - part.vref + 127, 0));
+        f1 = kv::power(max(static_cast<int>(vb1) - part.vref + 127, 0));
       }
-      uint32_t a[MT][4];
+      uint32_t pf[NTL][2];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) p_fragment<BF>(s[mt], f, a[mt]);
+      for (int nt = 0; nt < NTL; ++nt) p_fragment<BF>(s[nt], f0, f1, pf[nt]);
 #pragma unroll
       for (int c = 0; c < NL; ++c) {
         const uint4 u = own[(NL + c) * 32];
         uint32_t w[4] = {u.x, u.y, u.z, u.w};
-        if constexpr (BF) {
+        if constexpr (BF) {  // dimensions 2g, 2g + 1 of 16: words keys 01, 23 of the one, then of the other
+          const uint32_t a[4] = {w[0], w[2], w[1], w[3]};
           if (edge) {
             const uint32_t lo = __byte_perm(keep, 0, 0x1100), hi = __byte_perm(keep, 0, 0x3322);
-            w[0] &= lo, w[1] &= hi, w[2] &= lo, w[3] &= hi;
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-              pv_special<MT, NB>(part.acc, c * 2 + i, a, vis, w[2 * i], w[2 * i + 1]);
+            const uint32_t a2[4] = {a[0] & lo, a[1] & lo, a[2] & hi, a[3] & hi};
+            pv_special<NTL, MB>(part.acc, c, a2, pf, vis);
           } else {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-              for (int mt = 0; mt < MT; ++mt)
-                mma_bf16(part.acc[mt][c * 2 + i], a[mt][0], a[mt][1], a[mt][2], a[mt][3], w[2 * i], w[2 * i + 1]);
+            for (int nt = 0; nt < NTL; ++nt) mma<true>(part.acc[nt][c], a, pf[nt][0], pf[nt][1]);
           }
-        } else {
+        } else {  // dimensions 4g .. 4g + 3 of 32
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t b0, b1;
-            kv::decode4<KIND>(w[i] & keep, b0, b1);
+          for (int i = 0; i < 2; ++i) {
+            uint32_t a[4];
+            kv::decode4<KIND>(w[2 * i] & keep, a[0], a[2]);
+            kv::decode4<KIND>(w[2 * i + 1] & keep, a[1], a[3]);
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) mma_f16(part.acc[mt][c * 4 + i], a[mt], b0, b1);
+            for (int nt = 0; nt < NTL; ++nt) mma<false>(part.acc[nt][2 * c + i], a, pf[nt][0], pf[nt][1]);
           }
         }
       }
@@ -691,65 +651,63 @@ __global__ void __launch_bounds__(Shape<KIND, D, MT, RW>::NT)
     if (lost) {
       record_error(p.c.status, NOISE_DEV_BAD_INDEX);
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) part.l[mt][0] = part.l[mt][1] = __int_as_float(0x7fc00000);
+      for (int nt = 0; nt < NTL; ++nt) part.l[nt][0] = part.l[nt][1] = __int_as_float(0x7fc00000);
     }
 
     // ---- the warps' parts joined: those of the upper half handed to the lower, then 1 to 0
-    if constexpr (!BF) {
-      const float unit = ex2(static_cast<float>(part.vref - 127));
+    const float unit = BF ? 1.f : ex2(static_cast<float>(part.vref - 127));
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+    for (int nt = 0; nt < NTL; ++nt) {
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
+      for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) part.acc[mt][nb][e] *= unit;
-    }
+        for (int e = 0; e < 4; ++e) part.acc[nt][mb][e] *= unit;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        float x = part.l[mt][hh];
-        x += __shfl_xor_sync(0xffffffffu, x, 1);
-        part.l[mt][hh] = x + __shfl_xor_sync(0xffffffffu, x, 2);
+      for (int e = 0; e < 2; ++e) {
+        float x = part.l[nt][e];
+        x += __shfl_xor_sync(0xffffffffu, x, 4);
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        part.l[nt][e] = x + __shfl_xor_sync(0xffffffffu, x, 16);
       }
+    }
 #pragma unroll
     for (int from = KW / 2; from >= 1; from >>= 1) {
       __syncthreads();  // everyone is done with the ring, or with the last round's hand-over
       float4* slab = reinterpret_cast<float4*>(smem + (rw * 2 + kw % from) * S::JOIN) + lane;
       if (kw >= from && kw < 2 * from) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+        for (int nt = 0; nt < NTL; ++nt) {
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
-            slab[(mt * NB + nb) * 32] =
-                make_float4(part.acc[mt][nb][0], part.acc[mt][nb][1], part.acc[mt][nb][2], part.acc[mt][nb][3]);
-          slab[(MT * NB + mt) * 32] = make_float4(part.m[mt][0], part.m[mt][1], part.l[mt][0], part.l[mt][1]);
+          for (int mb = 0; mb < MB; ++mb)
+            slab[(nt * MB + mb) * 32] =
+                make_float4(part.acc[nt][mb][0], part.acc[nt][mb][1], part.acc[nt][mb][2], part.acc[nt][mb][3]);
+          slab[(NTL * MB + nt) * 32] = make_float4(part.off[nt][0], part.off[nt][1], part.l[nt][0], part.l[nt][1]);
         }
       }
       __syncthreads();
       if (kw < from) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          const float4 o = slab[(MT * NB + mt) * 32];
-          const float om[2] = {o.x, o.y}, ol[2] = {o.z, o.w};
+        for (int nt = 0; nt < NTL; ++nt) {
+          const float4 o = slab[(NTL * MB + nt) * 32];
+          const float oo[2] = {o.x, o.y}, ol[2] = {o.z, o.w};
           float mine[2], theirs[2];
 #pragma unroll
-          for (int hh = 0; hh < 2; ++hh) {
-            const float top = fmaxf(part.m[mt][hh], om[hh]);
-            mine[hh] = part.m[mt][hh] == NEG ? 0.f : ex2((part.m[mt][hh] - top) * part.rf[mt][hh]);
-            theirs[hh] = om[hh] == NEG ? 0.f : ex2((om[hh] - top) * part.rf[mt][hh]);
+          for (int e = 0; e < 2; ++e) {
+            const float off = fminf(part.off[nt][e], oo[e]);
+            mine[e] = part.off[nt][e] == NONE ? 0.f : ex2(off - part.off[nt][e]);
+            theirs[e] = oo[e] == NONE ? 0.f : ex2(off - oo[e]);
             // a row that saw no key may still hold the NaN of a lost page
-            part.l[mt][hh] = (part.m[mt][hh] == NEG ? part.l[mt][hh] : part.l[mt][hh] * mine[hh]) +
-                             (om[hh] == NEG ? ol[hh] : ol[hh] * theirs[hh]);
-            part.m[mt][hh] = top;
+            part.l[nt][e] = (part.off[nt][e] == NONE ? part.l[nt][e] : part.l[nt][e] * mine[e]) +
+                            (oo[e] == NONE ? ol[e] : ol[e] * theirs[e]);
+            part.off[nt][e] = off;
           }
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            const float4 x = slab[(mt * NB + nb) * 32];
-            part.acc[mt][nb][0] = part.acc[mt][nb][0] * mine[0] + x.x * theirs[0];
-            part.acc[mt][nb][1] = part.acc[mt][nb][1] * mine[0] + x.y * theirs[0];
-            part.acc[mt][nb][2] = part.acc[mt][nb][2] * mine[1] + x.z * theirs[1];
-            part.acc[mt][nb][3] = part.acc[mt][nb][3] * mine[1] + x.w * theirs[1];
+          for (int mb = 0; mb < MB; ++mb) {
+            const float4 x = slab[(nt * MB + mb) * 32];
+            part.acc[nt][mb][0] = part.acc[nt][mb][0] * mine[0] + x.x * theirs[0];
+            part.acc[nt][mb][1] = part.acc[nt][mb][1] * mine[1] + x.y * theirs[1];
+            part.acc[nt][mb][2] = part.acc[nt][mb][2] * mine[0] + x.z * theirs[0];
+            part.acc[nt][mb][3] = part.acc[nt][mb][3] * mine[1] + x.w * theirs[1];
           }
         }
       }
@@ -760,41 +718,37 @@ __global__ void __launch_bounds__(Shape<KIND, D, MT, RW>::NT)
       float* po = p.partial + static_cast<int64_t>(slot) * S::RT * D;
       float* pm = p.partial + static_cast<int64_t>(2 * p.grid) * S::RT * D + static_cast<int64_t>(slot) * 2 * S::RT;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int nt = 0; nt < NTL; ++nt)
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-          const int in = rw * 16 * MT + mt * 16 + hh * 8 + g, r = tile * S::RT + in;
+        for (int e = 0; e < 2; ++e) {
+          const int in = rw * 8 * NTL + nt * 8 + 2 * t + e, r = tile * S::RT + in;
           if (r >= rows) continue;
           const int node = r / p.group;
           const bool pad = p.depth[b * p.nodes + node] < 0;
-          const float l = part.l[mt][hh];
+          const float l = part.l[nt][e];
           const float f = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
           __nv_bfloat16* out =
               p.out + ((static_cast<int64_t>(b) * p.nodes + node) * p.heads * p.group + h * p.group + r - node * p.group) * D;
-          if (!whole && t == 0) {
-            pm[in] = part.m[mt][hh] * part.rf[mt][hh];
+          if (!whole && g == 0) {
+            pm[in] = part.off[nt][e];
             pm[S::RT + in] = l;
           }
-          constexpr int RUN = BF ? 2 : 4;  // the lane's consecutive dimensions: 2 RUN
+          constexpr int RUN = BF ? 1 : 2;  // tiles of 16 whose dimensions g, g + 8 are the lane's 2 RUN consecutive ones
 #pragma unroll
-          for (int c = 0; c < NB / RUN; ++c) {
+          for (int c = 0; c < MB / RUN; ++c) {
             float x[2 * RUN];
 #pragma unroll
             for (int i = 0; i < RUN; ++i) {
-              x[i] = pad ? 0.f : part.acc[mt][c * RUN + i][2 * hh] * f;
-              x[RUN + i] = pad ? 0.f : part.acc[mt][c * RUN + i][2 * hh + 1] * f;
+              x[2 * i] = pad ? 0.f : part.acc[nt][c * RUN + i][e] * f;
+              x[2 * i + 1] = pad ? 0.f : part.acc[nt][c * RUN + i][2 + e] * f;
             }
-            const int d = c * 8 * RUN + t * 2 * RUN;
-            if (whole) {
-              if constexpr (BF)
-                *reinterpret_cast<uint2*>(out + d) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
-              else
-                *reinterpret_cast<uint4*>(out + d) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]),
-                                                                pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+            const int d = c * 16 * RUN + g * 2 * RUN;
+            if constexpr (BF) {
+              if (whole) *reinterpret_cast<uint32_t*>(out + d) = pack_bf16(x[0], x[1]);
+              else *reinterpret_cast<float2*>(po + in * D + d) = make_float2(x[0], x[1]);
             } else {
-#pragma unroll
-              for (int i = 0; i < 2 * RUN; i += 4)
-                *reinterpret_cast<float4*>(po + in * D + d + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+              if (whole) *reinterpret_cast<uint2*>(out + d) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+              else *reinterpret_cast<float4*>(po + in * D + d) = make_float4(x[0], x[1], x[2], x[3]);
             }
           }
         }
@@ -805,7 +759,7 @@ __global__ void __launch_bounds__(Shape<KIND, D, MT, RW>::NT)
   }
 }
 
-// Joins the parts of one item (a block each): o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i, in the parts' order.
+// Joins the parts of one item (a block each): o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i (off = -m), in the parts' order.
 __global__ void __launch_bounds__(256) join_kernel(const Params p, int rt, int dim) {
   extern __shared__ int before[];
   line_of(p, before);
@@ -825,18 +779,18 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p, int rt, int d
     const int in = i / quads, d = (i - in * quads) * 4, r = tile * rt + in;
     if (r >= rows) return;
     const int node = r / p.group;
-    float top = NEG;
+    float off = NONE;
     for (int c = c0; c <= c1; ++c)
-      top = fmaxf(top, sums[static_cast<int64_t>(c == c0 ? slot0 : 2 * c) * 2 * rt + in]);
+      off = fminf(off, sums[static_cast<int64_t>(c == c0 ? slot0 : 2 * c) * 2 * rt + in]);
     float l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
     for (int c = c0; c <= c1; ++c) {
       const int64_t slot = c == c0 ? slot0 : 2 * c;
-      const float m = sums[slot * 2 * rt + in], sl = sums[slot * 2 * rt + rt + in];
+      const float oo = sums[slot * 2 * rt + in], sl = sums[slot * 2 * rt + rt + in];
       const float4 x = *reinterpret_cast<const float4*>(p.partial + (slot * rt + in) * dim + d);
-      const float f = m == NEG ? 0.f : ex2(m - top);
-      l += m == NEG ? sl : sl * f;
+      const float f = oo == NONE ? 0.f : ex2(off - oo);
+      l += oo == NONE ? sl : sl * f;
       o.x += x.x * f, o.y += x.y * f, o.z += x.z * f, o.w += x.w * f;
     }
     const bool none = l == 0.f || p.depth[b * p.nodes + node] < 0;
@@ -852,8 +806,8 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p, int rt, int d
 
 constexpr int MAX_GRID = 148 * 8;
 
-// The row tile and grid of a call: 16 rows a tile where they hold all, else 32, else 64.
-inline int tile_rows(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+// The row tile of a call: the least of 8, 16, 32 and 64 rows that holds all, or 64.
+inline int tile_rows(int rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 
 inline int sm_count() {
   int dev = 0, n = 0;
@@ -862,10 +816,10 @@ inline int sm_count() {
   return n;
 }
 
-template <int KIND, int D, int MT, int RW>
+template <int KIND, int D, int NTL, int RW>
 int run(Params& p, size_t workspace_bytes, cudaStream_t s) {
-  using S = Shape<KIND, D, MT, RW>;
-  const auto kernel = attend_kernel<KIND, D, MT, RW>;
+  using S = Shape<KIND, D, NTL, RW>;
+  const auto kernel = attend_kernel<KIND, D, NTL, RW>;
   const int smem = S::SMEM + (p.seqs + 1) * 4;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM + (MAX_SEQS + 1) * 4) !=
       cudaSuccess)
@@ -901,9 +855,10 @@ int run(Params& p, size_t workspace_bytes, cudaStream_t s) {
 template <int KIND, int D>
 int by_rows(Params& p, size_t bytes, cudaStream_t s) {
   const int rows = p.nodes * p.group;
-  if (rows <= 16) return run<KIND, D, 1, 1>(p, bytes, s);
-  if (rows <= 32) return run<KIND, D, 2, 1>(p, bytes, s);
-  return run<KIND, D, 2, 2>(p, bytes, s);
+  if (rows <= 8) return run<KIND, D, 1, 1>(p, bytes, s);
+  if (rows <= 16) return run<KIND, D, 2, 1>(p, bytes, s);
+  if (rows <= 32) return run<KIND, D, 4, 1>(p, bytes, s);
+  return run<KIND, D, 4, 2>(p, bytes, s);
 }
 
 template <int KIND>
