@@ -797,7 +797,7 @@ int noise_tree_plan(const int* parents, int seqs, int nodes, int64_t* mask, int*
  * mask[b, n], those at most `window` positions back (window < 0: all). depth >= 0 for a real node; a depth below 0
  * marks padding, whose output is 0; so is that of a row that sees nothing.
  *   q [seqs, nodes, q_heads, dim], k, v [seqs, nodes, heads, dim] bf16, the last dimension contiguous (strides in
- *   elements, of q and k multiples of 4; q 16-byte, k 8-byte aligned); q_heads a multiple of the cache's heads; table int32
+ *   elements, multiples of 8; 16-byte aligned); q_heads a multiple of the cache's heads; table int32
  *   [seqs, width]; lengths int32 [seqs] (taken as between 0 and width * page_size); out bf16 [seqs, nodes, q_heads,
  *   dim]. nodes at most 64, seqs at most 4096, q_heads / heads at most 64, scale from 1e-18 to 1e18. A page out of
  *   range makes its sequence's outputs NaN and sets the cache's status. workspace:

@@ -8,9 +8,9 @@
 //
 // A cached key costs D codes of K and of V and 4 D operations a row: with up to some 64 rows of 8-bit codes the
 // kernel is bound by the cache's bytes. So it is built to stream them:
-//  - Each warp walks the keys 16 at a time and keeps a running maximum, sum and output (32 bits) for its rows. A lane
-//    copies its own fragments (cp.async, 16 bytes each, a ring of STAGES steps) and reads back only what it copied
-//    itself: no barrier, and the loads of the next steps stay in flight while a step computes.
+//  - Each warp walks the keys 16 or 32 at a time and keeps a running maximum, sum and output (32 bits) for its rows. It
+//    copies its own steps (cp.async, a ring of STAGES of them), no other warp waits for it, and the next steps stay
+//    in flight while one computes.
 //  - Keys are the products' 16 rows (S^T = K Q^T, O^T = V^T P^T) and query rows their 8 columns, so a decoding step of
 //    up to 8 rows wastes no more than its own rounding to 8. P passes from one product to the other by a transpose of
 //    8 x 8 tiles in registers.
@@ -18,7 +18,7 @@
 //    consecutive bytes of a key's row, for V^T P^T four neighbouring keys of one dimension, which lie in one word of V's
 //    layout; codes become fp16 in registers.
 //  - The running maximum moves only when a score passes it by 2^8: a vote a step instead of a reduction over its keys.
-//  - The keys of all sequences, heads and row tiles form one line of units of 64 keys, cut into equal spans, one a
+//  - The keys of all sequences, heads and row tiles form one line of units of 64 or 128 keys, cut into equal spans, one a
 //    CTA, whatever the lengths are. Parts of an item are joined by a second kernel.
 // Roundings: Q to fp16 under a power of two per row (an element loses bits only below 2^-14 of the row's largest),
 // P 2^(scale of V) to fp16 relative to the largest scale seen; for a bf16 cache and for the nodes' own bf16 keys, P
@@ -34,9 +34,8 @@
 namespace noise {
 namespace tree {
 
-constexpr int KW = 4;            // warps that share a row tile's keys: a unit is 16 keys of each
-constexpr int UNIT = 16 * KW;
-constexpr int MAX_SEQS = 4096;
+constexpr int KW = 4;            // warps that share a row tile's keys: a unit is one step of each
+constexpr int MAX_SEQS = 4096;  // two words each in shared memory
 constexpr int VREF = 127 - 20;   // the output's first unit is 2^-20: V rows with less than that as a scale lose bits
 constexpr float NEG = -INFINITY;
 
@@ -54,6 +53,7 @@ struct Params {
   __nv_bfloat16* out;
   float* partial;  // [2 * grid][RT][D] then m, l [2 * grid][RT]
   int seqs, nodes, group, heads, width, window, page_shift, tiles, grid;
+  int unit_shift;  // log2 of a unit's keys
   float scale_log2;
 };
 
@@ -85,6 +85,9 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
+__device__ __forceinline__ void copy8(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -108,32 +111,33 @@ __device__ __forceinline__ int length_of(const Params& p, int b) {
   return len < 0 ? 0 : len > room ? static_cast<int>(room) : len;
 }
 
-// First unit of 64 keys that some node's window reaches (the least depth of a real node is 0).
+// First unit of keys that some node's window reaches (the least depth of a real node is 0).
 __device__ __forceinline__ int first_unit(const Params& p, int len) {
-  return p.window < 0 || p.window >= len ? 0 : (len - p.window) / UNIT;
+  return p.window < 0 || p.window >= len ? 0 : (len - p.window) >> p.unit_shift;
 }
 
-// Units of one item of sequence b: one for its nodes, then its cached keys'.
-__device__ __forceinline__ int units_of(const Params& p, int b) {
-  const int len = length_of(p, b);
-  return 1 + (len + UNIT - 1) / UNIT - first_unit(p, len);
+// Units of one item of a sequence: one for its nodes, then its cached keys'.
+__device__ __forceinline__ int units_of(const Params& p, int len) {
+  return 1 + ((len + (1 << p.unit_shift) - 1) >> p.unit_shift) - first_unit(p, len);
 }
 
-// before[b] = units of one item of each sequence before b; every thread of the block calls it.
-__device__ __forceinline__ void line_of(const Params& p, int* before) {
-  for (int b = threadIdx.x; b < p.seqs; b += blockDim.x) before[b + 1] = units_of(p, b);
-  __syncthreads();
+// before[b] = units of one item of each sequence before b, lens[b] its length; every thread of the block calls it.
+__device__ __forceinline__ void line_of(const Params& p, int* before, int* lens) {
   if (threadIdx.x < 32) {
     int carry = 0;
     for (int b0 = 0; b0 < p.seqs; b0 += 32) {
       const int b = b0 + threadIdx.x;
-      int x = b < p.seqs ? before[b + 1] : 0;
+      const int len = b < p.seqs ? length_of(p, b) : 0;
+      int x = b < p.seqs ? units_of(p, len) : 0;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, x, o);
         if (static_cast<int>(threadIdx.x) >= o) x += y;
       }
-      if (b < p.seqs) before[b + 1] = carry + x;
+      if (b < p.seqs) {
+        before[b + 1] = carry + x;
+        lens[b] = len;
+      }
       carry += __shfl_sync(0xffffffffu, x, 31);
     }
     if (threadIdx.x == 0) before[0] = 0;
@@ -141,20 +145,20 @@ __device__ __forceinline__ void line_of(const Params& p, int* before) {
   __syncthreads();
 }
 
-struct Spans {  // CTA i takes units [cut(i), cut(i + 1))
-  int64_t total;
-  int ctas;
+// CTA i takes units [cut(i), cut(i + 1)): each `each` of them, the first `more` one more. (The host made sure that all
+// of them are fewer than 2^31.)
+struct Spans {
+  int ctas, each, more;
   __device__ __forceinline__ Spans(const Params& p, const int* before) {
-    total = static_cast<int64_t>(before[p.seqs]) * p.heads * p.tiles;
-    const int64_t most = total / 2;  // at least two units each: a shorter span is all overhead
-    ctas = most < 1 ? 1 : most < p.grid ? static_cast<int>(most) : p.grid;
+    const int total = before[p.seqs] * p.heads * p.tiles;
+    ctas = min(p.grid, max(1, total >> 1));  // at least two units each: a shorter span is all overhead
+    each = total / ctas;
+    more = total - each * ctas;
   }
-  __device__ __forceinline__ int64_t cut(int i) const { return total * i / ctas; }
-  __device__ __forceinline__ int owner(int64_t u) const {  // the CTA whose span holds unit u
-    int i = static_cast<int>(u * ctas / total);
-    while (cut(i) > u) --i;
-    while (cut(i + 1) <= u) ++i;
-    return i;
+  __device__ __forceinline__ int cut(int i) const { return each * i + min(i, more); }
+  __device__ __forceinline__ int owner(int u) const {  // the CTA whose span holds unit u
+    const int large = more * (each + 1);
+    return u < large ? u / (each + 1) : more + (u - large) / each;
   }
 };
 
@@ -169,14 +173,36 @@ struct Shape {
   static constexpr int NL = BF ? D / 16 : D / 32;    // 16-byte loads a lane of K, and of V
   static constexpr int NT = 32 * KW * RW;
   static constexpr int RT = 8 * NTL * RW;
-  static constexpr int STEP = 2 * NL * 512 + (BF ? 0 : 256);  // bytes of a warp's 16 keys
-  static constexpr int STAGES = STEP <= 2500 ? 4 : 3;
+  static constexpr int G = BF || NTL > 2 || D == 128 ? 1 : 2;  // groups of 16 keys a step: about 4 KB
+  static constexpr int CHAINS = NTL * G == 1 ? 2 : 1;  // sums of K Q^T side by side: one alone waits on itself
+  static constexpr int BLOCK = 2 * NL * 512 + (BF ? 0 : 256);  // bytes of 16 keys
+  static constexpr int STEP = G * BLOCK;
+  static constexpr int STAGES = STEP <= 2500 ? 4 : BF && NTL == 4 && D == 128 ? 2 : 3;
   static constexpr bool QREG = NTL * KS <= 16;       // Q's fragments in registers, else in shared memory
   static constexpr int RING = STAGES * STEP;
   static constexpr int JOIN = 32 * (4 * NTL * MB + 4 * NTL) * 4;  // a warp's output, maxima and sums
   static constexpr int QBYTES = QREG ? 0 : RW * NTL * KS * 256;
   static constexpr int WORK = KW * RW * RING > 2 * RW * JOIN ? KW * RW * RING : 2 * RW * JOIN;
-  static constexpr int SMEM = WORK + QBYTES;
+  static constexpr int RAW = BF ? 0 : RT * D * 2;    // 8-bit kinds: Q in bf16 for the tree's own keys
+  static constexpr int SMEM = WORK + QBYTES + RAW;
+  // Where the 16 bytes number u of a block of 16 keys' K (V) go: as they lie in memory, but XORed inside their 128 bytes
+  // so that the lanes' loads below do not meet on a bank. (Copies that spread a line of 128 bytes over several reached
+  // 5.0 TB/s, copies that keep it whole 6.5, permuted inside or not.)
+  __device__ static __forceinline__ int k_place(int u) {
+    constexpr int ROW = D * (BF ? 2 : 1) / 16;
+    return ROW < 8 ? u : u ^ (u / ROW & 1) * 4;
+  }
+  __device__ static __forceinline__ int v_place(int u) {
+    constexpr int QUAD = D * (BF ? 2 : 1) / 4;
+    return NL * 32 + (u ^ u / QUAD * 2);
+  }
+  // what lane 4g + t reads: 64 bytes c of key g (j = 0) or g + 8 (1); 128 bytes c of quad t
+  __device__ static __forceinline__ int k_read(int j, int c, int g, int t) {
+    return k_place((4 * (g >> 1) + (g & 1) + 2 * j) * (D * (BF ? 2 : 1) / 16) + c * 4 + t);
+  }
+  __device__ static __forceinline__ int v_read(int c, int g, int t) {
+    return v_place(t * (D * (BF ? 2 : 1) / 4) + c * 8 + g);
+  }
   // the dimension that word (ks) of lane t starts at in K Q^T: 16 consecutive bytes of a key's row a lane
   __device__ static __forceinline__ int dim_of(int ks, int t) {
     return BF ? (ks >> 1) * 32 + t * 8 + (ks & 1) * 4 : (ks >> 2) * 64 + t * 16 + (ks & 3) * 4;
@@ -199,14 +225,16 @@ struct Part {
   int vref;                     // acc holds the output in units of 2^(vref - 127) (8-bit kinds)
 
   // The maximum and the output's unit moved; every lane of the warp calls it.
-  __device__ __forceinline__ void move(const float (&s)[NTL][4], int new_ref) {
+  __device__ __forceinline__ void move(const float (&s)[S::G][NTL][4], int new_ref) {
     const float unit = ex2(static_cast<float>(vref - new_ref));
     vref = new_ref;
 #pragma unroll
     for (int nt = 0; nt < NTL; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float x = fmaxf(s[nt][e], s[nt][2 + e]);
+        float x = NEG;
+#pragma unroll
+        for (int j = 0; j < S::G; ++j) x = fmaxf(x, fmaxf(s[j][nt][e], s[j][nt][2 + e]));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16)) * rf[nt][e];
@@ -226,12 +254,14 @@ struct Part {
   }
 
   // Scores s (masked: -inf) to probabilities, their sums, and the running maximum; ref: the largest V scale there is.
-  __device__ __forceinline__ void soften(float (&s)[NTL][4], int ref) {
+  __device__ __forceinline__ void soften(float (&s)[S::G][NTL][4], int ref) {
     bool up = ref > vref;
 #pragma unroll
-    for (int nt = 0; nt < NTL; ++nt)
+    for (int j = 0; j < S::G; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) up |= fmaf(s[nt][e], rf[nt][e & 1], off[nt][e & 1]) > SLACK;
+      for (int nt = 0; nt < NTL; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) up |= fmaf(s[j][nt][e], rf[nt][e & 1], off[nt][e & 1]) > SLACK;
     if (__any_sync(0xffffffffu, up)) {
       ref = max(ref, __shfl_xor_sync(0xffffffffu, ref, 4));
       ref = max(ref, __shfl_xor_sync(0xffffffffu, ref, 8));
@@ -239,12 +269,14 @@ struct Part {
       move(s, max(ref, vref));
     }
 #pragma unroll
-    for (int nt = 0; nt < NTL; ++nt)
+    for (int j = 0; j < S::G; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[nt][e] = ex2(fmaf(s[nt][e], rf[nt][e & 1], off[nt][e & 1]));
-        l[nt][e & 1] += s[nt][e];
-      }
+      for (int nt = 0; nt < NTL; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[j][nt][e] = ex2(fmaf(s[j][nt][e], rf[nt][e & 1], off[nt][e & 1]));
+          l[nt][e & 1] += s[j][nt][e];
+        }
   }
 };
 
@@ -316,78 +348,121 @@ __global__ void __launch_bounds__(Shape<KIND, D, NTL, RW>::NT)
     attend_kernel(const Params p) {
   using S = Shape<KIND, D, NTL, RW>;
   constexpr bool BF = S::BF;
-  constexpr int NL = S::NL, KS = S::KS, MB = S::MB;
+  constexpr int NL = S::NL, KS = S::KS, MB = S::MB, G = S::G;
   extern __shared__ __align__(16) uint8_t smem[];
   uint2* const qs = reinterpret_cast<uint2*>(smem + S::WORK);
   int* const before = reinterpret_cast<int*>(smem + S::SMEM);
+  int* const lens = before + p.seqs + 1;
+  // the nodes' masks, depths, keys and values: [nodes][D + 8] bf16 each (the 8 keep neighbouring rows off each other's
+  // banks). What an item needs besides the cache is copied here first: behind the cache's copies it would wait for them
+  constexpr int PITCH = D + 8;
+  uint64_t* const masks = reinterpret_cast<uint64_t*>(smem + S::SMEM + ((2 * p.seqs + 4) & ~3) * 4);
+  int* const depths = reinterpret_cast<int*>(masks + (p.nodes + 1) / 2 * 2);  // both regions whole 16 bytes
+  __nv_bfloat16* const tree_k = reinterpret_cast<__nv_bfloat16*>(depths + (p.nodes + 3) / 4 * 4);
+  __nv_bfloat16* const tree_v = tree_k + p.nodes * PITCH;
+  uint2* const raw = reinterpret_cast<uint2*>(smem + S::WORK + S::QBYTES);
   cudaTriggerProgrammaticLaunchCompletion();
-  line_of(p, before);
+  line_of(p, before, lens);
   const Spans spans(p, before);
   if (static_cast<int>(blockIdx.x) >= spans.ctas) return;
-  const int64_t first = spans.cut(blockIdx.x), last = spans.cut(blockIdx.x + 1);
+  const int first = spans.cut(blockIdx.x), last = spans.cut(blockIdx.x + 1);
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int warp = threadIdx.x >> 5, kw = warp % KW, rw = warp / KW;
   const int rows = p.nodes * p.group, hr = p.heads * p.tiles;
   uint8_t* const ring = smem + warp * S::RING;
-  const uint32_t ring_at = smem_u32(ring) + lane * 16;
   int b;
   {
     int low = 0, high = p.seqs - 1;  // the last sequence that begins at or before the span
     while (low < high) {
       const int mid = (low + high + 1) >> 1;
-      if (static_cast<int64_t>(before[mid]) * hr <= first) low = mid;
+      if (before[mid] * hr <= first) low = mid;
       else high = mid - 1;
     }
     b = low;
   }
-  for (int64_t at = first; at < last;) {
-    const int64_t base = static_cast<int64_t>(before[b]) * hr;
-    const int per = before[b + 1] - before[b];
-    const int item = static_cast<int>((at - base) / per);
-    const int u0 = static_cast<int>(at - base - static_cast<int64_t>(item) * per);
-    const int u1 = last - at < per - u0 ? u0 + static_cast<int>(last - at) : per;
+  for (int at = first; at < last;) {
+    const int base = before[b] * hr, per = before[b + 1] - before[b];
+    const int item = (at - base) / per, u0 = at - base - item * per, u1 = min(per, u0 + last - at);
     const int h = item / p.tiles, tile = item - h * p.tiles;
     const int row0 = tile * S::RT + rw * 8 * NTL;
-    const int len = length_of(p, b);
-    const int unit0 = first_unit(p, len) - 1;  // unit u holds the keys from (unit0 + u) * 64 on
+    const int len = lens[b];
+    const int unit0 = first_unit(p, len) - 1;  // unit u holds the keys from (unit0 + u) << unit_shift on
 
-    // ---- the cached keys' first copies: issued before Q is read
+    // ---- first on their way: Q and the tree's own keys and values
+    const __nv_bfloat16* qb = p.q + b * p.q_seq;
+    const auto depth_of = [&](int nt, int e) {  // of the node of row 2t + e
+      const int r = row0 + nt * 8 + 2 * t + e;
+      return depths[r < rows ? r / p.group : 0];
+    };
+    const auto q_row = [&](int nt, bool& real) {
+      const int r = row0 + nt * 8 + g;
+      real = r < rows;
+      const int node = real ? r / p.group : 0;
+      return qb + node * p.q_node + (h * p.group + (real ? r - node * p.group : 0)) * p.q_head;
+    };
+    uint2 qx[NTL][KS];
+#pragma unroll
+    for (int nt = 0; nt < NTL; ++nt) {
+      bool real;
+      const __nv_bfloat16* q = q_row(nt, real);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        qx[nt][ks] = real ? __ldg(reinterpret_cast<const uint2*>(q + S::dim_of(ks, t))) : make_uint2(0, 0);
+    }
+    for (int i = threadIdx.x; i < p.nodes; i += S::NT) {
+      copy4(smem_u32(depths + i), p.depth + b * p.nodes + i);
+      if (u0 == 0) copy8(smem_u32(masks + i), p.mask + b * p.nodes + i);
+    }
+    if (u0 == 0) {
+      const __nv_bfloat16* kb = p.k + b * p.k_seq + h * p.k_head;
+      const __nv_bfloat16* vb = p.v + b * p.v_seq + h * p.v_head;
+      for (int i = threadIdx.x; i < p.nodes * (D / 8); i += S::NT) {
+        const int node = i / (D / 8), d = i % (D / 8) * 8;
+        copy16(smem_u32(tree_k + node * PITCH + d), kb + node * p.k_node + d);
+        copy16(smem_u32(tree_v + node * PITCH + d), vb + node * p.v_node + d);
+      }
+    }
+    cp_async_commit();
+
+    // ---- then the cached keys' first copies
     const int* table = p.table + static_cast<int64_t>(b) * p.width;
     const int cshift = p.page_shift - 4;
-    int chunk = (unit0 + (u0 > 1 ? u0 : 1)) * KW + kw;  // of 16 keys
-    const int chunk_end = min((unit0 + u1) * KW, (len + 15) >> 4);
+    int chunk = (unit0 + (u0 > 1 ? u0 : 1)) * KW + kw;  // of 16 G keys
+    const int chunk_end = min((unit0 + u1) * KW, (len + 16 * G - 1) / (16 * G));
     int ahead = chunk, page0 = -64, pages = 0;
     bool lost = false;
-    const uint8_t* const k_lane = static_cast<const uint8_t*>(p.c.k) + key_of(g) * D * (BF ? 2 : 1) + t * 16;
-    const uint8_t* const v_lane = static_cast<const uint8_t*>(p.c.v) + t * D * (BF ? 8 : 4) + g * 16;
+    const uint8_t* const k_lane = static_cast<const uint8_t*>(p.c.k) + lane * 16;
+    const uint8_t* const v_lane = static_cast<const uint8_t*>(p.c.v) + lane * 16;
     const auto fetch = [&](int stage) {
       if (ahead < chunk_end) {
-        const int pi = ahead >> cshift;
-        if (pi >= page0 + 32) {  // the next 32 entries of the table, one a lane
-          page0 = pi;
-          pages = page0 + lane < p.width ? table[page0 + lane] : 0;
-        }
-        int page = __shfl_sync(0xffffffffu, pages, pi - page0);
-        if (page < 0 || page >= p.c.pages) {
-          lost = true;
-          page = 0;
-        }
-        const int64_t cell =
-            (((p.layer_cell + page) * p.heads + h) << p.page_shift) + ((ahead & ((1 << cshift) - 1)) << 4);
-        const uint32_t to = ring_at + stage * S::STEP;
-        const uint8_t* k = k_lane + cell * (D * (BF ? 2 : 1));
-        const uint8_t* v = v_lane + cell * (D * (BF ? 2 : 1));
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < G; ++j) {
+          const int block = ahead * G + j;  // of 16 keys: in one page
+          if (j > 0 && block << 4 >= len) break;  // (stays as it is: masked)
+          const int pi = block >> cshift;
+          if (pi >= page0 + 32) {  // the next 32 entries of the table, one a lane
+            page0 = pi;
+            pages = page0 + lane < p.width ? table[page0 + lane] : 0;
+          }
+          int page = __shfl_sync(0xffffffffu, pages, pi - page0);
+          if (page < 0 || page >= p.c.pages) {
+            lost = true;
+            page = 0;
+          }
+          const int64_t cell =
+              (((p.layer_cell + page) * p.heads + h) << p.page_shift) + ((block & ((1 << cshift) - 1)) << 4);
+          const uint32_t to = smem_u32(ring) + stage * S::STEP + j * S::BLOCK;
+          const uint8_t* k = k_lane + cell * (D * (BF ? 2 : 1));
+          const uint8_t* v = v_lane + cell * (D * (BF ? 2 : 1));
 #pragma unroll
-          for (int c = 0; c < NL / 2; ++c)
-            copy16(to + (j * (NL / 2) + c) * 512, k + j * 2 * D * (BF ? 2 : 1) + c * 64);
+          for (int c = 0; c < NL; ++c) copy16(to + S::k_place(c * 32 + lane) * 16, k + c * 512);
 #pragma unroll
-        for (int c = 0; c < NL; ++c) copy16(to + (NL + c) * 512, v + c * 128);
-        if constexpr (!BF) {
-          const uint32_t s4 = smem_u32(ring) + stage * S::STEP + 2 * NL * 512 + lane * 4;
-          copy4(s4, p.c.k_scale + cell + (g & 6) * 2);
-          copy4(s4 + 128, p.c.v_scale + cell + (g & 6) * 2);
+          for (int c = 0; c < NL; ++c) copy16(to + S::v_place(c * 32 + lane) * 16, v + c * 512);
+          if constexpr (!BF) {
+            const uint32_t s4 = to + lane * 4 + 2 * NL * 512;
+            copy4(s4, p.c.k_scale + cell + (g & 6) * 2);
+            copy4(s4 + 128, p.c.v_scale + cell + (g & 6) * 2);
+          }
         }
       }
       cp_async_commit();
@@ -398,25 +473,9 @@ __global__ void __launch_bounds__(Shape<KIND, D, NTL, RW>::NT)
     // ---- Q's fragments: row g of each tile
     Part<KIND, D, NTL, RW> part;
     uint32_t qr[S::QREG ? NTL : 1][S::QREG ? KS : 1][2];
-    const __nv_bfloat16* qb = p.q + b * p.q_seq;
-    const auto depth_of = [&](int nt, int e) {  // of the node of row 2t + e
-      const int r = row0 + nt * 8 + 2 * t + e;
-      return p.depth[b * p.nodes + (r < rows ? r / p.group : 0)];
-    };
-    const auto q_row = [&](int nt, bool& real) {
-      const int r = row0 + nt * 8 + g;
-      real = r < rows;
-      const int node = real ? r / p.group : 0;
-      return qb + node * p.q_node + (h * p.group + (real ? r - node * p.group : 0)) * p.q_head;
-    };
 #pragma unroll
     for (int nt = 0; nt < NTL; ++nt) {
-      bool real;
-      const __nv_bfloat16* q = q_row(nt, real);
-      uint2 x[KS];
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-        x[ks] = real ? *reinterpret_cast<const uint2*>(q + S::dim_of(ks, t)) : make_uint2(0, 0);
+      uint2(&x)[KS] = qx[nt];
       float scale = 1.f;
       if constexpr (!BF) {  // fp16 under a power of two: the row's largest is brought to [1, 2)
         uint32_t top = 0;
@@ -431,6 +490,10 @@ __global__ void __launch_bounds__(Shape<KIND, D, NTL, RW>::NT)
         e = e == 255 || e < 1 ? 127 : e < 67 ? 67 : e > 253 ? 253 : e;  // (not finite or zero: as it is)
         const float f = kv::power(254 - e);
         scale = kv::power(e);
+        if (u0 == 0 && kw == 0) {
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) raw[((rw * NTL + nt) * KS + ks) * 32 + lane] = x[ks];
+        }
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
           x[ks].x = pack_f16(low_f(x[ks].x) * f, high_f(x[ks].x) * f);
@@ -449,7 +512,6 @@ __global__ void __launch_bounds__(Shape<KIND, D, NTL, RW>::NT)
         else if (kw == 0) qs[((rw * NTL + nt) * KS + ks) * 32 + lane] = x[ks];
       }
     }
-    if constexpr (!S::QREG) __syncthreads();
 #pragma unroll
     for (int nt = 0; nt < NTL; ++nt)
 #pragma unroll
@@ -459,14 +521,18 @@ __global__ void __launch_bounds__(Shape<KIND, D, NTL, RW>::NT)
     part.vref = BF ? 127 : VREF;
 
     // ---- the tree's own keys: 16 nodes a warp, unquantised, in bf16
+    cp_async_wait<S::STAGES - 1>();
+    __syncthreads();  // depths, the tree's rows and masks, Q in shared memory
     if (u0 == 0 && kw * 16 < p.nodes) {
-      float s[NTL][4];
+      float both[G][NTL][4];  // the second group of 16: none
+      float(&s)[NTL][4] = both[0];
 #pragma unroll
       for (int nt = 0; nt < NTL; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
-      const __nv_bfloat16* kb = p.k + b * p.k_seq + h * p.k_head;
-      const __nv_bfloat16* vb = p.v + b * p.v_seq + h * p.v_head;
+        for (int e = 0; e < 4; ++e) {
+          s[nt][e] = 0.f;
+          if constexpr (G == 2) both[1][nt][e] = NEG;
+        }
       int node2[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) node2[j] = kw * 16 + key_of(g) + 2 * j;
@@ -475,27 +541,29 @@ __global__ void __launch_bounds__(Shape<KIND, D, NTL, RW>::NT)
         uint2 kk[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j)
-          kk[j] = node2[j] < p.nodes ? *reinterpret_cast<const uint2*>(kb + node2[j] * p.k_node + S::dim_of(ks, t))
-                                     : make_uint2(0, 0);
+          kk[j] = node2[j] < p.nodes
+                      ? *reinterpret_cast<const uint2*>(tree_k + node2[j] * PITCH + S::dim_of(ks, t))
+                      : make_uint2(0, 0);
         const uint32_t a[4] = {kk[0].x, kk[1].x, kk[0].y, kk[1].y};
 #pragma unroll
         for (int nt = 0; nt < NTL; ++nt) {
-          bool real;
-          const __nv_bfloat16* q = q_row(nt, real);
-          const uint2 x = real ? *reinterpret_cast<const uint2*>(q + S::dim_of(ks, t)) : make_uint2(0, 0);
+          uint2 x;
+          if constexpr (!BF) x = raw[((rw * NTL + nt) * KS + ks) * 32 + lane];
+          else if constexpr (S::QREG) x = make_uint2(qr[nt][ks][0], qr[nt][ks][1]);
+          else x = qs[((rw * NTL + nt) * KS + ks) * 32 + lane];
           mma<true>(s[nt], a, x.x, x.y);
         }
       }
       int dk[2];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) dk[j] = node2[j] < p.nodes ? p.depth[b * p.nodes + node2[j]] : 0;
+      for (int j = 0; j < 2; ++j) dk[j] = node2[j] < p.nodes ? depths[node2[j]] : 0;
 #pragma unroll
       for (int nt = 0; nt < NTL; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int r = row0 + nt * 8 + 2 * t + e;
           const int node = r < rows ? r / p.group : 0;
-          const uint64_t mask = r < rows ? p.mask[b * p.nodes + node] : 0;
+          const uint64_t mask = r < rows ? masks[node] : 0;
           const int reach = p.window < 0 ? 0 : depth_of(nt, e) - p.window;
           const float f = p.scale_log2 / part.rf[nt][e];  // scores in the units of the cached keys' (a power of two)
 #pragma unroll
@@ -506,7 +574,7 @@ __global__ void __launch_bounds__(Shape<KIND, D, NTL, RW>::NT)
         }
       uint32_t vis[NTL][2], pf[NTL][2];
       visible<NTL>(s, vis);
-      part.soften(s, part.vref);
+      part.soften(both, part.vref);
       constexpr float UNITS = BF ? 1.f : 1048576.f;  // 1 in units of 2^(VREF - 127)
 #pragma unroll
       for (int nt = 0; nt < NTL; ++nt) p_fragment<true>(s[nt], UNITS, UNITS, pf[nt]);
@@ -517,9 +585,9 @@ __global__ void __launch_bounds__(Shape<KIND, D, NTL, RW>::NT)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int node = kw * 16 + 4 * t + i;
-          const unsigned short* from = reinterpret_cast<const unsigned short*>(vb + node * p.v_node + d);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) w[j][i] = node < p.nodes ? __ldg(from + j) : 0u;
+          const uint32_t two =
+              node < p.nodes ? *reinterpret_cast<const uint32_t*>(tree_v + node * PITCH + d) : 0u;
+          w[0][i] = two & 0xffffu, w[1][i] = two >> 16;
         }
         const uint32_t v4[4] = {w[0][0] | w[0][1] << 16, w[1][0] | w[1][1] << 16, w[0][2] | w[0][3] << 16,
                                 w[1][2] | w[1][3] << 16};
@@ -531,117 +599,148 @@ __global__ void __launch_bounds__(Shape<KIND, D, NTL, RW>::NT)
     int stage = 0;
     for (; chunk < chunk_end; chunk += KW) {
       cp_async_wait<S::STAGES - 2>();
-      fetch(stage == 0 ? S::STAGES - 1 : stage - 1);  // the step read last is free
+      __syncwarp();  // every lane's copies of this step are there, and the step read last is read
+      fetch(stage == 0 ? S::STAGES - 1 : stage - 1);
       const uint8_t* step = ring + stage * S::STEP;
-      const uint4* own = reinterpret_cast<const uint4*>(step) + lane;
-      float s[NTL][4];
-#pragma unroll
-      for (int nt = 0; nt < NTL; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
-#pragma unroll
-      for (int c = 0; c < NL / 2; ++c) {
-        constexpr int PER = BF ? 2 : 4;  // steps in 16 bytes
-        uint32_t w[2][4];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint4 u = own[(j * (NL / 2) + c) * 32];
-          w[j][0] = u.x, w[j][1] = u.y, w[j][2] = u.z, w[j][3] = u.w;
-        }
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          const int ks = c * PER + i;
-          uint32_t a[4];
-          if constexpr (BF) {
-            a[0] = w[0][2 * i], a[1] = w[1][2 * i], a[2] = w[0][2 * i + 1], a[3] = w[1][2 * i + 1];
-          } else {
-            kv::decode4<KIND>(w[0][i], a[0], a[2]);
-            kv::decode4<KIND>(w[1][i], a[1], a[3]);
-          }
-#pragma unroll
-          for (int nt = 0; nt < NTL; ++nt) {
-            if constexpr (S::QREG) {
-              mma<BF>(s[nt], a, qr[nt][ks][0], qr[nt][ks][1]);
-            } else {
-              const uint2 x = qs[((rw * NTL + nt) * KS + ks) * 32 + lane];
-              mma<BF>(s[nt], a, x.x, x.y);
-            }
-          }
-        }
-      }
-      const int key0 = chunk << 4;
+      const int key0 = chunk * 16 * G;
       // some key is past the end, or before the window of the deepest node there could be
-      const bool edge = key0 + 16 > len || (p.window >= 0 && key0 < len + p.nodes - p.window);
-      uint32_t vb0 = 0, vb1 = 0;  // V's scale bytes of keys g and g + 8
-      if constexpr (!BF) {
-        const uint32_t* sc = reinterpret_cast<const uint32_t*>(step + 2 * NL * 512) + lane;
-        const uint32_t kb = sc[0] >> (8 * (g & 1)), vb = sc[32] >> (8 * (g & 1));
-        vb0 = vb & 0xffu, vb1 = vb >> 16 & 0xffu;
-        // byte 255 gives infinity, times the row's zero codes NaN
-        const float f0 = __uint_as_float((kb & 0xffu) << 23), f1 = __uint_as_float((kb & 0xff0000u) << 7);
+      const bool edge = key0 + 16 * G > len || (p.window >= 0 && key0 < len + p.nodes - p.window);
+      float s[G][NTL][4];
+      uint32_t vb[G][2];  // V's scale bytes of keys g and g + 8
+      uint32_t keep[G];   // a byte for each of quad t's keys that exist
 #pragma unroll
-        for (int nt = 0; nt < NTL; ++nt) s[nt][0] *= f0, s[nt][1] *= f0, s[nt][2] *= f1, s[nt][3] *= f1;
-      }
-      uint32_t keep = 0xffffffffu;  // a byte for each of quad t's keys that exist
-      if (edge) {
-        const int left4 = len - key0 - 4 * t, k0 = key0 + key_of(g);
-        keep = left4 >= 4 ? 0xffffffffu : left4 <= 0 ? 0u : 0xffffffffu >> (32 - 8 * left4);
-        if (k0 >= len) vb0 = 0;
-        if (k0 + 2 >= len) vb1 = 0;
+      for (int j = 0; j < G; ++j) {
+        const uint4* own = reinterpret_cast<const uint4*>(step + j * S::BLOCK);
+        float chain[S::CHAINS][NTL][4];
 #pragma unroll
-        for (int nt = 0; nt < NTL; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int low = p.window < 0 ? 0 : len + depth_of(nt, e) - p.window;
-            if (k0 >= len || k0 < low) s[nt][e] = NEG;
-            if (k0 + 2 >= len || k0 + 2 < low) s[nt][2 + e] = NEG;
-          }
-      }
-      uint32_t vis[BF ? NTL : 1][2];
-      float f0 = 1.f, f1 = 1.f;
-      if constexpr (BF) {
-        if (edge) visible<NTL>(s, vis);
-        part.soften(s, part.vref);
-      } else {
-        if (__any_sync(0xffffffffu, vb0 == 255 || vb1 == 255)) {
-          // rows of V that read as NaN: taken out of the product (codes 0, factor 0) and put into the sums
+        for (int x = 0; x < S::CHAINS; ++x)
 #pragma unroll
           for (int nt = 0; nt < NTL; ++nt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if ((e & 2 ? vb1 : vb0) == 255 && s[nt][e] != NEG) part.l[nt][e & 1] = __int_as_float(0x7fc00000);
-          if (vb0 == 255) vb0 = 0;
-          if (vb1 == 255) vb1 = 0;
-        }
-        part.soften(s, static_cast<int>(max(vb0, vb1)));
-        f0 = kv::power(max(static_cast<int>(vb0) - part.vref + 127, 0));
-        f1 = kv::power(max(static_cast<int>(vb1) - part.vref + 127, 0));
-      }
-      uint32_t pf[NTL][2];
+            for (int e = 0; e < 4; ++e) chain[x][nt][e] = 0.f;
 #pragma unroll
-      for (int nt = 0; nt < NTL; ++nt) p_fragment<BF>(s[nt], f0, f1, pf[nt]);
-#pragma unroll
-      for (int c = 0; c < NL; ++c) {
-        const uint4 u = own[(NL + c) * 32];
-        uint32_t w[4] = {u.x, u.y, u.z, u.w};
-        if constexpr (BF) {  // dimensions 2g, 2g + 1 of 16: words keys 01, 23 of the one, then of the other
-          const uint32_t a[4] = {w[0], w[2], w[1], w[3]};
-          if (edge) {
-            const uint32_t lo = __byte_perm(keep, 0, 0x1100), hi = __byte_perm(keep, 0, 0x3322);
-            const uint32_t a2[4] = {a[0] & lo, a[1] & lo, a[2] & hi, a[3] & hi};
-            pv_special<NTL, MB>(part.acc, c, a2, pf, vis);
-          } else {
-#pragma unroll
-            for (int nt = 0; nt < NTL; ++nt) mma<true>(part.acc[nt][c], a, pf[nt][0], pf[nt][1]);
-          }
-        } else {  // dimensions 4g .. 4g + 3 of 32
+        for (int c = 0; c < NL / 2; ++c) {
+          constexpr int PER = BF ? 2 : 4;  // steps in 16 bytes
+          uint32_t w[2][4];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            uint32_t a[4];
-            kv::decode4<KIND>(w[2 * i] & keep, a[0], a[2]);
-            kv::decode4<KIND>(w[2 * i + 1] & keep, a[1], a[3]);
+            const uint4 u = own[S::k_read(i, c, g, t)];
+            w[i][0] = u.x, w[i][1] = u.y, w[i][2] = u.z, w[i][3] = u.w;
+          }
 #pragma unroll
-            for (int nt = 0; nt < NTL; ++nt) mma<false>(part.acc[nt][2 * c + i], a, pf[nt][0], pf[nt][1]);
+          for (int i = 0; i < PER; ++i) {
+            const int ks = c * PER + i;
+            uint32_t a[4];
+            if constexpr (BF) {
+              a[0] = w[0][2 * i], a[1] = w[1][2 * i], a[2] = w[0][2 * i + 1], a[3] = w[1][2 * i + 1];
+            } else {
+              kv::decode4<KIND>(w[0][i], a[0], a[2]);
+              kv::decode4<KIND>(w[1][i], a[1], a[3]);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NTL; ++nt) {
+              if constexpr (S::QREG) {
+                mma<BF>(chain[ks % S::CHAINS][nt], a, qr[nt][ks][0], qr[nt][ks][1]);
+              } else {
+                const uint2 x = qs[((rw * NTL + nt) * KS + ks) * 32 + lane];
+                mma<BF>(chain[ks % S::CHAINS][nt], a, x.x, x.y);
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NTL; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            s[j][nt][e] = S::CHAINS == 2 ? chain[0][nt][e] + chain[S::CHAINS - 1][nt][e] : chain[0][nt][e];
+        vb[j][0] = vb[j][1] = 0;
+        if constexpr (!BF) {
+          const uint32_t* sc = reinterpret_cast<const uint32_t*>(step + j * S::BLOCK + 2 * NL * 512) + lane;
+          const uint32_t kb = sc[0] >> (8 * (g & 1)), v2 = sc[32] >> (8 * (g & 1));
+          vb[j][0] = v2 & 0xffu, vb[j][1] = v2 >> 16 & 0xffu;
+          // byte 255 gives infinity, times the row's zero codes NaN
+          const float f0 = __uint_as_float((kb & 0xffu) << 23), f1 = __uint_as_float((kb & 0xff0000u) << 7);
+#pragma unroll
+          for (int nt = 0; nt < NTL; ++nt) s[j][nt][0] *= f0, s[j][nt][1] *= f0, s[j][nt][2] *= f1, s[j][nt][3] *= f1;
+        }
+        keep[j] = 0xffffffffu;
+        if (edge) {
+          const int k16 = key0 + 16 * j, left4 = len - k16 - 4 * t, k0 = k16 + key_of(g);
+          keep[j] = left4 >= 4 ? 0xffffffffu : left4 <= 0 ? 0u : 0xffffffffu >> (32 - 8 * left4);
+          if (k0 >= len) vb[j][0] = 0;
+          if (k0 + 2 >= len) vb[j][1] = 0;
+#pragma unroll
+          for (int nt = 0; nt < NTL; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int low = p.window < 0 ? 0 : len + depth_of(nt, e) - p.window;
+              if (k0 >= len || k0 < low) s[j][nt][e] = NEG;
+              if (k0 + 2 >= len || k0 + 2 < low) s[j][nt][2 + e] = NEG;
+            }
+        }
+      }
+      uint32_t vis[BF ? NTL : 1][2];
+      if constexpr (BF) {
+        if (edge) visible<NTL>(s[0], vis);
+        part.soften(s, part.vref);
+      } else {
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < G; ++j) top = max(top, max(vb[j][0], vb[j][1]));
+        if (__any_sync(0xffffffffu, top == 255)) {
+          // rows of V that read as NaN: taken out of the product (codes 0, factor 0) and put into the sums
+          top = 0;
+#pragma unroll
+          for (int j = 0; j < G; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              if (vb[j][i] == 255) {
+                vb[j][i] = 0;
+#pragma unroll
+                for (int nt = 0; nt < NTL; ++nt)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e)
+                    if (s[j][nt][2 * i + e] != NEG) part.l[nt][e] = __int_as_float(0x7fc00000);
+              }
+              top = max(top, vb[j][i]);
+            }
+        }
+        part.soften(s, static_cast<int>(top));
+      }
+#pragma unroll
+      for (int j = 0; j < G; ++j) {
+        const uint4* own = reinterpret_cast<const uint4*>(step + j * S::BLOCK);
+        float f0 = 1.f, f1 = 1.f;
+        if constexpr (!BF) {
+          f0 = kv::power(max(static_cast<int>(vb[j][0]) - part.vref + 127, 0));
+          f1 = kv::power(max(static_cast<int>(vb[j][1]) - part.vref + 127, 0));
+        }
+        uint32_t pf[NTL][2];
+#pragma unroll
+        for (int nt = 0; nt < NTL; ++nt) p_fragment<BF>(s[j][nt], f0, f1, pf[nt]);
+#pragma unroll
+        for (int c = 0; c < NL; ++c) {
+          const uint4 u = own[S::v_read(c, g, t)];
+          uint32_t w[4] = {u.x, u.y, u.z, u.w};
+          if constexpr (BF) {  // dimensions 2g, 2g + 1 of 16: words keys 01, 23 of the one, then of the other
+            const uint32_t a[4] = {w[0], w[2], w[1], w[3]};
+            if (edge) {
+              const uint32_t lo = __byte_perm(keep[j], 0, 0x1100), hi = __byte_perm(keep[j], 0, 0x3322);
+              const uint32_t a2[4] = {a[0] & lo, a[1] & lo, a[2] & hi, a[3] & hi};
+              pv_special<NTL, MB>(part.acc, c, a2, pf, vis);
+            } else {
+#pragma unroll
+              for (int nt = 0; nt < NTL; ++nt) mma<true>(part.acc[nt][c], a, pf[nt][0], pf[nt][1]);
+            }
+          } else {  // dimensions 4g .. 4g + 3 of 32
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              uint32_t a[4];
+              kv::decode4<KIND>(w[2 * i] & keep[j], a[0], a[2]);
+              kv::decode4<KIND>(w[2 * i + 1] & keep[j], a[1], a[3]);
+#pragma unroll
+              for (int nt = 0; nt < NTL; ++nt) mma<false>(part.acc[nt][2 * c + i], a, pf[nt][0], pf[nt][1]);
+            }
           }
         }
       }
@@ -724,7 +823,7 @@ __global__ void __launch_bounds__(Shape<KIND, D, NTL, RW>::NT)
           const int in = rw * 8 * NTL + nt * 8 + 2 * t + e, r = tile * S::RT + in;
           if (r >= rows) continue;
           const int node = r / p.group;
-          const bool pad = p.depth[b * p.nodes + node] < 0;
+          const bool pad = depths[node] < 0;
           const float l = part.l[nt][e];
           const float f = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
           __nv_bfloat16* out =
@@ -762,12 +861,12 @@ __global__ void __launch_bounds__(Shape<KIND, D, NTL, RW>::NT)
 // Joins the parts of one item (a block each): o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i (off = -m), in the parts' order.
 __global__ void __launch_bounds__(256) join_kernel(const Params p, int rt, int dim) {
   extern __shared__ int before[];
-  line_of(p, before);
+  line_of(p, before, before + p.seqs + 1);
   const Spans spans(p, before);
   const int hr = p.heads * p.tiles;
   const int b = blockIdx.x / hr, item = blockIdx.x - b * hr;
   const int per = before[b + 1] - before[b];
-  const int64_t u = static_cast<int64_t>(before[b]) * hr + static_cast<int64_t>(item) * per;
+  const int u = before[b] * hr + item * per;
   const int c0 = spans.owner(u), c1 = spans.owner(u + per - 1);
   cudaGridDependencySynchronize();
   if (c0 == c1) return;  // it was written whole
@@ -779,19 +878,29 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p, int rt, int d
     const int in = i / quads, d = (i - in * quads) * 4, r = tile * rt + in;
     if (r >= rows) return;
     const int node = r / p.group;
-    float off = NONE;
-    for (int c = c0; c <= c1; ++c)
-      off = fminf(off, sums[static_cast<int64_t>(c == c0 ? slot0 : 2 * c) * 2 * rt + in]);
-    float l = 0.f;
+    float off = NONE, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int c = c0; c <= c1; ++c) {
-      const int64_t slot = c == c0 ? slot0 : 2 * c;
-      const float oo = sums[slot * 2 * rt + in], sl = sums[slot * 2 * rt + rt + in];
-      const float4 x = *reinterpret_cast<const float4*>(p.partial + (slot * rt + in) * dim + d);
-      const float f = oo == NONE ? 0.f : ex2(off - oo);
-      l += oo == NONE ? sl : sl * f;
-      o.x += x.x * f, o.y += x.y * f, o.z += x.z * f, o.w += x.w * f;
+    for (int c = c0; c <= c1; c += 4) {  // four parts' loads at once
+      float oo[4], sl[4];
+      float4 x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        oo[j] = NONE, sl[j] = 0.f, x[j] = o;
+        if (c + j > c1) continue;
+        const int64_t slot = c + j == c0 ? slot0 : 2 * (c + j);
+        oo[j] = sums[slot * 2 * rt + in], sl[j] = sums[slot * 2 * rt + rt + in];
+        x[j] = *reinterpret_cast<const float4*>(p.partial + (slot * rt + in) * dim + d);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float low = fminf(off, oo[j]);
+        const float f = off == NONE ? 0.f : ex2(low - off), g = oo[j] == NONE ? 0.f : ex2(low - oo[j]);
+        // a part that saw no key may still hold the NaN of a lost page
+        l = (off == NONE ? l : l * f) + (oo[j] == NONE ? sl[j] : sl[j] * g);
+        o.x = o.x * f + x[j].x * g, o.y = o.y * f + x[j].y * g;
+        o.z = o.z * f + x[j].z * g, o.w = o.w * f + x[j].w * g;
+        off = low;
+      }
     }
     const bool none = l == 0.f || p.depth[b * p.nodes + node] < 0;
     const float f = none ? 0.f : 1.f / l;
@@ -820,9 +929,9 @@ template <int KIND, int D, int NTL, int RW>
 int run(Params& p, size_t workspace_bytes, cudaStream_t s) {
   using S = Shape<KIND, D, NTL, RW>;
   const auto kernel = attend_kernel<KIND, D, NTL, RW>;
-  const int smem = S::SMEM + (p.seqs + 1) * 4;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM + (MAX_SEQS + 1) * 4) !=
-      cudaSuccess)
+  const int smem = S::SMEM + ((2 * p.seqs + 4) & ~3) * 4 + (p.nodes + 1) / 2 * 16 + (p.nodes + 3) / 4 * 16 +
+                   p.nodes * (D + 8) * 4;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return NOISE_ERR_CUDA;
   int per_sm = 0;
   if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, S::NT, smem) != cudaSuccess || per_sm < 1)
@@ -832,7 +941,10 @@ int run(Params& p, size_t workspace_bytes, cudaStream_t s) {
   p.grid = sms * per_sm;
   if (p.grid > MAX_GRID) p.grid = MAX_GRID;
   const int64_t room = static_cast<int64_t>(p.width) << p.page_shift;
-  const int64_t units = static_cast<int64_t>(p.seqs) * p.heads * p.tiles * (1 + (room + UNIT - 1) / UNIT);
+  p.unit_shift = S::G == 2 ? 7 : 6;
+  static_assert(16 * KW == 64, "a unit is KW steps of 16 G keys");
+  const int64_t units = static_cast<int64_t>(p.seqs) * p.heads * p.tiles * (2 + (room >> p.unit_shift));
+  if (units > 0x7fffffff) return NOISE_ERR_SHAPE;
   if (units / 2 < p.grid) p.grid = units < 4 ? 1 : static_cast<int>(units / 2);
   if (static_cast<size_t>(2) * p.grid * S::RT * (D + 2) * sizeof(float) > workspace_bytes) return NOISE_ERR_WORKSPACE;
   kernel<<<p.grid, S::NT, smem, s>>>(p);
@@ -840,7 +952,7 @@ int run(Params& p, size_t workspace_bytes, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.seqs * p.heads * p.tiles);
   cfg.blockDim = dim3(256);
-  cfg.dynamicSmemBytes = (p.seqs + 1) * 4;
+  cfg.dynamicSmemBytes = (2 * p.seqs + 1) * 4;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -895,18 +1007,18 @@ int noise_tree_attention(const noise_kv_cache_t* cache, int layer, const void* q
   if (layer < 0 || layer >= cache->layers || seqs < 0 || seqs > MAX_SEQS || nodes < 1 || nodes > 64 || width < 0 ||
       q_heads < cache->heads || q_heads % cache->heads || q_heads / cache->heads > 64 ||
       static_cast<int64_t>(width) * cache->page_size > (1 << 30) ||
-      seqs * (static_cast<int64_t>(width) * cache->page_size / UNIT + 2) > 0x7fffffff)
+      static_cast<int64_t>(seqs) * cache->heads > 0x3fffffff)
     return NOISE_ERR_SHAPE;
   if (!(scale >= 1e-18f) || !(scale <= 1e18f)) return NOISE_ERR_ARGUMENT;
   if (seqs == 0) return NOISE_OK;
   if (!q || !k || !v || !lengths || !mask || !depth || !out || (width > 0 && !table)) return NOISE_ERR_ARGUMENT;
   for (const void* p : {static_cast<const void*>(cache->k), static_cast<const void*>(cache->v),
-                        static_cast<const void*>(cache->k_scale), static_cast<const void*>(cache->v_scale), q, k,
+                        static_cast<const void*>(cache->k_scale), static_cast<const void*>(cache->v_scale), q, k, v,
                         static_cast<const void*>(out), static_cast<const void*>(workspace)})
     if (reinterpret_cast<uintptr_t>(p) % 16) return NOISE_ERR_ALIGN;
-  if (reinterpret_cast<uintptr_t>(k) % 8 || reinterpret_cast<uintptr_t>(v) % 2) return NOISE_ERR_ALIGN;
-  for (int64_t stride : {q_seq_stride, q_node_stride, q_head_stride, k_seq_stride, k_node_stride, k_head_stride})
-    if (stride % 4) return NOISE_ERR_ALIGN;
+  for (int64_t stride : {q_seq_stride, q_node_stride, q_head_stride, k_seq_stride, k_node_stride, k_head_stride,
+                         v_seq_stride, v_node_stride, v_head_stride})
+    if (stride % 8) return NOISE_ERR_ALIGN;
   const int group = q_heads / cache->heads, tile = tile_rows(nodes * group);
   const int tiles = (nodes * group + tile - 1) / tile;
   if (static_cast<int64_t>(seqs) * cache->heads * tiles > 0x7fffffff) return NOISE_ERR_SHAPE;

@@ -350,14 +350,17 @@ def tree_attention(q, k, v, cache, table, lengths, mask, depth, layer=0, window=
     _ints('depth', depth, torch.int32, (seqs, nodes), dev)
     if not 0 <= layer < cache.layers:
         raise ValueError(f'layer: 0 to {cache.layers - 1}, got {layer}')
-    # the kernel loads four values of q and of k at once
+    # the kernel copies 16 bytes at a time
     qs, ks, vs = q.stride(), k.stride(), v.stride()
-    if q.data_ptr() % 16 or (qs[0] | qs[1] | qs[2]) % 4:
+    if q.data_ptr() % 16 or (qs[0] | qs[1] | qs[2]) % 8:
         q = q.contiguous()
         qs = q.stride()
-    if k.data_ptr() % 8 or (ks[0] | ks[1] | ks[2]) % 4:
+    if k.data_ptr() % 16 or (ks[0] | ks[1] | ks[2]) % 8:
         k = k.contiguous()
         ks = k.stride()
+    if v.data_ptr() % 16 or (vs[0] | vs[1] | vs[2]) % 8:
+        v = v.contiguous()
+        vs = v.stride()
     out = torch.empty((seqs, nodes, heads, dim), dtype=torch.bfloat16, device=dev)
     nbytes = _attention_bytes(seqs, nodes, heads, k_heads, dim)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
