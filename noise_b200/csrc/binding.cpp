@@ -1,0 +1,487 @@
+// The Python side of noise_b200.decode in C++: argument checks, allocation with torch, the current stream, and the call of
+// the C ABI. A decoding step makes dozens of these calls, each a few microseconds on the GPU; the same checks and
+// the ctypes call took 12 to 19 us of the host, here 4 to 6.
+//
+// Errors: TypeError for a dtype, ValueError for a shape, layout, device or value, NoiseError for tensors that are not
+// on a GPU and for the library's own statuses. The entry points come from the library that load() is given.
+#include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <dlfcn.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <cmath>
+#include <initializer_list>
+#include <limits>
+#include <string>
+
+#include "noise_b200.h"
+
+namespace {
+
+using at::Tensor;
+
+struct Entries {
+  decltype(&noise_head_norm_rope) head_norm_rope;
+  decltype(&noise_head_norm_rope_backward_workspace_bytes) backward_bytes;
+  decltype(&noise_head_norm_rope_backward) head_norm_rope_backward;
+  decltype(&noise_kv_write) kv_write;
+  decltype(&noise_kv_read) kv_read;
+  decltype(&noise_tree_plan) tree_plan;
+  decltype(&noise_tree_attention_workspace_bytes) attention_bytes;
+  decltype(&noise_tree_attention) tree_attention;
+  decltype(&noise_verify_tree) verify_tree;
+  decltype(&noise_status_string) status_string;
+} entry;
+PyObject* noise_error = nullptr;
+
+[[noreturn]] void fail(const std::string& message) {
+  PyErr_SetString(noise_error ? noise_error : PyExc_RuntimeError, message.c_str());
+  throw python_error();
+}
+[[noreturn]] void type_error(const std::string& message) {
+  PyErr_SetString(PyExc_TypeError, message.c_str());
+  throw python_error();
+}
+[[noreturn]] void value_error(const std::string& message) {
+  PyErr_SetString(PyExc_ValueError, message.c_str());
+  throw python_error();
+}
+
+std::string text(at::IntArrayRef v) {
+  std::string s = "(";
+  for (size_t i = 0; i < v.size(); ++i) s += (i ? ", " : "") + std::to_string(v[i]);
+  return s + ")";
+}
+std::string text(const Tensor& t) {
+  return std::string(c10::toString(t.scalar_type())) + " " + text(t.sizes()) + ", strides " + text(t.strides()) + " on " +
+         t.device().str();
+}
+
+void check(int status, const char* name) {
+  if (status != NOISE_OK)
+    fail(std::string(name) + ": " + entry.status_string(status) + " (status " + std::to_string(status) + ")");
+}
+
+const Tensor& tensor(PyObject* o, const char* name) {
+  if (!THPVariable_Check(o)) type_error(std::string(name) + ": a tensor is expected, got " + Py_TYPE(o)->tp_name);
+  const Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_cuda()) fail("noise_b200 ops run on CUDA tensors only (no CPU fallback)");
+  return t;
+}
+Tensor optional(PyObject* o, const char* name) { return o == Py_None ? Tensor() : tensor(o, name); }
+
+int64_t integer(PyObject* o, const char* name) {
+  const long long v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) throw python_error();
+  if (v < std::numeric_limits<int>::min() || v > std::numeric_limits<int>::max())
+    value_error(std::string(name) + ": " + std::to_string(v));
+  return v;
+}
+double number(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw python_error();
+  return v;
+}
+
+bool floating(const Tensor& t) { return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16; }
+int dtype_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? NOISE_DTYPE_F32 : NOISE_DTYPE_BF16; }
+
+// A floating operand: `dims` dimensions, the last one contiguous.
+void rows(const char* name, const Tensor& t, int64_t dims, c10::Device device) {
+  if (t.dim() != dims || (t.stride(-1) != 1 && t.size(-1) > 1))
+    value_error(std::string(name) + ": " + std::to_string(dims) + " dimensions, the last one contiguous; got " + text(t));
+  if (t.device() != device) value_error(std::string(name) + ": expected on " + device.str() + ", got " + text(t));
+  for (const int64_t n : t.sizes())
+    if (n > std::numeric_limits<int>::max()) value_error(std::string(name) + ": too large, " + text(t));
+}
+
+// Whole numbers or random ones: a contiguous tensor of that type and shape.
+void plain(const char* name, const Tensor& t, at::ScalarType type, at::IntArrayRef shape, c10::Device device) {
+  if (t.scalar_type() != type)
+    type_error(std::string(name) + ": " + c10::toString(type) + " is expected, got " + text(t));
+  if (t.sizes() != shape || !t.is_contiguous() || t.device() != device)
+    value_error(std::string(name) + ": contiguous " + text(shape) + " on " + device.str() + " is expected, got " + text(t));
+}
+
+void* address(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+struct On {  // the device current, and its current stream
+  c10::cuda::CUDAGuard guard;
+  void* stream;
+  explicit On(c10::Device d) : guard(d), stream(c10::cuda::getCurrentCUDAStream(d.index()).stream()) {}
+};
+
+void arguments(Py_ssize_t got, Py_ssize_t want, const char* name) {
+  if (got != want) type_error(std::string(name) + ": " + std::to_string(want) + " arguments, got " + std::to_string(got));
+  if (!entry.status_string) fail("the library is not loaded");
+}
+
+// ---- head norm and rotation -------------------------------------------------------------------------------------
+
+struct Norm {  // q, k, cos, sin, positions, q_weight, k_weight, eps
+  Tensor q, k, cos, sin, positions, q_weight, k_weight;
+  float eps;
+  int tokens, dim;
+  noise_heads_t qh, kh;
+
+  explicit Norm(PyObject* const* a)
+      : q(tensor(a[0], "q")), k(tensor(a[1], "k")), cos(tensor(a[2], "cos")), sin(tensor(a[3], "sin")),
+        positions(tensor(a[4], "positions")), q_weight(optional(a[5], "q_weight")), k_weight(optional(a[6], "k_weight")) {
+    const c10::Device dev = q.device();
+    if (!floating(q) || k.scalar_type() != q.scalar_type()) type_error("q and k: fp32 or bf16, alike; got " + text(q) + "; " + text(k));
+    if (!floating(cos) || sin.scalar_type() != cos.scalar_type())
+      type_error("cos and sin: fp32 or bf16, alike; got " + text(cos) + "; " + text(sin));
+    rows("q", q, 3, dev);
+    rows("k", k, 3, dev);
+    if (k.size(0) != q.size(0) || k.size(2) != q.size(2))
+      value_error("q [tokens, heads, D], k [tokens, k heads, D]: got " + text(q) + "; " + text(k));
+    tokens = static_cast<int>(q.size(0));
+    dim = static_cast<int>(q.size(2));
+    if (dim < 2 || dim > 256 || dim % 2) value_error("D: even, 2 to 256; got " + std::to_string(dim));
+    if (q.size(1) < 1 || q.size(1) > 4096 || k.size(1) < 1 || k.size(1) > 4096)
+      value_error("heads: 1 to 4096; got " + text(q) + "; " + text(k));
+    if (cos.dim() != 2 || cos.size(0) < 1 || cos.size(0) > std::numeric_limits<int>::max() || cos.size(1) * 2 != dim ||
+        sin.sizes() != cos.sizes() || !cos.is_contiguous() || !sin.is_contiguous() || cos.device() != dev ||
+        sin.device() != dev)
+      value_error("cos, sin: contiguous [positions, D / 2] on q's device; got " + text(cos) + "; " + text(sin));
+    plain("positions", positions, at::kInt, {tokens}, dev);
+    for (const Tensor* w : {&q_weight, &k_weight})
+      if (w->defined()) plain(w == &q_weight ? "q_weight" : "k_weight", *w, q.scalar_type(), {dim}, dev);
+    if (a[7] == Py_None)  // F.rms_norm's
+      eps = q.scalar_type() == at::kFloat ? std::numeric_limits<float>::epsilon() : 0.0078125f;
+    else
+      eps = static_cast<float>(number(a[7]));
+    if (!(eps >= 0.f) || std::isinf(eps)) value_error("eps: " + std::to_string(eps));
+    qh = heads(q);
+    kh = heads(k);
+  }
+  static noise_heads_t heads(const Tensor& t) {
+    return {t.data_ptr(), t.stride(0), t.stride(1), static_cast<int>(t.size(1))};
+  }
+};
+
+PyObject* pair(const Tensor& a, const Tensor& b) {
+  PyObject* t = PyTuple_New(2);
+  if (!t) throw python_error();
+  PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(a));
+  PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(b));
+  return t;
+}
+
+PyObject* head_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arguments(n, 8, "head_norm_rope");
+  const Norm c(a);
+  const Tensor q = at::empty(c.q.sizes(), c.q.options()), k = at::empty(c.k.sizes(), c.q.options());
+  const On on(c.q.device());
+  check(entry.head_norm_rope(&c.qh, &c.kh, c.cos.data_ptr(), c.sin.data_ptr(), dtype_of(c.cos),
+                             static_cast<int>(c.cos.size(0)), static_cast<const int*>(c.positions.data_ptr()), c.tokens,
+                             c.dim, dtype_of(c.q), address(c.q_weight), address(c.k_weight), c.eps, q.data_ptr(),
+                             k.data_ptr(), on.stream),
+        "noise_head_norm_rope");
+  return pair(q, k);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* head_norm_rope_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arguments(n, 10, "head_norm_rope_backward");
+  const Norm c(a + 2);
+  const Tensor dq = tensor(a[0], "dq"), dk = tensor(a[1], "dk");
+  const c10::Device dev = c.q.device();
+  if (dq.scalar_type() != c.q.scalar_type() || dk.scalar_type() != c.q.scalar_type())
+    type_error("dq, dk: of q's dtype; got " + text(dq) + "; " + text(dk));
+  rows("dq", dq, 3, dev);
+  rows("dk", dk, 3, dev);
+  if (dq.sizes() != c.q.sizes() || dk.sizes() != c.k.sizes())
+    value_error("dq, dk: of the shapes " + text(c.q.sizes()) + ", " + text(c.k.sizes()) + "; got " + text(dq) + "; " + text(dk));
+  const Tensor q = at::empty(c.q.sizes(), c.q.options()), k = at::empty(c.k.sizes(), c.q.options());
+  Tensor qw, kw, ws;
+  size_t bytes = 0;
+  if (c.q_weight.defined()) qw = at::empty({c.dim}, c.q.options().dtype(at::kFloat));
+  if (c.k_weight.defined()) kw = at::empty({c.dim}, c.q.options().dtype(at::kFloat));
+  if (qw.defined() || kw.defined()) {
+    bytes = entry.backward_bytes(c.dim);
+    ws = at::empty({static_cast<int64_t>(bytes)}, c.q.options().dtype(at::kByte));
+  }
+  const noise_heads_t dqh = Norm::heads(dq), dkh = Norm::heads(dk);
+  const On on(dev);
+  check(entry.head_norm_rope_backward(
+            &dqh, &dkh, &c.qh, &c.kh, c.cos.data_ptr(), c.sin.data_ptr(), dtype_of(c.cos),
+            static_cast<int>(c.cos.size(0)), static_cast<const int*>(c.positions.data_ptr()), c.tokens, c.dim,
+            dtype_of(c.q), address(c.q_weight), address(c.k_weight), c.eps, q.data_ptr(), k.data_ptr(),
+            static_cast<float*>(address(qw)), static_cast<float*>(address(kw)), address(ws), bytes, on.stream),
+        "noise_head_norm_rope_backward");
+  PyObject* t = PyTuple_New(4);
+  if (!t) throw python_error();
+  PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(q));
+  PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(k));
+  PyTuple_SET_ITEM(t, 2, THPVariable_Wrap(qw));  // (an undefined tensor is None)
+  PyTuple_SET_ITEM(t, 3, THPVariable_Wrap(kw));
+  return t;
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- the cache ----------------------------------------------------------------------------------------------------
+
+struct Cache {  // its k tensor and the address of its noise_kv_cache_t
+  const noise_kv_cache_t* c;
+  c10::Device device;
+  at::TensorOptions options;
+  Cache(PyObject* k, PyObject* at) : c(nullptr), device(c10::kCUDA) {
+    const Tensor& t = tensor(k, "cache.k");
+    device = t.device();
+    options = t.options();
+    c = static_cast<const noise_kv_cache_t*>(PyLong_AsVoidPtr(at));
+    if (!c) {
+      if (!PyErr_Occurred()) value_error("no cache");
+      throw python_error();
+    }
+  }
+};
+
+struct Places {  // seq, pos, table, layer
+  Tensor seq, pos, table;
+  int tokens, first, layers;
+  bool all;
+  Places(PyObject* const* a, const Cache& cache)
+      : seq(tensor(a[0], "seq")), pos(tensor(a[1], "pos")), table(tensor(a[2], "table")) {
+    if (seq.dim() != 1 || table.dim() != 2)
+      value_error("seq [tokens], table [sequences, pages]: got " + text(seq) + "; " + text(table));
+    plain("seq", seq, at::kInt, seq.sizes(), cache.device);
+    plain("pos", pos, at::kInt, seq.sizes(), cache.device);
+    plain("table", table, at::kInt, table.sizes(), cache.device);
+    for (const int64_t size : {seq.size(0), table.size(0), table.size(1)})
+      if (size > std::numeric_limits<int>::max()) value_error("too large: " + text(seq) + "; " + text(table));
+    tokens = static_cast<int>(seq.size(0));
+    all = a[3] == Py_None;
+    first = all ? 0 : static_cast<int>(integer(a[3], "layer"));
+    layers = all ? cache.c->layers : 1;
+    if (first < 0 || first >= cache.c->layers)
+      value_error("layer: 0 to " + std::to_string(cache.c->layers - 1) + ", or None for all; got " + std::to_string(first));
+  }
+  const int* of(const Tensor& t) const { return static_cast<const int*>(t.data_ptr()); }
+};
+
+// cache.k, address, k, v, seq, pos, table, layer, rows
+PyObject* kv_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arguments(n, 9, "write");
+  const Cache cache(a[0], a[1]);
+  const Tensor &k = tensor(a[2], "k"), &v = tensor(a[3], "v");
+  const Places at(a + 4, cache);
+  const Tensor list = optional(a[8], "rows");
+  if (!floating(k) || v.scalar_type() != k.scalar_type()) type_error("k and v: fp32 or bf16, alike; got " + text(k) + "; " + text(v));
+  const int dims = at.all ? 4 : 3;
+  rows("k", k, dims, cache.device);
+  rows("v", v, dims, cache.device);
+  const int64_t source = k.size(-3);
+  if (k.size(-2) != cache.c->heads || k.size(-1) != cache.c->dim || (at.all && k.size(0) != at.layers) || v.sizes() != k.sizes())
+    value_error("k, v: [" + std::string(at.all ? std::to_string(at.layers) + ", " : "") + "rows, " +
+                std::to_string(cache.c->heads) + ", " + std::to_string(cache.c->dim) + "]; got " + text(k) + "; " + text(v));
+  if (list.defined()) plain("rows", list, at::kInt, at.seq.sizes(), cache.device);
+  else if (source < at.tokens) value_error(std::to_string(at.tokens) + " tokens, but " + std::to_string(source) + " rows");
+  const On on(cache.device);
+  check(entry.kv_write(cache.c, at.first, at.layers, k.data_ptr(), at.all ? k.stride(0) : 0, k.stride(-3), k.stride(-2),
+                       v.data_ptr(), at.all ? v.stride(0) : 0, v.stride(-3), v.stride(-2), static_cast<int>(source),
+                       dtype_of(k), at.tokens, at.of(at.seq), at.of(at.pos),
+                       list.defined() ? at.of(list) : nullptr, at.of(at.table), static_cast<int>(at.table.size(0)),
+                       static_cast<int>(at.table.size(1)), on.stream),
+        "noise_kv_write");
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+// cache.k, address, seq, pos, table, layer, bf16 or fp32
+PyObject* kv_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arguments(n, 7, "read");
+  const Cache cache(a[0], a[1]);
+  const Places at(a + 2, cache);
+  const int dtype = static_cast<int>(integer(a[6], "dtype"));
+  const auto options = cache.options.dtype(dtype == NOISE_DTYPE_F32 ? at::kFloat : at::kBFloat16);
+  c10::SmallVector<int64_t, 4> shape;
+  if (at.all) shape.push_back(at.layers);
+  shape.append({at.tokens, cache.c->heads, cache.c->dim});
+  const Tensor k = at::empty(shape, options), v = at::empty(shape, options);
+  const On on(cache.device);
+  check(entry.kv_read(cache.c, at.first, at.layers, k.data_ptr(), v.data_ptr(), dtype, at.tokens, at.of(at.seq),
+                      at.of(at.pos), at.of(at.table), static_cast<int>(at.table.size(0)),
+                      static_cast<int>(at.table.size(1)), on.stream),
+        "noise_kv_read");
+  return pair(k, v);
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- the tree -----------------------------------------------------------------------------------------------------
+
+constexpr int64_t MAX_NODES = 64, MAX_VOCAB = 393216;
+
+PyObject* tree_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arguments(n, 1, "tree_plan");
+  const Tensor& parents = tensor(a[0], "parents");
+  if (parents.dim() != 2 || parents.size(1) < 1 || parents.size(1) > MAX_NODES || parents.size(0) > (1 << 24))
+    value_error("parents: [B, N], N 1 to 64; got " + text(parents));
+  plain("parents", parents, at::kInt, parents.sizes(), parents.device());
+  const Tensor mask = at::empty(parents.sizes(), parents.options().dtype(at::kLong));
+  const Tensor depth = at::empty(parents.sizes(), parents.options());
+  const On on(parents.device());
+  check(entry.tree_plan(static_cast<const int*>(parents.data_ptr()), static_cast<int>(parents.size(0)),
+                        static_cast<int>(parents.size(1)), static_cast<int64_t*>(mask.data_ptr()),
+                        static_cast<int*>(depth.data_ptr()), on.stream),
+        "noise_tree_plan");
+  return pair(mask, depth);
+  END_HANDLE_TH_ERRORS
+}
+
+// The kernel copies 16 bytes at a time.
+Tensor aligned(const Tensor& t) {
+  return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 || (t.stride(0) | t.stride(1) | t.stride(2)) % 8 ? t.contiguous() : t;
+}
+
+// q, k, v, cache.k, address, table, lengths, mask, depth, layer, window, scale
+PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arguments(n, 12, "tree_attention");
+  Tensor q = tensor(a[0], "q"), k = tensor(a[1], "k"), v = tensor(a[2], "v");
+  const Cache cache(a[3], a[4]);
+  const Tensor &table = tensor(a[5], "table"), &lengths = tensor(a[6], "lengths"), &mask = tensor(a[7], "mask"),
+               &depth = tensor(a[8], "depth");
+  if (q.scalar_type() != at::kBFloat16 || k.scalar_type() != at::kBFloat16 || v.scalar_type() != at::kBFloat16)
+    type_error("q, k, v: bf16; got " + text(q) + "; " + text(k) + "; " + text(v));
+  rows("q", q, 4, cache.device);
+  rows("k", k, 4, cache.device);
+  rows("v", v, 4, cache.device);
+  const int64_t seqs = q.size(0), nodes = q.size(1), heads = q.size(2), dim = q.size(3), kheads = cache.c->heads;
+  if (dim != cache.c->dim || (dim != 64 && dim != 128))
+    value_error("D: the cache's, 64 or 128; got " + std::to_string(dim) + ", the cache has " + std::to_string(cache.c->dim));
+  const int64_t want[4] = {seqs, nodes, kheads, dim};
+  if (k.sizes() != at::IntArrayRef(want) || v.sizes() != at::IntArrayRef(want))
+    value_error("k, v: " + text(at::IntArrayRef(want)) + "; got " + text(k) + "; " + text(v));
+  if (nodes < 1 || nodes > MAX_NODES) value_error("nodes: 1 to 64, got " + std::to_string(nodes));
+  if (heads < kheads || heads % kheads || heads / kheads > 64)
+    value_error("q heads: a multiple of the cache's " + std::to_string(kheads) + ", at most 64 times it; got " + std::to_string(heads));
+  if (table.dim() != 2 || table.size(0) != seqs || table.size(1) > std::numeric_limits<int>::max())
+    value_error("table: [" + std::to_string(seqs) + ", pages]; got " + text(table));
+  plain("table", table, at::kInt, table.sizes(), cache.device);
+  plain("lengths", lengths, at::kInt, {seqs}, cache.device);
+  plain("mask", mask, at::kLong, {seqs, nodes}, cache.device);
+  plain("depth", depth, at::kInt, {seqs, nodes}, cache.device);
+  const int layer = static_cast<int>(integer(a[9], "layer")), window = static_cast<int>(integer(a[10], "window"));
+  if (layer < 0 || layer >= cache.c->layers)
+    value_error("layer: 0 to " + std::to_string(cache.c->layers - 1) + ", got " + std::to_string(layer));
+  const float scale = a[11] == Py_None ? 1.f / std::sqrt(static_cast<float>(dim)) : static_cast<float>(number(a[11]));
+  q = aligned(q), k = aligned(k), v = aligned(v);
+  const Tensor out = at::empty({seqs, nodes, heads, dim}, q.options());
+  const size_t bytes = entry.attention_bytes(static_cast<int>(seqs), static_cast<int>(nodes), static_cast<int>(heads),
+                                             static_cast<int>(kheads), static_cast<int>(dim));
+  const Tensor ws = at::empty({static_cast<int64_t>(bytes ? bytes : 16)}, q.options().dtype(at::kByte));
+  const On on(cache.device);
+  check(entry.tree_attention(
+            cache.c, layer, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), static_cast<int>(heads), k.data_ptr(),
+            k.stride(0), k.stride(1), k.stride(2), v.data_ptr(), v.stride(0), v.stride(1), v.stride(2),
+            static_cast<int>(seqs), static_cast<int>(nodes), static_cast<const int*>(table.data_ptr()),
+            static_cast<int>(table.size(1)), static_cast<const int*>(lengths.data_ptr()),
+            static_cast<const int64_t*>(mask.data_ptr()), static_cast<const int*>(depth.data_ptr()), window, scale,
+            out.data_ptr(), ws.data_ptr(), bytes, on.stream),
+        "noise_tree_attention");
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// logits, tokens, parents, u, race, probs, temperature, softcap
+PyObject* verify_tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arguments(n, 8, "verify_tree");
+  const Tensor &logits = tensor(a[0], "logits"), &tokens = tensor(a[1], "tokens"), &parents = tensor(a[2], "parents");
+  const c10::Device dev = logits.device();
+  if (!floating(logits)) type_error("logits: fp32 or bf16, got " + text(logits));
+  rows("logits", logits, 3, dev);
+  const int64_t seqs = logits.size(0), nodes = logits.size(1), vocab = logits.size(2);
+  if (nodes < 1 || nodes > MAX_NODES) value_error("nodes: 1 to 64, got " + std::to_string(nodes));
+  if (vocab < 1 || vocab > MAX_VOCAB) value_error("vocabulary: 1 to 393216, got " + std::to_string(vocab));
+  const double temperature = number(a[6]), softcap = number(a[7]);
+  if (!(temperature >= 0) || std::isinf(temperature) || !(softcap >= 0) || std::isinf(softcap))
+    value_error("temperature and softcap: at least 0; got " + std::to_string(temperature) + ", " + std::to_string(softcap));
+  plain("tokens", tokens, at::kLong, {seqs, nodes}, dev);
+  plain("parents", parents, at::kInt, {seqs, nodes}, dev);
+  Tensor u, race, probs;
+  if (temperature > 0) {
+    u = tensor(a[3], "u"), race = tensor(a[4], "race"), probs = optional(a[5], "probs");
+    plain("u", u, at::kFloat, {seqs, nodes}, dev);
+    plain("race", race, at::kFloat, {seqs, vocab}, dev);
+    if (probs.defined()) {
+      if (probs.scalar_type() != at::kFloat) type_error("probs: fp32, got " + text(probs));
+      rows("probs", probs, 3, dev);
+      if (probs.sizes() != logits.sizes()) value_error("probs: " + text(logits.sizes()) + ", got " + text(probs));
+    }
+  }
+  const auto ints = logits.options().dtype(at::kInt);
+  const Tensor count = at::empty({seqs}, ints), path = at::empty({seqs, nodes}, ints);
+  const Tensor token = at::empty({seqs}, logits.options().dtype(at::kLong));
+  const On on(dev);
+  check(entry.verify_tree(logits.data_ptr(), dtype_of(logits), logits.stride(0), logits.stride(1),
+                          static_cast<const int64_t*>(tokens.data_ptr()), static_cast<const int*>(parents.data_ptr()),
+                          static_cast<const float*>(address(u)), static_cast<const float*>(address(race)),
+                          static_cast<const float*>(address(probs)), probs.defined() ? probs.stride(0) : 0,
+                          probs.defined() ? probs.stride(1) : 0, static_cast<int>(seqs), static_cast<int>(nodes),
+                          static_cast<int>(vocab), static_cast<float>(temperature), static_cast<float>(softcap),
+                          static_cast<int*>(count.data_ptr()), static_cast<int*>(path.data_ptr()),
+                          static_cast<int64_t*>(token.data_ptr()), on.stream),
+        "noise_verify_tree");
+  PyObject* t = PyTuple_New(3);
+  if (!t) throw python_error();
+  PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(count));
+  PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(path));
+  PyTuple_SET_ITEM(t, 2, THPVariable_Wrap(token));
+  return t;
+  END_HANDLE_TH_ERRORS
+}
+
+// load(path of the library, NoiseError)
+PyObject* load(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 2) type_error("load: 2 arguments");
+  const char* path = PyUnicode_AsUTF8(a[0]);
+  if (!path) throw python_error();
+  Py_INCREF(a[1]);
+  Py_XDECREF(noise_error);
+  noise_error = a[1];
+  void* lib = dlopen(path, RTLD_NOW | RTLD_LOCAL);
+  if (!lib) fail(dlerror());
+  const auto find = [&](const char* name) {
+    void* f = dlsym(lib, name);
+    if (!f) fail(std::string(path) + " has no " + name);
+    return f;
+  };
+  Entries e;
+#define NOISE_FIND(field, name) e.field = reinterpret_cast<decltype(&name)>(find(#name))
+  NOISE_FIND(head_norm_rope, noise_head_norm_rope);
+  NOISE_FIND(backward_bytes, noise_head_norm_rope_backward_workspace_bytes);
+  NOISE_FIND(head_norm_rope_backward, noise_head_norm_rope_backward);
+  NOISE_FIND(kv_write, noise_kv_write);
+  NOISE_FIND(kv_read, noise_kv_read);
+  NOISE_FIND(tree_plan, noise_tree_plan);
+  NOISE_FIND(attention_bytes, noise_tree_attention_workspace_bytes);
+  NOISE_FIND(tree_attention, noise_tree_attention);
+  NOISE_FIND(verify_tree, noise_verify_tree);
+  NOISE_FIND(status_string, noise_status_string);
+#undef NOISE_FIND
+  entry = e;
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+#define NOISE_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
+PyMethodDef methods[] = {NOISE_METHOD(load),           NOISE_METHOD(head_norm_rope), NOISE_METHOD(head_norm_rope_backward),
+                         NOISE_METHOD(kv_write),       NOISE_METHOD(kv_read),        NOISE_METHOD(tree_plan),
+                         NOISE_METHOD(tree_attention), NOISE_METHOD(verify_tree),    {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_decode_ext", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__decode_ext(void) { return PyModule_Create(&module); }

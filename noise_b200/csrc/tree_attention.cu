@@ -35,6 +35,8 @@ namespace noise {
 namespace tree {
 
 constexpr int KW = 4;            // warps that share a row tile's keys: a unit is one step of each
+constexpr int LEAST = 2;         // units a CTA takes at least: a shorter span is all overhead
+constexpr int HEAD = 3;          // what an item costs beside its cached keys, in units
 constexpr int MAX_SEQS = 4096;  // two words each in shared memory
 constexpr int VREF = 127 - 20;   // the output's first unit is 2^-20: V rows with less than that as a scale lose bits
 constexpr float NEG = -INFINITY;
@@ -116,9 +118,9 @@ __device__ __forceinline__ int first_unit(const Params& p, int len) {
   return p.window < 0 || p.window >= len ? 0 : (len - p.window) >> p.unit_shift;
 }
 
-// Units of one item of a sequence: one for its nodes, then its cached keys'.
+// Units of one item of a sequence: HEAD for its queries, its nodes' own keys and its output, then its cached keys'.
 __device__ __forceinline__ int units_of(const Params& p, int len) {
-  return 1 + ((len + (1 << p.unit_shift) - 1) >> p.unit_shift) - first_unit(p, len);
+  return HEAD + ((len + (1 << p.unit_shift) - 1) >> p.unit_shift) - first_unit(p, len);
 }
 
 // before[b] = units of one item of each sequence before b, lens[b] its length; every thread of the block calls it.
@@ -151,7 +153,7 @@ struct Spans {
   int ctas, each, more;
   __device__ __forceinline__ Spans(const Params& p, const int* before) {
     const int total = before[p.seqs] * p.heads * p.tiles;
-    ctas = min(p.grid, max(1, total >> 1));  // at least two units each: a shorter span is all overhead
+    ctas = min(p.grid, max(1, total / LEAST));
     each = total / ctas;
     more = total - each * ctas;
   }
@@ -386,7 +388,7 @@ __global__ void __launch_bounds__(Shape<KIND, D, NTL, RW>::NT)
     const int h = item / p.tiles, tile = item - h * p.tiles;
     const int row0 = tile * S::RT + rw * 8 * NTL;
     const int len = lens[b];
-    const int unit0 = first_unit(p, len) - 1;  // unit u holds the keys from (unit0 + u) << unit_shift on
+    const int unit0 = first_unit(p, len) - HEAD;  // unit u holds the keys from (unit0 + u) << unit_shift on
 
     // ---- first on their way: Q and the tree's own keys and values
     const __nv_bfloat16* qb = p.q + b * p.q_seq;
@@ -427,7 +429,7 @@ __global__ void __launch_bounds__(Shape<KIND, D, NTL, RW>::NT)
     // ---- then the cached keys' first copies
     const int* table = p.table + static_cast<int64_t>(b) * p.width;
     const int cshift = p.page_shift - 4;
-    int chunk = (unit0 + (u0 > 1 ? u0 : 1)) * KW + kw;  // of 16 G keys
+    int chunk = (unit0 + max(u0, HEAD)) * KW + kw;  // of 16 G keys
     const int chunk_end = min((unit0 + u1) * KW, (len + 16 * G - 1) / (16 * G));
     int ahead = chunk, page0 = -64, pages = 0;
     bool lost = false;
@@ -858,9 +860,29 @@ __global__ void __launch_bounds__(Shape<KIND, D, NTL, RW>::NT)
   }
 }
 
-// Joins the parts of one item (a block each): o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i (off = -m), in the parts' order.
-__global__ void __launch_bounds__(256) join_kernel(const Params p, int rt, int dim) {
+// A part of a row's output: the sum of its values, of its probabilities, and less its maximum in powers of two.
+struct Sum {
+  float4 o;
+  float l, off;
+  __device__ __forceinline__ void add(const float4& x, float xl, float xoff) {
+    const float low = fminf(off, xoff);
+    const float f = off == NONE ? 0.f : ex2(low - off), g = xoff == NONE ? 0.f : ex2(low - xoff);
+    // a part that saw no key may still hold the NaN of a lost page
+    l = (off == NONE ? l : l * f) + (xoff == NONE ? xl : xl * g);
+    o.x = o.x * f + x.x * g, o.y = o.y * f + x.y * g, o.z = o.z * f + x.z * g, o.w = o.w * f + x.w * g;
+    off = low;
+  }
+};
+
+constexpr int JOIN_NT = 256;
+
+// Joins the parts of an item: o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i (off = -m). A block takes JOIN_NT / shares
+// groups of 4 values (blockIdx.y: which); `shares` threads go through a group's parts, every shares-th each, and the
+// first joins theirs, so the order is the same from call to call. (The CTA whose part comes last joining them all, one
+// launch, measured slower: 117 us against 102 on 8 rows of up to 65,536 keys, 14.5 against 11.0 on a decoding step.)
+__global__ void __launch_bounds__(JOIN_NT) join_kernel(const Params p, int rt, int dim, int shares) {
   extern __shared__ int before[];
+  __shared__ Sum sums[JOIN_NT];
   line_of(p, before, before + p.seqs + 1);
   const Spans spans(p, before);
   const int hr = p.heads * p.tiles;
@@ -871,44 +893,45 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p, int rt, int d
   cudaGridDependencySynchronize();
   if (c0 == c1) return;  // it was written whole
   const int slot0 = 2 * c0 + (spans.cut(c0) == u ? 0 : 1);
-  const int h = item / p.tiles, tile = item - h * p.tiles, rows = p.nodes * p.group;
-  const float* sums = p.partial + static_cast<int64_t>(2 * p.grid) * rt * dim;
-  const int quads = dim / 4;
-  for (int i = threadIdx.x; i < rt * quads; i += blockDim.x) {
-    const int in = i / quads, d = (i - in * quads) * 4, r = tile * rt + in;
-    if (r >= rows) return;
-    const int node = r / p.group;
-    float off = NONE, l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c = c0; c <= c1; c += 4) {  // four parts' loads at once
+  const int h = item / p.tiles, tile = item - h * p.tiles, rows = p.nodes * p.group, quads = dim / 4;
+  const int groups = JOIN_NT / shares, share = threadIdx.x / groups;
+  const int i = blockIdx.y * groups + threadIdx.x % groups, in = i / quads, d = (i - in * quads) * 4, r = tile * rt + in;
+  const bool real = in < rt && r < rows;
+  const float* ml = p.partial + static_cast<int64_t>(2 * p.grid) * rt * dim;
+  Sum sum = {make_float4(0.f, 0.f, 0.f, 0.f), 0.f, NONE};
+  if (real)
+    for (int c = c0 + share; c <= c1; c += 4 * shares) {  // four parts' loads at once
       float oo[4], sl[4];
       float4 x[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        oo[j] = NONE, sl[j] = 0.f, x[j] = o;
-        if (c + j > c1) continue;
-        const int64_t slot = c + j == c0 ? slot0 : 2 * (c + j);
-        oo[j] = sums[slot * 2 * rt + in], sl[j] = sums[slot * 2 * rt + rt + in];
+        const int at = c + j * shares;
+        oo[j] = NONE, sl[j] = 0.f, x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (at > c1) continue;
+        const int64_t slot = at == c0 ? slot0 : 2 * at;
+        oo[j] = ml[slot * 2 * rt + in], sl[j] = ml[slot * 2 * rt + rt + in];
         x[j] = *reinterpret_cast<const float4*>(p.partial + (slot * rt + in) * dim + d);
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float low = fminf(off, oo[j]);
-        const float f = off == NONE ? 0.f : ex2(low - off), g = oo[j] == NONE ? 0.f : ex2(low - oo[j]);
-        // a part that saw no key may still hold the NaN of a lost page
-        l = (off == NONE ? l : l * f) + (oo[j] == NONE ? sl[j] : sl[j] * g);
-        o.x = o.x * f + x[j].x * g, o.y = o.y * f + x[j].y * g;
-        o.z = o.z * f + x[j].z * g, o.w = o.w * f + x[j].w * g;
-        off = low;
-      }
+      for (int j = 0; j < 4; ++j) sum.add(x[j], sl[j], oo[j]);
     }
-    const bool none = l == 0.f || p.depth[b * p.nodes + node] < 0;
-    const float f = none ? 0.f : 1.f / l;
-    __nv_bfloat16* out =
-        p.out + ((static_cast<int64_t>(b) * p.nodes + node) * p.heads * p.group + h * p.group + r - node * p.group) * dim;
-    *reinterpret_cast<uint2*>(out + d) = none ? make_uint2(0, 0)
-                                              : make_uint2(pack_bf16(o.x * f, o.y * f), pack_bf16(o.z * f, o.w * f));
+  if (shares > 1) {
+    sums[threadIdx.x] = sum;
+    __syncthreads();
+    if (share > 0) return;
+    for (int k = 1; k < shares; ++k) {
+      const Sum& other = sums[k * groups + threadIdx.x];
+      sum.add(other.o, other.l, other.off);
+    }
   }
+  if (!real) return;
+  const int node = r / p.group;
+  const bool none = sum.l == 0.f || p.depth[b * p.nodes + node] < 0;
+  const float f = none ? 0.f : 1.f / sum.l;
+  __nv_bfloat16* out =
+      p.out + ((static_cast<int64_t>(b) * p.nodes + node) * p.heads * p.group + h * p.group + r - node * p.group) * dim;
+  *reinterpret_cast<uint2*>(out + d) =
+      none ? make_uint2(0, 0) : make_uint2(pack_bf16(sum.o.x * f, sum.o.y * f), pack_bf16(sum.o.z * f, sum.o.w * f));
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------
@@ -943,15 +966,19 @@ int run(Params& p, size_t workspace_bytes, cudaStream_t s) {
   const int64_t room = static_cast<int64_t>(p.width) << p.page_shift;
   p.unit_shift = S::G == 2 ? 7 : 6;
   static_assert(16 * KW == 64, "a unit is KW steps of 16 G keys");
-  const int64_t units = static_cast<int64_t>(p.seqs) * p.heads * p.tiles * (2 + (room >> p.unit_shift));
+  const int64_t units = static_cast<int64_t>(p.seqs) * p.heads * p.tiles * (HEAD + 1 + (room >> p.unit_shift));
   if (units > 0x7fffffff) return NOISE_ERR_SHAPE;
-  if (units / 2 < p.grid) p.grid = units < 4 ? 1 : static_cast<int>(units / 2);
+  if (units / LEAST < p.grid) p.grid = units < 2 * LEAST ? 1 : static_cast<int>(units / LEAST);
   if (static_cast<size_t>(2) * p.grid * S::RT * (D + 2) * sizeof(float) > workspace_bytes) return NOISE_ERR_WORKSPACE;
   kernel<<<p.grid, S::NT, smem, s>>>(p);
   if (cudaGetLastError() != cudaSuccess) return NOISE_ERR_CUDA;
+  // parts an item may have: with few, a thread goes through them all; with many (a few long rows over the whole GPU) 16
+  // threads share them
+  const int items = p.seqs * p.heads * p.tiles, shares = p.grid / items >= 8 ? 16 : p.grid / items >= 3 ? 4 : 1;
+  const int groups = S::RT * D / 4;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.seqs * p.heads * p.tiles);
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = dim3(items, (groups * shares + JOIN_NT - 1) / JOIN_NT);
+  cfg.blockDim = dim3(JOIN_NT);
   cfg.dynamicSmemBytes = (2 * p.seqs + 1) * 4;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -959,7 +986,7 @@ int run(Params& p, size_t workspace_bytes, cudaStream_t s) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, join_kernel, static_cast<const Params>(p), static_cast<int>(S::RT), D) == cudaSuccess
+  return cudaLaunchKernelEx(&cfg, join_kernel, static_cast<const Params>(p), static_cast<int>(S::RT), D, shares) == cudaSuccess
              ? NOISE_OK
              : NOISE_ERR_CUDA;
 }
