@@ -10,10 +10,12 @@
 // Without q the drafts were picked, not drawn: q is 1 at the child's token. At temperature 0 a child is accepted if
 // its token is the largest logit's, and that is the next token (the lowest of equals).
 //
-// Only the rows that the walk visits are read, once each. A cluster of CTAs takes one sequence, each CTA a slice of the
+// Only the rows that the walk visits are read, and those of first children, which it is likely to visit next, are asked
+// into the L2 while their parents are judged. A cluster of CTAs takes one sequence, each CTA a slice of the
 // vocabulary in shared memory; a node is one pass with a running maximum and sum, a rejection one more over the slice.
-// What the children's tests need of their own tokens is read by one warp beside the row, so a test costs no pass. All
-// CTAs of a cluster combine the same parts in the same order, so they take the same turns. Sums are in fp32.
+// What the children's tests need of their own tokens is read before the walk and follows r on its own, so a test costs no
+// pass. All CTAs of a cluster combine the same parts in the same order, so they take the same turns.
+// Sums are in fp32.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -28,7 +30,8 @@ namespace cg = cooperative_groups;
 namespace noise {
 namespace verify {
 
-constexpr int NT = 1024, WARPS = NT / 32, MAX_NODES = 64, MAX_CTAS = 8, MAX_SLICE = 49152;
+constexpr int NT = 512, WARPS = NT / 32, MAX_NODES = 64, MAX_CTAS = 8, MAX_SLICE = 49152;
+constexpr int BATCH = 8;  // values a thread has on their way at once
 
 struct Params {
   const void* logits;
@@ -40,189 +43,266 @@ struct Params {
   const float* u;
   const float* race;  // [seqs, vocab]
   int seqs, nodes, vocab, slice;
-  float temperature, softcap;
+  bool greedy;
+  float softcap, inv_cap, unit;  // 1 / softcap; log2 e / temperature (greedy: 1)
   int* count;
   int* path;
   int64_t* token;
 };
 
-struct Pair {
-  float a, b;
+// Floats as whole numbers of the same order (NaN above all).
+__device__ __forceinline__ uint32_t ordered(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float unordered(uint32_t u) {
+  return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+struct Best {  // the largest value (as ordered) and, of equals, the lowest index; none: index -1
+  uint32_t key;
+  int index;
 };
 
-// (maximum, sum of exp(x - maximum)) of two parts.
-__device__ __forceinline__ Pair soft_join(Pair x, Pair y) {
-  const float m = fmaxf(x.a, y.a);
-  if (m == -INFINITY) return {m, x.b + y.b};  // (NaN sums stay)
-  return {m, x.b * expf(x.a - m) + y.b * expf(y.a - m)};
-}
+// What a cluster's threads reduce through. Two buffers in turn: whoever writes one again has passed a barrier after
+// everyone's reads of it.
+struct Scratch {
+  uint2 warps[2][WARPS];
+  uint2 ctas[2][MAX_CTAS];
+};
 
-// The larger value, the lower index of equals. a: value, b: index as an int's bits.
-__device__ __forceinline__ Pair best_join(Pair x, Pair y) {
-  const bool other = y.a > x.a || (y.a == x.a && __float_as_int(y.b) < __float_as_int(x.b));
-  return other ? y : x;
-}
+struct Group {
+  Scratch& s;
+  int turn = 0, cturn = 0;
 
-__device__ __forceinline__ Pair sum_join(Pair x, Pair y) { return {x.a + y.a, 0.f}; }
-
-// One value from all threads of the cluster; the parts of the warps and of the CTAs are combined in their order.
-template <typename F>
-__device__ __forceinline__ Pair reduce(Pair v, F join, Pair* warps, Pair (*ctas)[MAX_CTAS], int& turn) {
-  cg::cluster_group cluster = cg::this_cluster();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, size = cluster.num_blocks();
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1)  // butterfly: lower lanes first, alike in every lane
-  {
-    const Pair w = {__shfl_xor_sync(0xffffffffu, v.a, o), __shfl_xor_sync(0xffffffffu, v.b, o)};
-    v = lane & o ? join(w, v) : join(v, w);
+  // Of every thread's largest value top and sum of 2^(x - top): the same of the cluster's.
+  __device__ __forceinline__ void soft(float& top, float& total) {
+    warp_soft(top, total);
+    const uint2 w = block(make_uint2(ordered(top), __float_as_uint(total)));
+    top = unordered(w.x ? w.x : ordered(-INFINITY)), total = __uint_as_float(w.y);
+    warp_soft(top, total);
+    if (const uint2* all = cluster(make_uint2(__float_as_uint(top), __float_as_uint(total)))) {
+      const int lane = threadIdx.x & 31, ctas = cg::this_cluster().num_blocks();
+      top = lane < ctas ? __uint_as_float(all[lane].x) : -INFINITY;
+      total = lane < ctas ? __uint_as_float(all[lane].y) : 0.f;
+      warp_soft(top, total);
+    }
   }
-  __syncthreads();  // the last turn's parts were read
-  if (lane == 0) warps[warp] = v;
-  __syncthreads();
-  v = warps[lane];
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const Pair w = {__shfl_xor_sync(0xffffffffu, v.a, o), __shfl_xor_sync(0xffffffffu, v.b, o)};
-    v = lane & o ? join(w, v) : join(v, w);
+  __device__ __forceinline__ float sum_of(float v) {  // of the cluster, in the same order everywhere
+    v = warp_sum(warp_sum(v, true), false);
+    if (const uint2* all = cluster(make_uint2(__float_as_uint(v), 0))) {
+      const int lane = threadIdx.x & 31;
+      v = lane < static_cast<int>(cg::this_cluster().num_blocks()) ? __uint_as_float(all[lane].x) : 0.f;
+      v = warp_sum(v, false);
+    }
+    return v;
   }
-  if (size == 1) return v;
-  if (static_cast<int>(threadIdx.x) < size) cluster.map_shared_rank(&ctas[turn][0], threadIdx.x)[cluster.block_rank()] = v;
-  cluster.sync();
-  v = ctas[turn][0];
-  for (int i = 1; i < size; ++i) v = join(v, ctas[turn][i]);
-  turn ^= 1;
-  return v;
+  __device__ __forceinline__ Best best_of(Best b) {  // of the cluster
+    b = warp_best(b);
+    const uint2 w = block(make_uint2(b.key, b.index + 1));
+    b = warp_best({w.x, static_cast<int>(w.y) - 1});
+    const uint2* all = cluster(make_uint2(b.key, b.index + 1));
+    if (!all) return b;
+    const int lane = threadIdx.x & 31;
+    const uint2 c = lane < static_cast<int>(cg::this_cluster().num_blocks()) ? all[lane] : make_uint2(0, 0);
+    return warp_best({c.x, static_cast<int>(c.y) - 1});
+  }
+
+ private:
+  // v of every CTA of the cluster, or null where there is one
+  __device__ __forceinline__ const uint2* cluster(uint2 v) {
+    cg::cluster_group c = cg::this_cluster();
+    if (c.num_blocks() == 1) return nullptr;
+    uint2* mine = s.ctas[cturn];
+    if (threadIdx.x < c.num_blocks()) c.map_shared_rank(mine, threadIdx.x)[c.block_rank()] = v;
+    c.sync();
+    cturn ^= 1;
+    return mine;
+  }
+  __device__ __forceinline__ float warp_sum(float v, bool hand_on) {  // hand_on: lane i gets warp i's sum
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return hand_on ? __uint_as_float(block(make_uint2(__float_as_uint(v), 0)).x) : v;
+  }
+  __device__ __forceinline__ void warp_soft(float& top, float& total) {
+    const float m = unordered(__reduce_max_sync(0xffffffffu, ordered(top)));
+    total = top == -INFINITY ? 0.f : total * ex2(top - m);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    top = m;
+  }
+  __device__ __forceinline__ uint2 block(uint2 v) {  // lane i gets warp i's v (zeros past the last)
+    if ((threadIdx.x & 31) == 0) s.warps[turn][threadIdx.x >> 5] = v;
+    __syncthreads();
+    const int lane = threadIdx.x & 31;
+    const uint2 r = lane < WARPS ? s.warps[turn][lane] : make_uint2(0, 0);
+    turn ^= 1;
+    return r;
+  }
+  __device__ __forceinline__ Best warp_best(Best b) {
+    const uint32_t key = __reduce_max_sync(0xffffffffu, b.index >= 0 ? b.key : 0u);
+    const uint32_t last = b.index >= 0 && b.key == key ? 0x7fffffffu - b.index : 0u;
+    const uint32_t low = __reduce_max_sync(0xffffffffu, last);
+    return {key, low ? static_cast<int>(0x7fffffffu - low) : -1};
+  }
+};
+
+// A logit in powers of two (greedy: as it is, softcapped).
+__device__ __forceinline__ float scaled(const Params& p, float z) {
+  if (p.softcap > 0.f) z = p.softcap * tanhf(z * p.inv_cap);
+  return z * p.unit;
 }
+
+// n values from p on asked into the L2, a line a thread.
+template <typename T>
+__device__ __forceinline__ void prefetch(const T* p, int n, int tid) {
+  const char* from = reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(p) & ~static_cast<uintptr_t>(127));
+  for (int64_t o = tid * 128ll; from + o < reinterpret_cast<const char*>(p + n); o += NT * 128ll)
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(from + o));
+}
+
+struct Running {  // a thread's best so far; its indexes come in rising order
+  float x = -INFINITY;
+  int index = -1;
+  __device__ __forceinline__ void take(float v, int i) {
+    if (v > x || (index < 0 && v == v)) x = v, index = i;
+  }
+  __device__ __forceinline__ Best best() const { return {ordered(x + 0.f), index}; }  // (-0 as 0)
+};
 
 template <typename T>
-__device__ __forceinline__ float logit(const Params& p, const T* row, int64_t v, bool greedy) {
-  float z = static_cast<float>(row[v]);
-  if (p.softcap > 0.f) z = p.softcap * tanhf(z / p.softcap);
-  return greedy ? z : z / p.temperature;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(NT) verify_kernel(const Params p) {
-  extern __shared__ float left[];  // the slice of r: exp(z - top) before the first rejection
-  __shared__ Pair warps[WARPS];
-  __shared__ Pair ctas[2][MAX_CTAS];
-  __shared__ int parents[MAX_NODES];
-  __shared__ int kids[MAX_NODES];
-  __shared__ float kid_logit[MAX_NODES], kid_u[MAX_NODES], kid_q[MAX_NODES];
-  __shared__ int64_t kid_token[MAX_NODES];
-  __shared__ int kid_count;
+__global__ void __launch_bounds__(NT, 2) verify_kernel(const Params p) {
+  extern __shared__ float left[];  // the slice: logits, from the first rejection on r
+  __shared__ Scratch scratch;
+  __shared__ int parents[MAX_NODES], tokens[MAX_NODES], first_kid[MAX_NODES], later_kid[MAX_NODES], sibling[MAX_NODES];
+  __shared__ float u[MAX_NODES], node_r[MAX_NODES], node_q[MAX_NODES];  // x's logit, then r(x); q(x), at a node's parent
   cg::cluster_group cluster = cg::this_cluster();
-  const auto everyone = [&] {  // all threads of the cluster
-    if (cluster.num_blocks() > 1) cluster.sync();
-    else __syncthreads();
-  };
   const int rank = cluster.block_rank(), seq = blockIdx.x / cluster.num_blocks(), tid = threadIdx.x;
   const int v0 = rank * p.slice, n = min(p.slice, p.vocab - v0);  // n < 1: an empty slice
-  const bool greedy = p.temperature == 0.f;
-  const int64_t* tokens = p.tokens + static_cast<int64_t>(seq) * p.nodes;
-  if (tid < p.nodes) parents[tid] = p.parents[seq * p.nodes + tid];
-  everyone();  // the cluster's other CTAs have started too
-  int at = 0, count = 0, turn = 0;
-  Pair best = {-INFINITY, 0.f};
+  const bool greedy = p.greedy;
+  const T* const logits = static_cast<const T*>(p.logits) + seq * p.seq_stride;
+  const float* const all_probs = p.probs ? p.probs + seq * p.probs_seq : nullptr;
+  const float* const race = greedy ? nullptr : p.race + static_cast<int64_t>(seq) * p.vocab + v0;
+  prefetch(logits + v0, n, tid);
+  if (!greedy) prefetch(race, n, tid);
+  if (tid < MAX_NODES) {  // two warps
+    const bool node = tid < p.nodes;
+    const int up = node ? p.parents[seq * p.nodes + tid] : -1;
+    const int64_t x = node ? p.tokens[static_cast<int64_t>(seq) * p.nodes + tid] : -1;
+    const bool kid = node && up >= 0 && up < tid, real = kid && x >= 0 && x < p.vocab;
+    parents[tid] = kid ? up : -1;
+    tokens[tid] = real ? static_cast<int>(x) : -1;  // a token that is none is never accepted
+    u[tid] = node && p.u ? p.u[seq * p.nodes + tid] : 0.f;
+    node_r[tid] = real ? scaled(p, static_cast<float>(logits[up * p.node_stride + x])) : -INFINITY;
+    node_q[tid] = real && all_probs ? all_probs[up * p.probs_node + x] : 1.f;
+    first_kid[tid] = later_kid[tid] = MAX_NODES;
+    // siblings among the warp's 32 nodes
+    const unsigned same = __match_any_sync(0xffffffffu, kid ? up : -1 - tid), after = same & ~((2u << (tid & 31)) - 1);
+    sibling[tid] = after ? (tid & 32) + __ffs(after) - 1 : MAX_NODES;
+    asm volatile("bar.sync 1, 64;" ::: "memory");  // of the two warps: the lists are cleared
+    if (kid && __ffs(same) - 1 == (tid & 31)) (tid < 32 ? first_kid : later_kid)[up] = tid;
+    asm volatile("bar.sync 1, 64;" ::: "memory");
+    if (kid && tid < 32 && !after) sibling[tid] = later_kid[up];  // goes on among the second 32
+    if (first_kid[tid] == MAX_NODES) first_kid[tid] = later_kid[tid];
+  }
+  if (cluster.num_blocks() > 1) cluster.sync();  // the other CTAs have started too
+  else __syncthreads();
+  Group group{scratch};
+  int at = 0, count = 0;
+  Best best = {0, -1};
   int* path = p.path + seq * p.nodes;
   if (rank == 0 && tid < p.nodes) path[tid] = tid == 0 ? 0 : -1;
-  while (true) {
-    const T* row = static_cast<const T*>(p.logits) + seq * p.seq_stride + at * p.node_stride;
-    const float* probs = p.probs ? p.probs + seq * p.probs_seq + at * p.probs_node : nullptr;
-    // the children, in their order, and what their tests read
-    if (tid < 32) {
-      int found = 0;
+  // values i = tid, tid + NT, ... of the slice, BATCH at a time: f(i, value) after all of a batch's get(i)
+  const auto each = [&](auto get, auto f) {
+#pragma unroll 1
+    for (int i0 = tid; i0 < n; i0 += BATCH * NT) {
+      float x[BATCH];
 #pragma unroll
-      for (int i = 0; i < MAX_NODES; i += 32) {
-        const int c = i + tid;
-        const bool is = c < p.nodes && c > at && parents[c] == at;
-        const unsigned all = __ballot_sync(0xffffffffu, is);
-        if (is) {
-          const int k = found + __popc(all & ((1u << tid) - 1));
-          const int64_t x = tokens[c];
-          const bool real = x >= 0 && x < p.vocab;  // a token that is none is never accepted
-          kids[k] = c;
-          kid_token[k] = real ? x : -1;
-          kid_u[k] = p.u ? p.u[seq * p.nodes + c] : 0.f;
-          kid_q[k] = real && probs ? probs[x] : 1.f;
-          kid_logit[k] = real ? logit(p, row, x, greedy) : -INFINITY;
-        }
-        found += __popc(all);
-      }
-      if (tid == 0) kid_count = found;
+      for (int j = 0; j < BATCH; ++j) x[j] = i0 + j * NT < n ? get(i0 + j * NT) : 0.f;
+#pragma unroll
+      for (int j = 0; j < BATCH; ++j)
+        if (i0 + j * NT < n) f(i0 + j * NT, x[j]);
     }
-    int next = -1;
+  };
+  while (true) {
+    const T* const row = logits + at * p.node_stride + v0;
+    const float* const probs = all_probs ? all_probs + at * p.probs_node + v0 : nullptr;
+    const int first = first_kid[at];
+    int next = MAX_NODES;
+    if (first < MAX_NODES) {  // what is likely to be read next
+      prefetch(logits + first * p.node_stride + v0, n, tid);
+      if (probs && !greedy) prefetch(probs, n, tid);
+    }
     if (greedy) {
-      Pair b = {-INFINITY, __int_as_float(p.vocab)};
-      for (int i = tid; i < n; i += NT) {
-        const Pair x = {logit(p, row, v0 + i, true), __int_as_float(v0 + i)};
-        b = best_join(b, x);
-      }
-      best = reduce(b, best_join, warps, ctas, turn);
-      for (int k = 0; k < kid_count && next < 0; ++k)
-        if (kid_token[k] == __float_as_int(best.b)) next = kids[k];
+      Running b;
+      each([&](int i) { return static_cast<float>(row[i]); }, [&](int i, float z) { b.take(scaled(p, z), v0 + i); });
+      best = group.best_of(b.best());
+      for (next = first; next < MAX_NODES && (tokens[next] < 0 || tokens[next] != best.index);) next = sibling[next];
     } else {
-      Pair mine = {-INFINITY, 0.f};
-      for (int i = tid; i < n; i += NT) {
-        const float z = logit(p, row, v0 + i, false);
-        left[i] = z;
-        mine.a = fmaxf(mine.a, z);
-      }
-      if (mine.a != -INFINITY)
-        for (int i = tid; i < n; i += NT) mine.b += expf(left[i] - mine.a);
-      const Pair all = reduce(mine, soft_join, warps, ctas, turn);
-      const float top = all.a, total = all.b;
-      for (int i = tid; i < n; i += NT) left[i] = expf(left[i] - top) / total;
+      float top = -INFINITY, total = 0.f;
+      each([&](int i) { return static_cast<float>(row[i]); },
+           [&](int i, float z) {
+             z = scaled(p, z);
+             left[i] = z;
+             top = fmaxf(top, z);
+           });
+      if (top != -INFINITY)
+        for (int i = tid; i < n; i += NT) total += ex2(left[i] - top);
+      group.soft(top, total);
+      const float inv = 1.f / total;
       float mass = 1.f;
-      bool first = true;
-      for (int k = 0; k < kid_count; ++k) {
-        const int64_t x = kid_token[k];
-        // r(x): p(x), less q(x) once for each sibling before
-        float value = expf(kid_logit[k] - top) / total;
-        if (!first) {  // the owner's slice has it
-          value = 0.f;
-          const int owner = x >= 0 ? static_cast<int>(x / p.slice) : 0;
-          if (x >= 0) value = cluster.map_shared_rank(left, owner)[x - static_cast<int64_t>(owner) * p.slice];
-        }
-        if (x >= 0 && kid_u[k] * mass * kid_q[k] < value) {
-          next = kids[k];
-          break;
-        }
-        if (!first) everyone();  // everyone has read the value
-        const float div = mass > 0.f ? mass : 1.f;
-        Pair s = {0.f, 0.f};
-        for (int i = tid; i < n; i += NT) {
-          const float q = probs ? probs[v0 + i] : v0 + i == x ? 1.f : 0.f;
-          const float r = fmaxf(left[i] / div - q, 0.f);
+      bool fresh = true;  // no rejection yet: the slice holds logits, node_r the children's
+      for (next = first; next < MAX_NODES; next = sibling[next]) {
+        const int x = tokens[next];
+        const float value = fresh ? ex2(node_r[next] - top) * inv : node_r[next];
+        if (x >= 0 && u[next] * mass * node_q[next] < value) break;
+        const float div = mass > 0.f ? 1.f / mass : 1.f;
+        float sum = 0.f;
+        const auto less = [&](int i, float q) {
+          const float r = fmaxf((fresh ? ex2(left[i] - top) * inv : left[i]) * div - q, 0.f);
           left[i] = r;
-          s.a += r;
+          sum += r;
+        };
+        if (probs) each([&](int i) { return probs[i]; }, less);
+        else each([&](int i) { return v0 + i == x ? 1.f : 0.f; }, less);
+        mass = group.sum_of(sum);
+        // the same for the siblings' own tokens; everyone has passed a barrier since reading them
+        if (tid < MAX_NODES && parents[tid] == at) {
+          const float q = probs ? node_q[tid] : tokens[tid] == x ? 1.f : 0.f;
+          node_r[tid] = fmaxf((fresh ? ex2(node_r[tid] - top) * inv : node_r[tid]) * div - q, 0.f);
         }
-        mass = reduce(s, sum_join, warps, ctas, turn).a;
-        first = false;
+        __syncthreads();
+        fresh = false;
       }
-      if (next < 0) {
-        const float* race = p.race + static_cast<int64_t>(seq) * p.vocab;
-        Pair b = {-INFINITY, __int_as_float(p.vocab)};
-        for (int i = tid; i < n; i += NT) {
-          // nothing left of r (the drafts' own distribution): p
-          const float r = mass > 0.f ? left[i] : expf(logit(p, row, v0 + i, false) - top) / total;
-          const Pair x = {r / race[v0 + i], __int_as_float(v0 + i)};
-          b = best_join(b, x);
-        }
-        best = reduce(b, best_join, warps, ctas, turn);
+      if (next == MAX_NODES) {
+        Running b;
+        each([&](int i) { return race[i]; },
+             [&](int i, float e) {
+               // nothing left of r (the drafts' own distribution): p
+               const float r = fresh ? ex2(left[i] - top) * inv
+                               : mass > 0.f ? left[i]
+                                            : ex2(scaled(p, static_cast<float>(row[i])) - top) * inv;
+               b.take(__fdividef(r, e), v0 + i);
+             });
+        best = group.best_of(b.best());
       }
     }
-    everyone();  // the children's list and the slices were read
-    if (next < 0) break;
+    if (next == MAX_NODES) break;
     at = next;
     ++count;
     if (rank == 0 && tid == 0) path[count] = at;
   }
   if (rank == 0 && tid == 0) {
     p.count[seq] = count;
-    const int v = __float_as_int(best.b);
-    p.token[seq] = v < p.vocab ? v : -1;  // (no logit above -inf)
+    p.token[seq] = best.index;  // (-1: no logit is a number)
   }
+  if (cluster.num_blocks() > 1) cluster.sync();  // no CTA leaves while another may write to it
 }
 
 // mask: a node's ancestors and itself; depth: its distance from the root. A parent that is not -1 or an earlier node that is
@@ -275,7 +355,7 @@ int run(const Params& p, int ctas, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.seqs * ctas);
   cfg.blockDim = dim3(NT);
-  cfg.dynamicSmemBytes = p.temperature == 0.f ? 0 : p.slice * 4;
+  cfg.dynamicSmemBytes = p.greedy ? 0 : p.slice * 4;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -314,11 +394,13 @@ int noise_verify_tree(const void* logits, int logits_dtype, int64_t seq_stride, 
   if (seqs == 0) return NOISE_OK;
   if (!logits || !tokens || !parents || !count || !path || !token || (temperature > 0.f && (!u || !race)))
     return NOISE_ERR_ARGUMENT;
-  // a cluster of the fewest CTAs with at most 8 values a thread, 8 CTAs at most
+  // a cluster of the fewest CTAs with at most one batch a thread, 8 CTAs at most
   int ctas = 1;
-  while (ctas < MAX_CTAS && (vocab + ctas - 1) / ctas > 8 * NT) ctas *= 2;
+  while (ctas < MAX_CTAS && (vocab + ctas - 1) / ctas > BATCH * NT) ctas *= 2;
   Params p = {logits, seq_stride, node_stride, probs, probs_seq_stride, probs_node_stride, tokens, parents, u, race,
-              seqs, nodes, vocab, (vocab + ctas - 1) / ctas, temperature, softcap, count, path, token};
+              seqs, nodes, vocab, (vocab + ctas - 1) / ctas, temperature == 0.f, softcap,
+              softcap > 0.f ? 1.f / softcap : 0.f, temperature == 0.f ? 1.f : 1.4426950408889634f / temperature, count,
+              path, token};
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   return logits_dtype == NOISE_DTYPE_F32 ? run<float>(p, ctas, s) : run<__nv_bfloat16>(p, ctas, s);
 }
