@@ -26,6 +26,7 @@
 #include <cuda_runtime.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "kv.cuh"
 #include "ptx.cuh"
@@ -104,6 +105,10 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 }
 __device__ __forceinline__ float low_f(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float high_f(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+
+#ifndef WIDE_FROM
+#define WIDE_FROM 32
+#endif
 
 // ---- the line of units ------------------------------------------------------------------------------------------
 
@@ -934,18 +939,58 @@ __global__ void __launch_bounds__(JOIN_NT) join_kernel(const Params p, int rt, i
       none ? make_uint2(0, 0) : make_uint2(pack_bf16(sum.o.x * f, sum.o.y * f), pack_bf16(sum.o.z * f, sum.o.w * f));
 }
 
+}  // namespace tree
+}  // namespace noise
+
+#include "tree_wide.cuh"
+
+namespace noise {
+namespace tree {
+
 // ---- host -------------------------------------------------------------------------------------------------------
 
-constexpr int MAX_GRID = 148 * 8;
+// CTAs of a row tile at most (more would not be resident at once): what the workspace is made for.
+constexpr int max_grid(int tile) { return 148 * (tile <= 8 ? 8 : tile <= 16 ? 4 : tile <= 32 ? 3 : 2); }
 
-// The row tile of a call: the least of 8, 16, 32 and 64 rows that holds all, or 64.
-inline int tile_rows(int rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+constexpr int MAX_WIDE_GRID = 148;
+
+// Whether a call goes to the tcgen05 kernel: its tile of 128 rows is worth filling from 33 rows on; a bf16 cache has no
+// codes to bring to shared memory and stays; the line's lengths have to fit beside the tiles.
+inline bool wide_rows(int kind, int rows, int seqs) {
+  return kind != NOISE_KV_BF16 && rows > WIDE_FROM && seqs <= 2048;
+}
+
+// The row tile of a call: the least of 8, 16, 32 and 64 rows that holds all, or 64; W_ROWS on tcgen05.
+inline int tile_rows(int kind, int rows, int seqs) {
+  return wide_rows(kind, rows, seqs) ? W_ROWS : rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+}
 
 inline int sm_count() {
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return 0;
   return n;
+}
+
+// Joins the items' parts after the kernel that makes them.
+inline int launch_join(const Params& p, int rt, int dim, cudaStream_t s) {
+  // parts an item may have: with few, a thread goes through them all; with many (a few long rows over the whole GPU) 16
+  // threads share them
+  const int items = p.seqs * p.heads * p.tiles, shares = p.grid / items >= 8 ? 16 : p.grid / items >= 3 ? 4 : 1;
+  const int groups = rt * dim / 4;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(items, (groups * shares + JOIN_NT - 1) / JOIN_NT);
+  cfg.blockDim = dim3(JOIN_NT);
+  cfg.dynamicSmemBytes = (2 * p.seqs + 1) * 4;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, join_kernel, p, rt, dim, shares) == cudaSuccess
+             ? NOISE_OK
+             : NOISE_ERR_CUDA;
 }
 
 template <int KIND, int D, int NTL, int RW>
@@ -962,7 +1007,7 @@ int run(Params& p, size_t workspace_bytes, cudaStream_t s) {
   const int sms = sm_count();
   if (sms < 1) return NOISE_ERR_CUDA;
   p.grid = sms * per_sm;
-  if (p.grid > MAX_GRID) p.grid = MAX_GRID;
+  if (p.grid > max_grid(S::RT)) p.grid = max_grid(S::RT);
   const int64_t room = static_cast<int64_t>(p.width) << p.page_shift;
   p.unit_shift = S::G == 2 ? 7 : 6;
   static_assert(16 * KW == 64, "a unit is KW steps of 16 G keys");
@@ -972,28 +1017,35 @@ int run(Params& p, size_t workspace_bytes, cudaStream_t s) {
   if (static_cast<size_t>(2) * p.grid * S::RT * (D + 2) * sizeof(float) > workspace_bytes) return NOISE_ERR_WORKSPACE;
   kernel<<<p.grid, S::NT, smem, s>>>(p);
   if (cudaGetLastError() != cudaSuccess) return NOISE_ERR_CUDA;
-  // parts an item may have: with few, a thread goes through them all; with many (a few long rows over the whole GPU) 16
-  // threads share them
-  const int items = p.seqs * p.heads * p.tiles, shares = p.grid / items >= 8 ? 16 : p.grid / items >= 3 ? 4 : 1;
-  const int groups = S::RT * D / 4;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(items, (groups * shares + JOIN_NT - 1) / JOIN_NT);
-  cfg.blockDim = dim3(JOIN_NT);
-  cfg.dynamicSmemBytes = (2 * p.seqs + 1) * 4;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, join_kernel, static_cast<const Params>(p), static_cast<int>(S::RT), D, shares) == cudaSuccess
-             ? NOISE_OK
-             : NOISE_ERR_CUDA;
+  return launch_join(p, S::RT, D, s);
+}
+
+template <int KIND, int D>
+int run_wide(Params& p, size_t workspace_bytes, cudaStream_t s) {
+  const auto kernel = wide_kernel<KIND, D>;
+  const int smem = 1024 + Wide<D>::SMEM + (2 * p.seqs + 1 + p.nodes) * 4;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return NOISE_ERR_CUDA;
+  const int sms = sm_count();
+  if (sms < 1) return NOISE_ERR_CUDA;
+  const int64_t room = static_cast<int64_t>(p.width) << p.page_shift;
+  p.unit_shift = 7;
+  p.tiles = (p.nodes * p.group + W_ROWS - 1) / W_ROWS;
+  const int64_t units = static_cast<int64_t>(p.seqs) * p.heads * p.tiles * (HEAD + 1 + (room >> p.unit_shift));
+  if (units > 0x7fffffff) return NOISE_ERR_SHAPE;
+  p.grid = sms < MAX_WIDE_GRID ? sms : MAX_WIDE_GRID;
+  if (units / LEAST < p.grid) p.grid = units < 2 * LEAST ? 1 : static_cast<int>(units / LEAST);
+  if (static_cast<size_t>(2) * p.grid * W_ROWS * (D + 2) * sizeof(float) > workspace_bytes) return NOISE_ERR_WORKSPACE;
+  kernel<<<p.grid, W_NT, smem, s>>>(p);
+  if (cudaGetLastError() != cudaSuccess) return NOISE_ERR_CUDA;
+  return launch_join(p, W_ROWS, D, s);
 }
 
 template <int KIND, int D>
 int by_rows(Params& p, size_t bytes, cudaStream_t s) {
   const int rows = p.nodes * p.group;
+  if constexpr (KIND != NOISE_KV_BF16) {
+    if (wide_rows(KIND, rows, p.seqs)) return run_wide<KIND, D>(p, bytes, s);
+  }
   if (rows <= 8) return run<KIND, D, 1, 1>(p, bytes, s);
   if (rows <= 16) return run<KIND, D, 2, 1>(p, bytes, s);
   if (rows <= 32) return run<KIND, D, 4, 1>(p, bytes, s);
@@ -1012,8 +1064,14 @@ extern "C" {
 
 size_t noise_tree_attention_workspace_bytes(int seqs, int nodes, int q_heads, int heads, int dim) {
   if (seqs < 1 || nodes < 1 || heads < 1 || q_heads < heads || q_heads % heads || (dim != 64 && dim != 128)) return 0;
-  return static_cast<size_t>(2) * noise::tree::MAX_GRID * noise::tree::tile_rows(nodes * (q_heads / heads)) *
-         (dim + 2) * sizeof(float);
+  using namespace noise::tree;
+  size_t rows = 0;  // of either kernel: the cache's kind is not known here
+  for (const int kind : {NOISE_KV_BF16, NOISE_KV_INT8}) {
+    const int tile = tile_rows(kind, nodes * (q_heads / heads), seqs);
+    const size_t need = static_cast<size_t>(2) * (tile == W_ROWS ? MAX_WIDE_GRID : max_grid(tile)) * tile;
+    if (need > rows) rows = need;
+  }
+  return rows * (dim + 2) * sizeof(float);
 }
 
 int noise_tree_attention(const noise_kv_cache_t* cache, int layer, const void* q, int64_t q_seq_stride,
@@ -1046,7 +1104,7 @@ int noise_tree_attention(const noise_kv_cache_t* cache, int layer, const void* q
   for (int64_t stride : {q_seq_stride, q_node_stride, q_head_stride, k_seq_stride, k_node_stride, k_head_stride,
                          v_seq_stride, v_node_stride, v_head_stride})
     if (stride % 8) return NOISE_ERR_ALIGN;
-  const int group = q_heads / cache->heads, tile = tile_rows(nodes * group);
+  const int group = q_heads / cache->heads, tile = tile_rows(cache->kind, nodes * group, seqs);
   const int tiles = (nodes * group + tile - 1) / tile;
   if (static_cast<int64_t>(seqs) * cache->heads * tiles > 0x7fffffff) return NOISE_ERR_SHAPE;
   if (!workspace) return NOISE_ERR_WORKSPACE;

@@ -1,0 +1,578 @@
+// Tree attention over an 8-bit cache with many query rows a key head, on tcgen05 (included by tree_attention.cu, whose
+// line of units, parts and join it shares).
+//
+// With more than 32 rows the products bound the call, not the cache's bytes: 4 D operations a row and key, on a dense
+// tile of 128 rows. A CTA takes up to 256 rows of one key head (groups A and B of 128) and walks 128 keys at a time:
+//   warps 0..3, 4..7  softmax of groups A and B, one row a thread: S from tensor memory, P = 2^(x - m) V's scale as fp16
+//                     pairs back into the first half of S's columns (the next product's A operand);
+//   warps 8..11       codes to fp16 in shared memory, in the swizzled rows that tcgen05.mma reads: K by keys, V by
+//                     dimensions with the keys along the row (its four-token quads are 8 bytes of such a row); the codes of
+//                     the next tile are on their way in registers meanwhile; each key's scales beside them;
+//   warp 12           tensor memory (512 columns: S / P and O of both groups) and the MMAs: S_g = Q_g K^T and
+//                     O_g += P_g V, group B's while group A's softmax runs.
+// A row's maximum moves when a score passes it by 2^8, and O in tensor memory is rescaled then by its own warps: S_g of
+// a tile is only issued after P_g V of the last one, so O is still. The tree's own keys are the first tile, brought to
+// fp16 under a power of two per key like the codes.
+#pragma once
+
+#include "kv.cuh"
+#include "ptx.cuh"
+
+namespace noise {
+namespace tree {
+
+constexpr int W_KEYS = 128, W_ROWS = 256, W_NT = 13 * 32;
+
+__host__ __device__ constexpr uint32_t idesc_f16(int M, int N) {  // fp16 A and B, fp32 D
+  return (1u << 4) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+template <int D>
+struct Wide {
+  static constexpr int Q_BYTES = 128 * D * 2;         // of a group
+  static constexpr int K_BYTES = W_KEYS * D * 2;      // of a stage; V's are as many
+  static constexpr int K_AT = 2 * Q_BYTES;            // [stage] K, V
+  static constexpr int SCALES_AT = K_AT + 4 * K_BYTES;  // [stage] kf, vf: 128 floats each
+  static constexpr int BAR_AT = SCALES_AT + 2 * 2 * W_KEYS * 4;
+  static constexpr int SMEM = BAR_AT + 128;           // then the line's ints, then depths
+  static constexpr uint32_t S_COL = 0, O_COL = 256;   // S_A, S_B of 128 columns; O_A, O_B of D
+};
+
+struct TileInfo {
+  float unit;  // what O is to be multiplied by before this tile: 2^(old reference - new)
+  int nan_v;   // some key's V reads as NaN
+};
+
+template <int KIND, int D>
+__global__ void __launch_bounds__(W_NT, 1) wide_kernel(const Params p) {
+  using W = Wide<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* const bar = reinterpret_cast<uint64_t*>(smem + W::BAR_AT);
+  uint64_t *const full = bar, *const empty = bar + 2, *const s_full = bar + 4, *const p_full = bar + 6, *const o_full = bar + 8,
+           *const told = bar + 9;
+  uint32_t* const tmem_at = reinterpret_cast<uint32_t*>(bar + 10);
+  int* const before = reinterpret_cast<int*>(smem + W::SMEM);
+  int* const lens = before + p.seqs + 1;
+  int* const depths = lens + p.seqs;
+  __shared__ TileInfo info[2];
+  __shared__ int gave_up, lost[2], last_ref, tops[2][4];  // lost: a page of this (or the next) item out of range
+  __shared__ unsigned special[2];  // nodes whose V is not finite
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  cudaTriggerProgrammaticLaunchCompletion();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&full[i], 4);
+      mbar_init(&empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+    }
+    mbar_init(o_full, 1);
+    mbar_init(told, 4);
+    fence_barrier_init();
+    gave_up = lost[0] = lost[1] = 0;
+  }
+  if (warp == 12) {
+    tmem_alloc(tmem_at, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  line_of(p, before, lens);
+  tc_fence_after();
+  const uint32_t tmem = *tmem_at, sbase = smem_u32(smem);
+  const Spans spans(p, before);
+  const int first = spans.cut(min(static_cast<int>(blockIdx.x), spans.ctas));
+  const int last = spans.cut(min(static_cast<int>(blockIdx.x) + 1, spans.ctas));
+  const int rows = p.nodes * p.group, hr = p.heads * p.tiles;
+  int b = 0;
+  {
+    int low = 0, high = p.seqs - 1;
+    while (low < high) {
+      const int mid = (low + high + 1) >> 1;
+      if (before[mid] * hr <= first) low = mid;
+      else high = mid - 1;
+    }
+    b = low;
+  }
+  int done = 0, done_b = 0, parts = 0;  // tiles, group B's tiles and items gone through: the barriers' phases
+  for (int at = first, turn = 0; at < last; turn ^= 1) {
+    const int base = before[b] * hr, per = before[b + 1] - before[b];
+    const int item = (at - base) / per, u0 = at - base - item * per, u1 = min(per, u0 + last - at);
+    const int h = item / p.tiles, tile = item - h * p.tiles, row0 = tile * W_ROWS;
+    const int groups = rows - row0 > 128 ? 2 : 1;
+    const int len = lens[b];
+    const int unit0 = first_unit(p, len) - HEAD;
+    const int key_lo = (unit0 + max(u0, HEAD)) * W_KEYS, key_hi = min((unit0 + u1) * W_KEYS, len);
+    const bool tree = u0 == 0;
+    const int tiles = (tree ? 1 : 0) + (key_hi > key_lo ? (key_hi - key_lo + W_KEYS - 1) / W_KEYS : 0);
+    const bool whole = u0 == 0 && u1 == per;
+    if (threadIdx.x < 2) special[threadIdx.x] = 0;
+    if (threadIdx.x < p.nodes) depths[threadIdx.x] = p.depth[b * p.nodes + threadIdx.x];
+
+    if (warp < 8) {
+      // ---- a row a thread: Q as fp16 under a power of two, into K-major swizzled rows
+      const int g = warp >> 2, in = threadIdx.x & 127, r = row0 + g * 128 + in;
+      const bool real = g < groups && r < rows;
+      const int node = real ? r / p.group : 0;
+      const __nv_bfloat16* q =
+          p.q + b * p.q_seq + node * p.q_node + (h * p.group + (real ? r - node * p.group : 0)) * p.q_head;
+      const uint64_t mask = real && tree ? p.mask[b * p.nodes + node] : 0;
+      float rf = p.scale_log2;
+      if (g < groups) {
+        uint4 x[D / 8];
+        uint32_t top = 0;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          x[c] = real ? __ldg(reinterpret_cast<const uint4*>(q) + c) : make_uint4(0, 0, 0, 0);
+          for (const uint32_t w : {x[c].x, x[c].y, x[c].z, x[c].w}) top = max(top, max(w & 0x7fffu, w >> 16 & 0x7fffu));
+        }
+        int e = static_cast<int>(top >> 7);
+        e = e == 255 || e < 1 ? 127 : e < 67 ? 67 : e > 253 ? 253 : e;  // (not finite or zero: as it is)
+        const float f = kv::power(254 - e);
+        rf *= kv::power(e);
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          const uint4 y = make_uint4(pack_f16(low_f(x[c].x) * f, high_f(x[c].x) * f), pack_f16(low_f(x[c].y) * f, high_f(x[c].y) * f),
+                                     pack_f16(low_f(x[c].z) * f, high_f(x[c].z) * f), pack_f16(low_f(x[c].w) * f, high_f(x[c].w) * f));
+          *reinterpret_cast<uint4*>(smem + g * W::Q_BYTES + (c >> 3) * 16384 + in * 128 + ((c & 7) ^ (in & 7)) * 16) = y;
+        }
+        fence_proxy_async_smem();
+      }
+      __syncthreads();  // Q, depths and the cleared marks are there
+      if (threadIdx.x == 0) lost[turn ^ 1] = 0;
+      if (g < groups) {
+        const int mine = g == 0 ? done : done_b;
+        const int depth = depths[node];
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);  // this warp's 32 lanes
+        const uint32_t s_at = lanes + W::S_COL + g * 128, o_at = lanes + W::O_COL + g * D;
+        float l = 0.f, off = NONE;
+        bool ok = true;
+        for (int i = 0; i < tiles && ok; ++i) {
+          const int n = done + i, st = n & 1;
+          ok = mbar_wait_warp(&full[st], n >> 1 & 1, &gave_up) && mbar_wait_warp(&s_full[g], mine + i & 1, &gave_up);
+          if (!ok) break;
+          tc_fence_after();
+          const float4* kf = reinterpret_cast<const float4*>(smem + W::SCALES_AT + st * 2 * W_KEYS * 4);
+          const float4* vf = kf + W_KEYS / 4;
+          const bool own = tree && i == 0;
+          const int key0 = key_lo + (i - (tree ? 1 : 0)) * W_KEYS;
+          const bool edge = own || key0 + W_KEYS > len || (p.window >= 0 && key0 < len + p.nodes - p.window);
+          uint32_t see[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+          if (own) {
+            uint64_t m = mask;
+            if (p.window >= 0)
+              for (int j = 0; j < p.nodes; ++j)
+                if (depths[j] < depth - p.window) m &= ~(1ull << j);
+            if (p.nodes < 64) m &= (1ull << p.nodes) - 1;
+            see[0] = static_cast<uint32_t>(m), see[1] = static_cast<uint32_t>(m >> 32), see[2] = see[3] = 0;
+          } else if (edge) {
+            const int low = p.window < 0 ? 0 : max(0, len + depth - p.window - key0), high = len - key0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int a = min(max(low - 32 * j, 0), 32), z = min(max(high - 32 * j, 0), 32);  // keys a .. z - 1
+              const uint32_t up_to = z == 32 ? 0xffffffffu : (1u << z) - 1, from = a == 32 ? 0u : 0xffffffffu << a;
+              see[j] = up_to & from;
+            }
+          }
+          if (info[st].nan_v) {  // keys whose V reads as NaN have factor 0 in the product: their rows' sums say it
+#pragma unroll 1
+            for (int c = 0; c < W_KEYS; ++c)
+              if (reinterpret_cast<const float*>(vf)[c] != reinterpret_cast<const float*>(vf)[c] &&
+                  (see[c >> 5] >> (c & 31) & 1))
+                l = __int_as_float(0x7fc00000);
+          }
+          // Probabilities of the tile as packed pairs, their sum, and how far the largest passes the maximum.
+          uint32_t pk[W_KEYS / 2];
+          float sum, most;
+          const auto soften = [&](auto masked) {
+            sum = 0.f, most = NEG;
+            float2 sums = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              float s[32];
+              __syncwarp();
+              tmem_ld32(s_at + c * 32, s);
+              tc_wait_ld();
+              reg_fence<32>(s);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const float4 k4 = kf[c * 8 + j], v4 = vf[c * 8 + j];
+                float2 a = __fmul2_rn(make_float2(s[4 * j], s[4 * j + 1]), make_float2(k4.x, k4.y));
+                float2 z = __fmul2_rn(make_float2(s[4 * j + 2], s[4 * j + 3]), make_float2(k4.z, k4.w));
+                if constexpr (decltype(masked)::value) {
+                  if (!(see[c] >> (4 * j) & 1)) a.x = NEG;
+                  if (!(see[c] >> (4 * j + 1) & 1)) a.y = NEG;
+                  if (!(see[c] >> (4 * j + 2) & 1)) z.x = NEG;
+                  if (!(see[c] >> (4 * j + 3) & 1)) z.y = NEG;
+                }
+                a = __ffma2_rn(a, make_float2(rf, rf), make_float2(off, off));
+                z = __ffma2_rn(z, make_float2(rf, rf), make_float2(off, off));
+                most = fmaxf(fmaxf(most, fmaxf(a.x, a.y)), fmaxf(z.x, z.y));
+                a = make_float2(ex2(a.x), ex2(a.y));
+                z = make_float2(ex2(z.x), ex2(z.y));
+                sums = __fadd2_rn(sums, __fadd2_rn(a, z));
+                float2 va = make_float2(v4.x, v4.y), vz = make_float2(v4.z, v4.w);
+                if constexpr (decltype(masked)::value) {  // (a masked key's factor may be NaN)
+                  va = make_float2(va.x == va.x ? va.x : 0.f, va.y == va.y ? va.y : 0.f);
+                  vz = make_float2(vz.x == vz.x ? vz.x : 0.f, vz.y == vz.y ? vz.y : 0.f);
+                }
+                a = __fmul2_rn(a, va);
+                z = __fmul2_rn(z, vz);
+                pk[c * 16 + 2 * j] = pack_f16(a.x, a.y);
+                pk[c * 16 + 2 * j + 1] = pack_f16(z.x, z.y);
+              }
+            }
+            sum = sums.x + sums.y;
+          };
+          const bool careful = edge || info[st].nan_v;
+          if (careful) soften(std::true_type{});
+          else soften(std::false_type{});
+          const float unit = info[st].unit;
+          if (__any_sync(0xffffffffu, most > SLACK || unit != 1.f)) {
+            float x = NEG;  // the largest score, in powers of two
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              float s[32];
+              __syncwarp();
+              tmem_ld32(s_at + c * 32, s);
+              tc_wait_ld();
+              reg_fence<32>(s);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const float v = s[j] * reinterpret_cast<const float*>(kf)[c * 32 + j];
+                if (see[c] >> j & 1) x = fmaxf(x, v);
+              }
+            }
+            x *= rf;
+            float f = 1.f;
+            if (most > SLACK && x > -off) {
+              f = ex2(-off - x);
+              off = -x;
+              l *= f;
+            }
+            f *= unit;
+            __syncwarp();
+            if (i > 0) {  // O holds the tiles before
+#pragma unroll 1
+              for (int c = 0; c < D / 16; ++c) {
+                float o[16];
+                __syncwarp();
+                tmem_ld16(o_at + c * 16, o);
+                tc_wait_ld();
+                reg_fence<16>(o);
+                uint32_t w[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(o[j] * f);
+                tmem_st16(o_at + c * 16, w);
+              }
+            }
+            if (careful) soften(std::true_type{});
+            else soften(std::false_type{});
+          }
+          l += sum;
+          __syncwarp();
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_st16(s_at + c * 16, pk + c * 16);
+          tc_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[g]);
+        }
+        // ---- the item's output
+        const int slot = 2 * blockIdx.x + (at == first ? 0 : 1);
+        if (tiles > 0) ok = ok && mbar_wait_warp(o_full, parts & 1, &gave_up);
+        tc_fence_after();
+        const float to = tiles > 0 ? ex2(static_cast<float>(last_ref - 127)) : 0.f;
+        if (lost[turn] || !ok) l = __int_as_float(0x7fc00000);
+        const uint64_t odd = (mask & (static_cast<uint64_t>(special[1]) << 32 | special[0]));
+        const bool pad = depth < 0;
+        const float f = pad ? 0.f : !whole ? to : l == 0.f ? 0.f : to / l;
+        __nv_bfloat16* out =
+            p.out + ((static_cast<int64_t>(b) * p.nodes + node) * p.heads * p.group + h * p.group + r - node * p.group) * D;
+        float* po = p.partial + (static_cast<int64_t>(slot) * W_ROWS + g * 128 + in) * D;
+        float* pm = p.partial + static_cast<int64_t>(2 * p.grid) * W_ROWS * D + static_cast<int64_t>(slot) * 2 * W_ROWS + g * 128 + in;
+        if (real && !whole) {
+          pm[0] = off;
+          pm[W_ROWS] = l;
+        }
+#pragma unroll 1
+        for (int c = 0; c < D / 16; ++c) {
+          float o[16];
+          __syncwarp();
+          tmem_ld16(o_at + c * 16, o);
+          tc_wait_ld();
+          reg_fence<16>(o);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) o[j] = f == 0.f ? 0.f : o[j] * f;
+          if (odd && !pad) {  // values that are not finite were left out of the product: they reach the rows that see them
+            for (int j = 0; j < p.nodes; ++j) {
+              if (!(odd >> j & 1) || (p.window >= 0 && depths[j] < depth - p.window)) continue;
+              const __nv_bfloat16* v = p.v + b * p.v_seq + j * p.v_node + h * p.v_head + c * 16;
+#pragma unroll
+              for (int d = 0; d < 16; ++d) {
+                const float x = __bfloat162float(v[d]);
+                if (!(fabsf(x) < INFINITY)) o[d] += x;
+              }
+            }
+          }
+          if (!real) continue;
+          if (whole) {
+            uint4* w = reinterpret_cast<uint4*>(out + c * 16);
+            w[0] = make_uint4(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]), pack_bf16(o[4], o[5]), pack_bf16(o[6], o[7]));
+            w[1] = make_uint4(pack_bf16(o[8], o[9]), pack_bf16(o[10], o[11]), pack_bf16(o[12], o[13]), pack_bf16(o[14], o[15]));
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; j += 4)
+              *reinterpret_cast<float4*>(po + c * 16 + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+          }
+        }
+        tc_fence_before();
+      }
+    } else if (warp < 12) {
+      // ---- codes to fp16
+      const int t = threadIdx.x - 256, w = t >> 5;
+      constexpr int PIECES = D / 16;  // 16-byte loads a thread of K, and of V, for 128 keys
+      uint4 kc[PIECES], vc[PIECES];
+      uint32_t scales = 0;  // of key t: K's byte, V's byte
+      int ahead = 0;        // cached tiles asked for
+      const int cshift = p.page_shift - 4;
+      const int* table = p.table + static_cast<int64_t>(b) * p.width;
+      const auto fetch = [&] {
+        const int key0 = key_lo + ahead++ * W_KEYS;
+        if (key0 >= key_hi) return;
+        int page = 0;  // lane i: of keys 16 i on
+        if (lane < 8 && key0 + 16 * lane < len) {
+          page = __ldg(table + ((key0 >> 4) + lane >> cshift));
+          if (page < 0 || page >= p.c.pages) {
+            lost[turn] = 1;
+            record_error(p.c.status, NOISE_DEV_BAD_INDEX);
+            page = 0;
+          }
+        }
+        const auto cell = [&](int block) {  // of 16 keys
+          const int pg = __shfl_sync(0xffffffffu, page, block);
+          return (((p.layer_cell + pg) * p.heads + h) << p.page_shift) +
+                 ((((key0 >> 4) + block) & ((1 << cshift) - 1)) << 4);
+        };
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+          const int piece = j * 128 + t, key = piece / PIECES, c = piece % PIECES;
+          const int64_t at16 = cell(key >> 4);
+          kc[j] = make_uint4(0, 0, 0, 0);
+          if (key0 + key < len)
+            kc[j] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.c.k) + (at16 + (key & 15)) * D + c * 16));
+        }
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {  // quad lane % 16 of 64 keys, dimensions 4 x .. 4 x + 3
+          const int half = j / (PIECES / 2), quad = half * 16 + (lane & 15);
+          const int x = 2 * (w * (PIECES / 2) + j % (PIECES / 2)) + (lane >> 4);
+          const int64_t at16 = cell(quad >> 2);
+          vc[j] = make_uint4(0, 0, 0, 0);
+          const int left = len - key0 - quad * 4;
+          if (left > 0) {
+            vc[j] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.c.v) + (at16 + (quad & 3) * 4) * D + x * 16));
+            if (left < 4) {
+              const uint32_t keep = 0xffffffffu >> (32 - 8 * left);
+              vc[j].x &= keep, vc[j].y &= keep, vc[j].z &= keep, vc[j].w &= keep;
+            }
+          }
+        }
+        const int64_t at16 = cell(t >> 4);
+        scales = 1 | 1 << 8;
+        if (key0 + t < len)
+          scales = __ldg(p.c.k_scale + at16 + (t & 15)) | static_cast<uint32_t>(__ldg(p.c.v_scale + at16 + (t & 15))) << 8;
+      };
+      fetch();
+      __syncthreads();
+      bool ok = true;
+      int ref = 0;  // the largest scale byte of V so far
+      for (int i = 0; i < tiles && ok; ++i) {
+        const int n = done + i, st = n & 1;
+        ok = mbar_wait_warp(&empty[st], (n >> 1 & 1) ^ 1, &gave_up);
+        if (!ok) break;
+        uint32_t mine = scales;
+        int key = t;  // whose scales they are
+        uint8_t* const k_at = smem + W::K_AT + st * 2 * W::K_BYTES;
+        uint8_t* const v_at = k_at + W::K_BYTES;
+        float* const kf = reinterpret_cast<float*>(smem + W::SCALES_AT + st * 2 * W_KEYS * 4);
+        float* const vf = kf + W_KEYS;
+        if (tree && i == 0) {
+          // thread t: half the dimensions of node t / 2; a row's largest is brought to [64, 128), the codes' range
+          const int node = t >> 1, d0 = (t & 1) * (D / 2);
+          const bool here = node < p.nodes;
+          uint32_t bytes[2];
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv) {
+            const __nv_bfloat16* from = kv == 0 ? p.k + b * p.k_seq + node * p.k_node + h * p.k_head + d0
+                                                : p.v + b * p.v_seq + node * p.v_node + h * p.v_head + d0;
+            uint4 x[D / 16];
+            uint32_t top = 0;
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) {
+              x[c] = here ? __ldg(reinterpret_cast<const uint4*>(from) + c) : make_uint4(0, 0, 0, 0);
+              uint32_t* v = reinterpret_cast<uint32_t*>(&x[c]);
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int sh = 0; sh < 32; sh += 16)
+                  if ((v[j] >> sh & 0x7f80u) == 0x7f80u && kv == 1) {  // V: left out here, put in at the end
+                    v[j] &= ~(0xffffu << sh);
+                    atomicOr(&special[node >> 5], 1u << (node & 31));
+                  }
+#pragma unroll
+              for (int j = 0; j < 4; ++j) top = max(top, max(v[j] & 0x7fffu, v[j] >> 16 & 0x7fffu));
+            }
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            int e = static_cast<int>(top >> 7);
+            e = e == 255 || e < 1 ? 127 : e < 67 ? 67 : e > 247 ? 247 : e;
+            const float f = kv::power(254 - e + 6);
+            bytes[kv] = e - 6;
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) {
+              const uint32_t v[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+              uint32_t y[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) y[j] = pack_f16(low_f(v[j]) * f, high_f(v[j]) * f);
+              const int d = d0 + c * 8;
+              if (kv == 0) {
+                const int at16 = (d >> 6) * 16384 + ((d >> 3 & 7) ^ (node & 7)) * 16;
+                *reinterpret_cast<uint4*>(k_at + at16 + node * 128) = make_uint4(y[0], y[1], y[2], y[3]);
+                *reinterpret_cast<uint4*>(k_at + at16 + (node + 64) * 128) = make_uint4(0, 0, 0, 0);
+              } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                  const int row = d + j, chunk = (node >> 3) ^ (row & 7);
+                  *reinterpret_cast<unsigned short*>(v_at + row * 128 + chunk * 16 + (node & 7) * 2) =
+                      static_cast<unsigned short>(y[j >> 1] >> (16 * (j & 1)));
+                }
+                *reinterpret_cast<uint4*>(v_at + D * 128 + (t * (D / 16) + c) * 16) = make_uint4(0, 0, 0, 0);  // keys 64 on
+              }
+            }
+          }
+          // a node's first thread has its scales, the second those of an empty key past the nodes
+          mine = t & 1 || !here ? 1 | 1 << 8 : bytes[0] | bytes[1] << 8;
+          key = node + (t & 1) * 64;
+        } else {
+#pragma unroll
+          for (int j = 0; j < PIECES; ++j) {
+            const int piece = j * 128 + t, key = piece / PIECES, c = piece % PIECES;
+            const uint32_t v[4] = {kc[j].x, kc[j].y, kc[j].z, kc[j].w};
+            uint32_t y[8];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) kv::decode4<KIND>(v[x], y[2 * x], y[2 * x + 1]);
+            uint8_t* row = k_at + (c >> 2) * 16384 + key * 128;
+            const int chunk = (c & 3) * 2, swap = c >> 2 & 1;  // the two halves' lanes store in turn: no shared banks
+            const uint4 y0 = make_uint4(y[0], y[1], y[2], y[3]), y1 = make_uint4(y[4], y[5], y[6], y[7]);
+            *reinterpret_cast<uint4*>(row + ((chunk + swap) ^ (key & 7)) * 16) = swap ? y1 : y0;
+            *reinterpret_cast<uint4*>(row + ((chunk + 1 - swap) ^ (key & 7)) * 16) = swap ? y0 : y1;
+          }
+#pragma unroll
+          for (int j = 0; j < PIECES; ++j) {
+            const int half = j / (PIECES / 2), quad = lane & 15;
+            const int x = 2 * (w * (PIECES / 2) + j % (PIECES / 2)) + (lane >> 4);
+            const uint32_t v[4] = {vc[j].x, vc[j].y, vc[j].z, vc[j].w};
+#pragma unroll
+            for (int d4 = 0; d4 < 4; ++d4) {
+              const int d = x * 4 + d4;
+              uint2 y;
+              kv::decode4<KIND>(v[d4], y.x, y.y);
+              *reinterpret_cast<uint2*>(v_at + half * D * 128 + d * 128 + ((quad >> 1) ^ (d & 7)) * 16 + (quad & 1) * 8) = y;
+            }
+          }
+        }
+        // the keys' scales, V's relative to the largest so far
+        const uint32_t kb = mine & 0xffu, vb = mine >> 8 & 0xffu;
+        const uint32_t top = __reduce_max_sync(0xffffffffu, vb == 255 ? 0u : vb);
+        const bool nan_here = __any_sync(0xffffffffu, vb == 255);
+        if (lane == 0) {
+          tops[st][w] = static_cast<int>(top) | (nan_here ? 256 : 0);
+          mbar_arrive(told);
+        }
+        ok = mbar_wait_warp(told, n & 1, &gave_up);
+        if (!ok) break;
+        const int t0 = tops[st][0], t1 = tops[st][1], t2 = tops[st][2], t3 = tops[st][3];
+        const int new_ref = max(ref, max(max(t0 & 255, t1 & 255), max(t2 & 255, t3 & 255)));
+        kf[key] = kb == 255 ? __int_as_float(0x7fc00000) : kv::power(kb);
+        vf[key] = vb == 255 ? __int_as_float(0x7fc00000) : kv::power(max(static_cast<int>(vb) - new_ref + 127, 0));
+        if (t == 0) {
+          info[st].nan_v = (t0 | t1 | t2 | t3) >> 8;
+          info[st].unit = i == 0 ? 1.f : ex2(static_cast<float>(ref - new_ref));
+          last_ref = new_ref;
+        }
+        ref = new_ref;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[st]);
+        if (!(tree && i == 0)) fetch();
+      }
+    } else {
+      // ---- the products
+      __syncthreads();
+      constexpr uint32_t to_s = idesc_f16(128, W_KEYS), to_o = idesc_f16(128, D);
+      bool ok = true;
+      const auto scores = [&](int n, int g) {
+        const uint64_t qd = sdesc_kmajor_sw128(sbase + g * W::Q_BYTES);
+        const uint64_t kd = sdesc_kmajor_sw128(sbase + W::K_AT + (n & 1) * 2 * W::K_BYTES);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          if (elect_one())
+            tc_mma(tmem + W::S_COL + g * 128, qd + (k >> 2) * (16384 >> 4) + (k & 3) * 2, kd + (k >> 2) * (16384 >> 4) + (k & 3) * 2,
+                   to_s, k > 0);
+        if (elect_one()) tc_commit(&s_full[g]);
+      };
+      for (int i = 0; i < tiles && ok; ++i) {
+        const int n = done + i;
+        if (i == 0) {
+          ok = mbar_wait_warp(&full[n & 1], n >> 1 & 1, &gave_up);
+          if (!ok) break;
+          tc_fence_after();
+          for (int g = 0; g < groups; ++g) scores(n, g);
+        }
+        for (int g = 0; g < groups && ok; ++g) {
+          ok = mbar_wait_warp(&p_full[g], (g == 0 ? n : done_b + i) & 1, &gave_up);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t vd = sdesc_kmajor_sw128(sbase + W::K_AT + (n & 1) * 2 * W::K_BYTES + W::K_BYTES);
+#pragma unroll
+          for (int k = 0; k < W_KEYS / 16; ++k)
+            if (elect_one())
+              tc_mma_ts(tmem + W::O_COL + g * D, tmem + W::S_COL + g * 128 + k * 8, vd + (k >> 2) * (D * 128 >> 4) + (k & 3) * 2,
+                        to_o, i > 0 || k > 0);
+          if (i + 1 < tiles) {
+            if (g == 0) ok = mbar_wait_warp(&full[n + 1 & 1], n + 1 >> 1 & 1, &gave_up);
+            if (!ok) break;
+            tc_fence_after();
+            scores(n + 1, g);
+          }
+        }
+        if (ok && elect_one()) {
+          tc_commit(&empty[n & 1]);
+          if (i + 1 == tiles) tc_commit(o_full);
+        }
+      }
+    }
+    done += tiles;
+    done_b += groups == 2 ? tiles : 0;
+    parts += tiles > 0;
+    at += u1 - u0;
+    if (u1 == per && item == hr - 1) ++b;
+    __syncthreads();  // Q, O and the marks are free
+    if (gave_up) break;
+  }
+  if (gave_up) {  // products may still be under way: their memory is freed after a bounded wait for them
+    if (warp == 12) {
+      if (elect_one()) tc_commit(o_full);
+      const uint64_t from = global_ns();
+      while (global_ns() - from < 1000000) {
+      }
+    }
+    if (threadIdx.x == 0) record_error(p.c.status, NOISE_DEV_TIMEOUT);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 12) tmem_dealloc(tmem, 512);
+}
+
+}  // namespace tree
+}  // namespace noise

@@ -205,9 +205,9 @@ __global__ void __launch_bounds__(NT, 2) verify_kernel(const Params p) {
     // siblings among the warp's 32 nodes
     const unsigned same = __match_any_sync(0xffffffffu, kid ? up : -1 - tid), after = same & ~((2u << (tid & 31)) - 1);
     sibling[tid] = after ? (tid & 32) + __ffs(after) - 1 : MAX_NODES;
-    asm volatile("bar.sync 1, 64;" ::: "memory");  // of the two warps: the lists are cleared
+    __barrier_sync_count(1, 64);  // of the two warps: the lists are cleared
     if (kid && __ffs(same) - 1 == (tid & 31)) (tid < 32 ? first_kid : later_kid)[up] = tid;
-    asm volatile("bar.sync 1, 64;" ::: "memory");
+    __barrier_sync_count(1, 64);
     if (kid && tid < 32 && !after) sibling[tid] = later_kid[up];  // goes on among the second 32
     if (first_kid[tid] == MAX_NODES) first_kid[tid] = later_kid[tid];
   }
