@@ -6,8 +6,10 @@
 //   warps 0..3, 4..7  softmax of groups A and B, one row a thread: S from tensor memory, P = 2^(x - m) V's scale as fp16
 //                     pairs back into the first half of S's columns (the next product's A operand);
 //   warps 8..11       codes to fp16 in shared memory, in the swizzled rows that tcgen05.mma reads: K by keys, V by
-//                     dimensions with the keys along the row (its four-token quads are 8 bytes of such a row); the codes of
-//                     the next tile are on their way in registers meanwhile; each key's scales beside them;
+//                     dimensions with the keys along the row (its four-token quads are 8 bytes of such a row), and each
+//                     key's scales; the codes of the next two tiles are on their way (cp.async, each thread its own
+//                     pieces). K of a tile is made while the last tile's softmax runs, V while its own does, so one buffer
+//                     of each is enough;
 //   warp 12           tensor memory (512 columns: S / P and O of both groups) and the MMAs: S_g = Q_g K^T and
 //                     O_g += P_g V, group B's while group A's softmax runs.
 // A row's maximum moves when a score passes it by 2^8, and O in tensor memory is rescaled then by its own warps: S_g of
@@ -17,6 +19,7 @@
 
 #include "kv.cuh"
 #include "ptx.cuh"
+#include "warp_mma.cuh"
 
 namespace noise {
 namespace tree {
@@ -30,13 +33,19 @@ __host__ __device__ constexpr uint32_t idesc_f16(int M, int N) {  // fp16 A and 
 template <int D>
 struct Wide {
   static constexpr int Q_BYTES = 128 * D * 2;         // of a group
-  static constexpr int K_BYTES = W_KEYS * D * 2;      // of a stage; V's are as many
-  static constexpr int K_AT = 2 * Q_BYTES;            // [stage] K, V
-  static constexpr int SCALES_AT = K_AT + 4 * K_BYTES;  // [stage] kf, vf: 128 floats each
+  static constexpr int K_BYTES = W_KEYS * D * 2;      // V's are as many
+  static constexpr int K_AT = 2 * Q_BYTES, V_AT = K_AT + K_BYTES;
+  static constexpr int RAW_AT = V_AT + K_BYTES;       // two tiles' codes, K_BYTES each (of K, then of V)
+  static constexpr int SCALES_AT = RAW_AT + 2 * K_BYTES;  // of the tile and the next: kf, vf, 128 floats each
   static constexpr int BAR_AT = SCALES_AT + 2 * 2 * W_KEYS * 4;
   static constexpr int SMEM = BAR_AT + 128;           // then the line's ints, then depths
   static constexpr uint32_t S_COL = 0, O_COL = 256;   // S_A, S_B of 128 columns; O_A, O_B of D
 };
+
+__device__ __forceinline__ void copy16_or_0(uint32_t dst, const void* src, bool there) {
+  const int n = there ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
 
 struct TileInfo {
   float unit;  // what O is to be multiplied by before this tile: 2^(old reference - new)
@@ -49,9 +58,10 @@ __global__ void __launch_bounds__(W_NT, 1) wide_kernel(const Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* const bar = reinterpret_cast<uint64_t*>(smem + W::BAR_AT);
-  uint64_t *const full = bar, *const empty = bar + 2, *const s_full = bar + 4, *const p_full = bar + 6, *const o_full = bar + 8,
-           *const told = bar + 9;
-  uint32_t* const tmem_at = reinterpret_cast<uint32_t*>(bar + 10);
+  // k_full has two barriers, of even and odd tiles: a softmax warp that is late would miss a phase of a single one
+  uint64_t *const k_full = bar, *const k_empty = bar + 2, *const v_full = bar + 3, *const v_empty = bar + 4;
+  uint64_t *const s_full = bar + 5, *const p_full = bar + 7, *const o_full = bar + 9, *const told = bar + 10;
+  uint32_t* const tmem_at = reinterpret_cast<uint32_t*>(bar + 11);
   int* const before = reinterpret_cast<int*>(smem + W::SMEM);
   int* const lens = before + p.seqs + 1;
   int* const depths = lens + p.seqs;
@@ -62,11 +72,13 @@ __global__ void __launch_bounds__(W_NT, 1) wide_kernel(const Params p) {
   cudaTriggerProgrammaticLaunchCompletion();
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&full[i], 4);
-      mbar_init(&empty[i], 1);
+      mbar_init(&k_full[i], 4);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
     }
+    mbar_init(k_empty, 1);
+    mbar_init(v_full, 4);
+    mbar_init(v_empty, 1);
     mbar_init(o_full, 1);
     mbar_init(told, 4);
     fence_barrier_init();
@@ -149,7 +161,7 @@ __global__ void __launch_bounds__(W_NT, 1) wide_kernel(const Params p) {
         bool ok = true;
         for (int i = 0; i < tiles && ok; ++i) {
           const int n = done + i, st = n & 1;
-          ok = mbar_wait_warp(&full[st], n >> 1 & 1, &gave_up) && mbar_wait_warp(&s_full[g], mine + i & 1, &gave_up);
+          ok = mbar_wait_warp(&k_full[st], n >> 1 & 1, &gave_up) && mbar_wait_warp(&s_full[g], mine + i & 1, &gave_up);
           if (!ok) break;
           tc_fence_after();
           const float4* kf = reinterpret_cast<const float4*>(smem + W::SCALES_AT + st * 2 * W_KEYS * 4);
@@ -188,22 +200,23 @@ __global__ void __launch_bounds__(W_NT, 1) wide_kernel(const Params p) {
             sum = 0.f, most = NEG;
             float2 sums = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              float s[32];
+            for (int c = 0; c < 8; ++c) {
+              float s[16];
               __syncwarp();
-              tmem_ld32(s_at + c * 32, s);
+              tmem_ld16(s_at + c * 16, s);
               tc_wait_ld();
-              reg_fence<32>(s);
+              reg_fence<16>(s);
+              const uint32_t bits = see[c >> 1] >> (c & 1) * 16;
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const float4 k4 = kf[c * 8 + j], v4 = vf[c * 8 + j];
+              for (int j = 0; j < 4; ++j) {
+                const float4 k4 = kf[c * 4 + j], v4 = vf[c * 4 + j];
                 float2 a = __fmul2_rn(make_float2(s[4 * j], s[4 * j + 1]), make_float2(k4.x, k4.y));
                 float2 z = __fmul2_rn(make_float2(s[4 * j + 2], s[4 * j + 3]), make_float2(k4.z, k4.w));
                 if constexpr (decltype(masked)::value) {
-                  if (!(see[c] >> (4 * j) & 1)) a.x = NEG;
-                  if (!(see[c] >> (4 * j + 1) & 1)) a.y = NEG;
-                  if (!(see[c] >> (4 * j + 2) & 1)) z.x = NEG;
-                  if (!(see[c] >> (4 * j + 3) & 1)) z.y = NEG;
+                  if (!(bits >> (4 * j) & 1)) a.x = NEG;
+                  if (!(bits >> (4 * j + 1) & 1)) a.y = NEG;
+                  if (!(bits >> (4 * j + 2) & 1)) z.x = NEG;
+                  if (!(bits >> (4 * j + 3) & 1)) z.y = NEG;
                 }
                 a = __ffma2_rn(a, make_float2(rf, rf), make_float2(off, off));
                 z = __ffma2_rn(z, make_float2(rf, rf), make_float2(off, off));
@@ -218,8 +231,8 @@ __global__ void __launch_bounds__(W_NT, 1) wide_kernel(const Params p) {
                 }
                 a = __fmul2_rn(a, va);
                 z = __fmul2_rn(z, vz);
-                pk[c * 16 + 2 * j] = pack_f16(a.x, a.y);
-                pk[c * 16 + 2 * j + 1] = pack_f16(z.x, z.y);
+                pk[c * 8 + 2 * j] = pack_f16(a.x, a.y);
+                pk[c * 8 + 2 * j + 1] = pack_f16(z.x, z.y);
               }
             }
             sum = sums.x + sums.y;
@@ -332,13 +345,13 @@ __global__ void __launch_bounds__(W_NT, 1) wide_kernel(const Params p) {
       // ---- codes to fp16
       const int t = threadIdx.x - 256, w = t >> 5;
       constexpr int PIECES = D / 16;  // 16-byte loads a thread of K, and of V, for 128 keys
-      uint4 kc[PIECES], vc[PIECES];
-      uint32_t scales = 0;  // of key t: K's byte, V's byte
-      int ahead = 0;        // cached tiles asked for
+      uint32_t scales = 0, next_scales = 0;  // of key t: K's byte, V's byte
+      int ahead = 0;                         // cached tiles asked for
       const int cshift = p.page_shift - 4;
       const int* table = p.table + static_cast<int64_t>(b) * p.width;
       const auto fetch = [&] {
         const int key0 = key_lo + ahead++ * W_KEYS;
+        scales = next_scales;
         if (key0 >= key_hi) return;
         int page = 0;  // lane i: of keys 16 i on
         if (lane < 8 && key0 + 16 * lane < len) {
@@ -354,49 +367,49 @@ __global__ void __launch_bounds__(W_NT, 1) wide_kernel(const Params p) {
           return (((p.layer_cell + pg) * p.heads + h) << p.page_shift) +
                  ((((key0 >> 4) + block) & ((1 << cshift) - 1)) << 4);
         };
-#pragma unroll
+        const uint32_t to = sbase + W::RAW_AT + (ahead - 1 & 1) * W::K_BYTES + t * 16;
+#pragma unroll 4
         for (int j = 0; j < PIECES; ++j) {
           const int piece = j * 128 + t, key = piece / PIECES, c = piece % PIECES;
           const int64_t at16 = cell(key >> 4);
-          kc[j] = make_uint4(0, 0, 0, 0);
-          if (key0 + key < len)
-            kc[j] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.c.k) + (at16 + (key & 15)) * D + c * 16));
+          copy16_or_0(to + j * 2048, static_cast<const uint8_t*>(p.c.k) + (at16 + (key & 15)) * D + c * 16, key0 + key < len);
         }
-#pragma unroll
+#pragma unroll 4
         for (int j = 0; j < PIECES; ++j) {  // quad lane % 16 of 64 keys, dimensions 4 x .. 4 x + 3
           const int half = j / (PIECES / 2), quad = half * 16 + (lane & 15);
           const int x = 2 * (w * (PIECES / 2) + j % (PIECES / 2)) + (lane >> 4);
           const int64_t at16 = cell(quad >> 2);
-          vc[j] = make_uint4(0, 0, 0, 0);
-          const int left = len - key0 - quad * 4;
-          if (left > 0) {
-            vc[j] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.c.v) + (at16 + (quad & 3) * 4) * D + x * 16));
-            if (left < 4) {
-              const uint32_t keep = 0xffffffffu >> (32 - 8 * left);
-              vc[j].x &= keep, vc[j].y &= keep, vc[j].z &= keep, vc[j].w &= keep;
-            }
-          }
+          copy16_or_0(to + (PIECES + j) * 2048, static_cast<const uint8_t*>(p.c.v) + (at16 + (quad & 3) * 4) * D + x * 16,
+                      key0 + quad * 4 < len);
         }
         const int64_t at16 = cell(t >> 4);
-        scales = 1 | 1 << 8;
+        next_scales = 1 | 1 << 8;
         if (key0 + t < len)
-          scales = __ldg(p.c.k_scale + at16 + (t & 15)) | static_cast<uint32_t>(__ldg(p.c.v_scale + at16 + (t & 15))) << 8;
+          next_scales =
+              __ldg(p.c.k_scale + at16 + (t & 15)) | static_cast<uint32_t>(__ldg(p.c.v_scale + at16 + (t & 15))) << 8;
       };
       fetch();
+      cp_async_commit();
+      fetch();
+      cp_async_commit();
       __syncthreads();
       bool ok = true;
       int ref = 0;  // the largest scale byte of V so far
       for (int i = 0; i < tiles && ok; ++i) {
         const int n = done + i, st = n & 1;
-        ok = mbar_wait_warp(&empty[st], (n >> 1 & 1) ^ 1, &gave_up);
+        const bool own = tree && i == 0;
+        ok = mbar_wait_warp(k_empty, (n & 1) ^ 1, &gave_up) && (!own || mbar_wait_warp(v_empty, (n & 1) ^ 1, &gave_up));
         if (!ok) break;
+        const int key0 = key_lo + (i - (tree ? 1 : 0)) * W_KEYS;
+        const uint4* const codes =
+            reinterpret_cast<const uint4*>(smem + W::RAW_AT + (i - (tree ? 1 : 0) & 1) * W::K_BYTES) + t;
         uint32_t mine = scales;
         int key = t;  // whose scales they are
-        uint8_t* const k_at = smem + W::K_AT + st * 2 * W::K_BYTES;
-        uint8_t* const v_at = k_at + W::K_BYTES;
+        uint8_t* const k_at = smem + W::K_AT;
+        uint8_t* const v_at = smem + W::V_AT;
         float* const kf = reinterpret_cast<float*>(smem + W::SCALES_AT + st * 2 * W_KEYS * 4);
         float* const vf = kf + W_KEYS;
-        if (tree && i == 0) {
+        if (own) {
           // thread t: half the dimensions of node t / 2; a row's largest is brought to [64, 128), the codes' range
           const int node = t >> 1, d0 = (t & 1) * (D / 2);
           const bool here = node < p.nodes;
@@ -453,31 +466,20 @@ __global__ void __launch_bounds__(W_NT, 1) wide_kernel(const Params p) {
           mine = t & 1 || !here ? 1 | 1 << 8 : bytes[0] | bytes[1] << 8;
           key = node + (t & 1) * 64;
         } else {
-#pragma unroll
+          cp_async_wait<1>();  // this tile's codes are there (each thread copied its own)
+#pragma unroll 4
           for (int j = 0; j < PIECES; ++j) {
-            const int piece = j * 128 + t, key = piece / PIECES, c = piece % PIECES;
-            const uint32_t v[4] = {kc[j].x, kc[j].y, kc[j].z, kc[j].w};
+            const int piece = j * 128 + t, row_key = piece / PIECES, c = piece % PIECES;
+            const uint4 u = codes[j * 128];
+            const uint32_t v[4] = {u.x, u.y, u.z, u.w};
             uint32_t y[8];
 #pragma unroll
             for (int x = 0; x < 4; ++x) kv::decode4<KIND>(v[x], y[2 * x], y[2 * x + 1]);
-            uint8_t* row = k_at + (c >> 2) * 16384 + key * 128;
+            uint8_t* row = k_at + (c >> 2) * 16384 + row_key * 128;
             const int chunk = (c & 3) * 2, swap = c >> 2 & 1;  // the two halves' lanes store in turn: no shared banks
             const uint4 y0 = make_uint4(y[0], y[1], y[2], y[3]), y1 = make_uint4(y[4], y[5], y[6], y[7]);
-            *reinterpret_cast<uint4*>(row + ((chunk + swap) ^ (key & 7)) * 16) = swap ? y1 : y0;
-            *reinterpret_cast<uint4*>(row + ((chunk + 1 - swap) ^ (key & 7)) * 16) = swap ? y0 : y1;
-          }
-#pragma unroll
-          for (int j = 0; j < PIECES; ++j) {
-            const int half = j / (PIECES / 2), quad = lane & 15;
-            const int x = 2 * (w * (PIECES / 2) + j % (PIECES / 2)) + (lane >> 4);
-            const uint32_t v[4] = {vc[j].x, vc[j].y, vc[j].z, vc[j].w};
-#pragma unroll
-            for (int d4 = 0; d4 < 4; ++d4) {
-              const int d = x * 4 + d4;
-              uint2 y;
-              kv::decode4<KIND>(v[d4], y.x, y.y);
-              *reinterpret_cast<uint2*>(v_at + half * D * 128 + d * 128 + ((quad >> 1) ^ (d & 7)) * 16 + (quad & 1) * 8) = y;
-            }
+            *reinterpret_cast<uint4*>(row + ((chunk + swap) ^ (row_key & 7)) * 16) = swap ? y1 : y0;
+            *reinterpret_cast<uint4*>(row + ((chunk + 1 - swap) ^ (row_key & 7)) * 16) = swap ? y0 : y1;
           }
         }
         // the keys' scales, V's relative to the largest so far
@@ -502,51 +504,80 @@ __global__ void __launch_bounds__(W_NT, 1) wide_kernel(const Params p) {
         ref = new_ref;
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&full[st]);
-        if (!(tree && i == 0)) fetch();
+        if (lane == 0) mbar_arrive(&k_full[st]);
+        if (!own) {
+          ok = mbar_wait_warp(v_empty, (n & 1) ^ 1, &gave_up);
+          if (!ok) break;
+#pragma unroll 4
+          for (int j = 0; j < PIECES; ++j) {
+            const int half = j / (PIECES / 2), quad = lane & 15;
+            const int x = 2 * (w * (PIECES / 2) + j % (PIECES / 2)) + (lane >> 4);
+            const int left = len - key0 - (half * 16 + quad) * 4;  // keys of the quad that are there
+            const uint32_t keep = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : 0xffffffffu >> (32 - 8 * left);
+            const uint4 u = codes[(PIECES + j) * 128];
+            const uint32_t v[4] = {u.x & keep, u.y & keep, u.z & keep, u.w & keep};
+#pragma unroll
+            for (int d4 = 0; d4 < 4; ++d4) {
+              const int d = x * 4 + d4;
+              uint2 y;
+              kv::decode4<KIND>(v[d4], y.x, y.y);
+              *reinterpret_cast<uint2*>(v_at + half * D * 128 + d * 128 + ((quad >> 1) ^ (d & 7)) * 16 + (quad & 1) * 8) = y;
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          fetch();
+          cp_async_commit();
+        }
+        if (lane == 0) mbar_arrive(v_full);
       }
+      cp_async_wait<0>();
     } else {
       // ---- the products
       __syncthreads();
       constexpr uint32_t to_s = idesc_f16(128, W_KEYS), to_o = idesc_f16(128, D);
       bool ok = true;
-      const auto scores = [&](int n, int g) {
+      const auto scores = [&](int g) {
         const uint64_t qd = sdesc_kmajor_sw128(sbase + g * W::Q_BYTES);
-        const uint64_t kd = sdesc_kmajor_sw128(sbase + W::K_AT + (n & 1) * 2 * W::K_BYTES);
+        const uint64_t kd = sdesc_kmajor_sw128(sbase + W::K_AT);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
           if (elect_one())
             tc_mma(tmem + W::S_COL + g * 128, qd + (k >> 2) * (16384 >> 4) + (k & 3) * 2, kd + (k >> 2) * (16384 >> 4) + (k & 3) * 2,
                    to_s, k > 0);
-        if (elect_one()) tc_commit(&s_full[g]);
+        if (elect_one()) {
+          tc_commit(&s_full[g]);
+          if (g + 1 == groups) tc_commit(k_empty);
+        }
       };
       for (int i = 0; i < tiles && ok; ++i) {
         const int n = done + i;
         if (i == 0) {
-          ok = mbar_wait_warp(&full[n & 1], n >> 1 & 1, &gave_up);
+          ok = mbar_wait_warp(&k_full[n & 1], n >> 1 & 1, &gave_up);
           if (!ok) break;
           tc_fence_after();
-          for (int g = 0; g < groups; ++g) scores(n, g);
+          for (int g = 0; g < groups; ++g) scores(g);
         }
         for (int g = 0; g < groups && ok; ++g) {
-          ok = mbar_wait_warp(&p_full[g], (g == 0 ? n : done_b + i) & 1, &gave_up);
+          ok = mbar_wait_warp(&p_full[g], (g == 0 ? n : done_b + i) & 1, &gave_up) &&
+               (g > 0 || mbar_wait_warp(v_full, n & 1, &gave_up));
           if (!ok) break;
           tc_fence_after();
-          const uint64_t vd = sdesc_kmajor_sw128(sbase + W::K_AT + (n & 1) * 2 * W::K_BYTES + W::K_BYTES);
+          const uint64_t vd = sdesc_kmajor_sw128(sbase + W::V_AT);
 #pragma unroll
           for (int k = 0; k < W_KEYS / 16; ++k)
             if (elect_one())
               tc_mma_ts(tmem + W::O_COL + g * D, tmem + W::S_COL + g * 128 + k * 8, vd + (k >> 2) * (D * 128 >> 4) + (k & 3) * 2,
                         to_o, i > 0 || k > 0);
           if (i + 1 < tiles) {
-            if (g == 0) ok = mbar_wait_warp(&full[n + 1 & 1], n + 1 >> 1 & 1, &gave_up);
+            if (g == 0) ok = mbar_wait_warp(&k_full[n + 1 & 1], n + 1 >> 1 & 1, &gave_up);
             if (!ok) break;
             tc_fence_after();
-            scores(n + 1, g);
+            scores(g);
           }
         }
         if (ok && elect_one()) {
-          tc_commit(&empty[n & 1]);
+          tc_commit(v_empty);
           if (i + 1 == tiles) tc_commit(o_full);
         }
       }
