@@ -349,38 +349,47 @@ __global__ void __launch_bounds__(W_NT, 1) wide_kernel(const Params p) {
       int ahead = 0;                         // cached tiles asked for
       const int cshift = p.page_shift - 4;
       const int* table = p.table + static_cast<int64_t>(b) * p.width;
+      int next_page = 0;  // of the tile to be asked for next, looked up one tile before
+      const auto look_up = [&](int key0) {
+        next_page = lane < 8 && key0 + 16 * lane < key_hi ? __ldg(table + ((key0 >> 4) + lane >> cshift)) : 0;
+      };
+      look_up(key_lo);
       const auto fetch = [&] {
         const int key0 = key_lo + ahead++ * W_KEYS;
-        scales = next_scales;
         if (key0 >= key_hi) return;
-        int page = 0;  // lane i: of keys 16 i on
-        if (lane < 8 && key0 + 16 * lane < len) {
-          page = __ldg(table + ((key0 >> 4) + lane >> cshift));
-          if (page < 0 || page >= p.c.pages) {
-            lost[turn] = 1;
-            record_error(p.c.status, NOISE_DEV_BAD_INDEX);
-            page = 0;
-          }
+        int page = next_page;  // lane i: of keys 16 i on
+        if (page < 0 || page >= p.c.pages) {
+          lost[turn] = 1;
+          record_error(p.c.status, NOISE_DEV_BAD_INDEX);
+          page = 0;
         }
+        look_up(key0 + W_KEYS);
         const auto cell = [&](int block) {  // of 16 keys
           const int pg = __shfl_sync(0xffffffffu, page, block);
           return (((p.layer_cell + pg) * p.heads + h) << p.page_shift) +
                  ((((key0 >> 4) + block) & ((1 << cshift) - 1)) << 4);
         };
         const uint32_t to = sbase + W::RAW_AT + (ahead - 1 & 1) * W::K_BYTES + t * 16;
-#pragma unroll 4
+        // piece j of K: 16 codes of key (j * 128 + t) / PIECES, which is key `in16` of a block that follows from j
+        constexpr int STEP16 = 128 / PIECES / 16;  // blocks of 16 keys from one j to the next
+        const int in16 = t / PIECES & 15, block0 = t / PIECES >> 4;
+        const bool tail = key0 + W_KEYS > len;
+        const uint8_t* const k_from = static_cast<const uint8_t*>(p.c.k) + in16 * D + t % PIECES * 16;
+#pragma unroll
         for (int j = 0; j < PIECES; ++j) {
-          const int piece = j * 128 + t, key = piece / PIECES, c = piece % PIECES;
-          const int64_t at16 = cell(key >> 4);
-          copy16_or_0(to + j * 2048, static_cast<const uint8_t*>(p.c.k) + (at16 + (key & 15)) * D + c * 16, key0 + key < len);
+          const int block = j * STEP16 + block0;
+          copy16_or_0(to + j * 2048, k_from + cell(block) * D, !tail || key0 + block * 16 + in16 < len);
         }
-#pragma unroll 4
-        for (int j = 0; j < PIECES; ++j) {  // quad lane % 16 of 64 keys, dimensions 4 x .. 4 x + 3
-          const int half = j / (PIECES / 2), quad = half * 16 + (lane & 15);
-          const int x = 2 * (w * (PIECES / 2) + j % (PIECES / 2)) + (lane >> 4);
-          const int64_t at16 = cell(quad >> 2);
-          copy16_or_0(to + (PIECES + j) * 2048, static_cast<const uint8_t*>(p.c.v) + (at16 + (quad & 3) * 4) * D + x * 16,
-                      key0 + quad * 4 < len);
+        // piece j of V: quad lane % 16 of 64 keys (the second half of j: the other 64), dimensions 4 x .. 4 x + 3
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int quad = half * 16 + (lane & 15);
+          const uint8_t* const v_from = static_cast<const uint8_t*>(p.c.v) + (cell(quad >> 2) + (quad & 3) * 4) * D +
+                                        (w * PIECES + (lane >> 4)) * 16;
+          const bool there = key0 + quad * 4 < len;
+#pragma unroll
+          for (int j = 0; j < PIECES / 2; ++j)
+            copy16_or_0(to + (PIECES + half * (PIECES / 2) + j) * 2048, v_from + j * 32, there);
         }
         const int64_t at16 = cell(t >> 4);
         next_scales = 1 | 1 << 8;
@@ -390,26 +399,72 @@ __global__ void __launch_bounds__(W_NT, 1) wide_kernel(const Params p) {
       };
       fetch();
       cp_async_commit();
+      scales = next_scales;
       fetch();
       cp_async_commit();
       __syncthreads();
       bool ok = true;
       int ref = 0;  // the largest scale byte of V so far
-      for (int i = 0; i < tiles && ok; ++i) {
+      uint8_t* const k_at = smem + W::K_AT;
+      uint8_t* const v_at = smem + W::V_AT;
+      // The scales of key `key` of tile n, V's relative to the largest so far; false if a wait gave up.
+      const auto put_scales = [&](int i, uint32_t mine, int key) {
         const int n = done + i, st = n & 1;
-        const bool own = tree && i == 0;
-        ok = mbar_wait_warp(k_empty, (n & 1) ^ 1, &gave_up) && (!own || mbar_wait_warp(v_empty, (n & 1) ^ 1, &gave_up));
-        if (!ok) break;
-        const int key0 = key_lo + (i - (tree ? 1 : 0)) * W_KEYS;
-        const uint4* const codes =
-            reinterpret_cast<const uint4*>(smem + W::RAW_AT + (i - (tree ? 1 : 0) & 1) * W::K_BYTES) + t;
-        uint32_t mine = scales;
-        int key = t;  // whose scales they are
-        uint8_t* const k_at = smem + W::K_AT;
-        uint8_t* const v_at = smem + W::V_AT;
         float* const kf = reinterpret_cast<float*>(smem + W::SCALES_AT + st * 2 * W_KEYS * 4);
         float* const vf = kf + W_KEYS;
-        if (own) {
+        const uint32_t kb = mine & 0xffu, vb = mine >> 8 & 0xffu;
+        const uint32_t top = __reduce_max_sync(0xffffffffu, vb == 255 ? 0u : vb);
+        const bool nan_here = __any_sync(0xffffffffu, vb == 255);
+        if (lane == 0) {
+          tops[st][w] = static_cast<int>(top) | (nan_here ? 256 : 0);
+          mbar_arrive(told);
+        }
+        if (!mbar_wait_warp(told, n & 1, &gave_up)) return false;
+        const int t0 = tops[st][0], t1 = tops[st][1], t2 = tops[st][2], t3 = tops[st][3];
+        const int new_ref = max(ref, max(max(t0 & 255, t1 & 255), max(t2 & 255, t3 & 255)));
+        kf[key] = kb == 255 ? __int_as_float(0x7fc00000) : kv::power(kb);
+        vf[key] = vb == 255 ? __int_as_float(0x7fc00000) : kv::power(max(static_cast<int>(vb) - new_ref + 127, 0));
+        if (t == 0) {
+          info[st].nan_v = (t0 | t1 | t2 | t3) >> 8;
+          info[st].unit = i == 0 ? 1.f : ex2(static_cast<float>(ref - new_ref));
+          last_ref = new_ref;
+        }
+        ref = new_ref;
+        return true;
+      };
+      const auto codes_of = [&](int i) {
+        return reinterpret_cast<const uint4*>(smem + W::RAW_AT + (i - (tree ? 1 : 0) & 1) * W::K_BYTES) + t;
+      };
+      const auto make_k = [&](int i) {  // K and the scales of tile i
+        const int n = done + i;
+        if (!mbar_wait_warp(k_empty, (n & 1) ^ 1, &gave_up)) return false;
+        cp_async_wait<0>();  // the tile's codes are there (each thread copied its own)
+        const uint4* const codes = codes_of(i);
+#pragma unroll 4
+        for (int j = 0; j < PIECES; ++j) {
+          const int piece = j * 128 + t, row_key = piece / PIECES, c = piece % PIECES;
+          const uint4 u = codes[j * 128];
+          const uint32_t v[4] = {u.x, u.y, u.z, u.w};
+          uint32_t y[8];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) kv::decode4<KIND>(v[x], y[2 * x], y[2 * x + 1]);
+          uint8_t* row = k_at + (c >> 2) * 16384 + row_key * 128;
+          const int chunk = (c & 3) * 2, swap = c >> 2 & 1;  // the two halves' lanes store in turn: no shared banks
+          const uint4 y0 = make_uint4(y[0], y[1], y[2], y[3]), y1 = make_uint4(y[4], y[5], y[6], y[7]);
+          *reinterpret_cast<uint4*>(row + ((chunk + swap) ^ (row_key & 7)) * 16) = swap ? y1 : y0;
+          *reinterpret_cast<uint4*>(row + ((chunk + 1 - swap) ^ (row_key & 7)) * 16) = swap ? y0 : y1;
+        }
+        if (!put_scales(i, scales, t)) return false;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&k_full[n & 1]);
+        return true;
+      };
+      if (tree) {  // the first tile: the nodes' own keys and values
+        ok = mbar_wait_warp(k_empty, (done & 1) ^ 1, &gave_up) && mbar_wait_warp(v_empty, (done & 1) ^ 1, &gave_up);
+        if (ok) {
+          uint32_t mine;
+          int key;
           // thread t: half the dimensions of node t / 2; a row's largest is brought to [64, 128), the codes' range
           const int node = t >> 1, d0 = (t & 1) * (D / 2);
           const bool here = node < p.nodes;
@@ -465,71 +520,45 @@ __global__ void __launch_bounds__(W_NT, 1) wide_kernel(const Params p) {
           // a node's first thread has its scales, the second those of an empty key past the nodes
           mine = t & 1 || !here ? 1 | 1 << 8 : bytes[0] | bytes[1] << 8;
           key = node + (t & 1) * 64;
-        } else {
-          cp_async_wait<1>();  // this tile's codes are there (each thread copied its own)
-#pragma unroll 4
-          for (int j = 0; j < PIECES; ++j) {
-            const int piece = j * 128 + t, row_key = piece / PIECES, c = piece % PIECES;
-            const uint4 u = codes[j * 128];
-            const uint32_t v[4] = {u.x, u.y, u.z, u.w};
-            uint32_t y[8];
-#pragma unroll
-            for (int x = 0; x < 4; ++x) kv::decode4<KIND>(v[x], y[2 * x], y[2 * x + 1]);
-            uint8_t* row = k_at + (c >> 2) * 16384 + row_key * 128;
-            const int chunk = (c & 3) * 2, swap = c >> 2 & 1;  // the two halves' lanes store in turn: no shared banks
-            const uint4 y0 = make_uint4(y[0], y[1], y[2], y[3]), y1 = make_uint4(y[4], y[5], y[6], y[7]);
-            *reinterpret_cast<uint4*>(row + ((chunk + swap) ^ (row_key & 7)) * 16) = swap ? y1 : y0;
-            *reinterpret_cast<uint4*>(row + ((chunk + 1 - swap) ^ (row_key & 7)) * 16) = swap ? y0 : y1;
-          }
-        }
-        // the keys' scales, V's relative to the largest so far
-        const uint32_t kb = mine & 0xffu, vb = mine >> 8 & 0xffu;
-        const uint32_t top = __reduce_max_sync(0xffffffffu, vb == 255 ? 0u : vb);
-        const bool nan_here = __any_sync(0xffffffffu, vb == 255);
-        if (lane == 0) {
-          tops[st][w] = static_cast<int>(top) | (nan_here ? 256 : 0);
-          mbar_arrive(told);
-        }
-        ok = mbar_wait_warp(told, n & 1, &gave_up);
-        if (!ok) break;
-        const int t0 = tops[st][0], t1 = tops[st][1], t2 = tops[st][2], t3 = tops[st][3];
-        const int new_ref = max(ref, max(max(t0 & 255, t1 & 255), max(t2 & 255, t3 & 255)));
-        kf[key] = kb == 255 ? __int_as_float(0x7fc00000) : kv::power(kb);
-        vf[key] = vb == 255 ? __int_as_float(0x7fc00000) : kv::power(max(static_cast<int>(vb) - new_ref + 127, 0));
-        if (t == 0) {
-          info[st].nan_v = (t0 | t1 | t2 | t3) >> 8;
-          info[st].unit = i == 0 ? 1.f : ex2(static_cast<float>(ref - new_ref));
-          last_ref = new_ref;
-        }
-        ref = new_ref;
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&k_full[st]);
-        if (!own) {
-          ok = mbar_wait_warp(v_empty, (n & 1) ^ 1, &gave_up);
-          if (!ok) break;
-#pragma unroll 4
-          for (int j = 0; j < PIECES; ++j) {
-            const int half = j / (PIECES / 2), quad = lane & 15;
-            const int x = 2 * (w * (PIECES / 2) + j % (PIECES / 2)) + (lane >> 4);
-            const int left = len - key0 - (half * 16 + quad) * 4;  // keys of the quad that are there
-            const uint32_t keep = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : 0xffffffffu >> (32 - 8 * left);
-            const uint4 u = codes[(PIECES + j) * 128];
-            const uint32_t v[4] = {u.x & keep, u.y & keep, u.z & keep, u.w & keep};
-#pragma unroll
-            for (int d4 = 0; d4 < 4; ++d4) {
-              const int d = x * 4 + d4;
-              uint2 y;
-              kv::decode4<KIND>(v[d4], y.x, y.y);
-              *reinterpret_cast<uint2*>(v_at + half * D * 128 + d * 128 + ((quad >> 1) ^ (d & 7)) * 16 + (quad & 1) * 8) = y;
-            }
-          }
+          ok = put_scales(0, mine, key);
           fence_proxy_async_smem();
           __syncwarp();
-          fetch();
-          cp_async_commit();
+          if (ok && lane == 0) {
+            mbar_arrive(&k_full[done & 1]);
+            mbar_arrive(v_full);
+          }
         }
+      }
+      if (ok && tiles > (tree ? 1 : 0)) ok = make_k(tree ? 1 : 0);
+      scales = next_scales;
+      for (int i = tree ? 1 : 0; i < tiles && ok; ++i) {
+        const int n = done + i, key0 = key_lo + (i - (tree ? 1 : 0)) * W_KEYS;
+        ok = mbar_wait_warp(v_empty, (n & 1) ^ 1, &gave_up);
+        if (!ok) break;
+        const uint4* const codes = codes_of(i);
+#pragma unroll 4
+        for (int j = 0; j < PIECES; ++j) {
+          const int half = j / (PIECES / 2), quad = lane & 15;
+          const int x = 2 * (w * (PIECES / 2) + j % (PIECES / 2)) + (lane >> 4);
+          const int left = len - key0 - (half * 16 + quad) * 4;  // keys of the quad that are there
+          const uint32_t keep = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : 0xffffffffu >> (32 - 8 * left);
+          const uint4 u = codes[(PIECES + j) * 128];
+          const uint32_t v[4] = {u.x & keep, u.y & keep, u.z & keep, u.w & keep};
+#pragma unroll
+          for (int d4 = 0; d4 < 4; ++d4) {
+            const int d = x * 4 + d4;
+            uint2 y;
+            kv::decode4<KIND>(v[d4], y.x, y.y);
+            *reinterpret_cast<uint2*>(v_at + half * D * 128 + d * 128 + ((quad >> 1) ^ (d & 7)) * 16 + (quad & 1) * 8) = y;
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
         if (lane == 0) mbar_arrive(v_full);
+        if (i + 1 < tiles) ok = make_k(i + 1);  // before the next copies: S waits for it
+        fetch();
+        cp_async_commit();
+        scales = next_scales;
       }
       cp_async_wait<0>();
     } else {
