@@ -106,10 +106,6 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 __device__ __forceinline__ float low_f(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float high_f(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
-#ifndef WIDE_FROM
-#define WIDE_FROM 32
-#endif
-
 // ---- the line of units ------------------------------------------------------------------------------------------
 
 __device__ __forceinline__ int length_of(const Params& p, int b) {
@@ -674,8 +670,9 @@ __global__ void __launch_bounds__(Shape<KIND, D, NTL, RW>::NT)
         if (edge) {
           const int k16 = key0 + 16 * j, left4 = len - k16 - 4 * t, k0 = k16 + key_of(g);
           keep[j] = left4 >= 4 ? 0xffffffffu : left4 <= 0 ? 0u : 0xffffffffu >> (32 - 8 * left4);
-          if (k0 >= len) vb[j][0] = 0;
-          if (k0 + 2 >= len) vb[j][1] = 0;
+          const int seen = p.window < 0 ? 0 : len - p.window;  // no row sees a key before: its scale counts for nothing
+          if (k0 >= len || k0 < seen) vb[j][0] = 0;
+          if (k0 + 2 >= len || k0 + 2 < seen) vb[j][1] = 0;
 #pragma unroll
           for (int nt = 0; nt < NTL; ++nt)
 #pragma unroll
@@ -954,16 +951,22 @@ constexpr int max_grid(int tile) { return 148 * (tile <= 8 ? 8 : tile <= 16 ? 4 
 
 constexpr int MAX_WIDE_GRID = 148;
 
-// Whether a call goes to the tcgen05 kernel: its tile of 128 rows is worth filling from 33 rows on; a bf16 cache has no
-// codes to bring to shared memory and stays; the line's lengths have to fit beside the tiles.
-inline bool wide_rows(int kind, int rows, int seqs) {
-  return kind != NOISE_KV_BF16 && rows > WIDE_FROM && seqs <= 2048;
+// Whether a call goes to the tcgen05 kernel: more than WIDE_ROWS rows a key head, WIDE_KEYS keys of all heads and
+// sequences that the tables have room for, an 8-bit cache (a bf16 one has no codes to convert), and lengths that fit
+// beside the tiles. Measured on int8, 8 key heads, this kernel's tiles of 64 rows : tcgen05's of 256, in us:
+//   D = 64,  16 x 8192 keys: 110 : 264 at 64 rows, 208 : 277 at 128, 303 : 296 at 192, 399 : 303 at 256
+//   D = 128, 16 x 8192 keys: 177 : 359 at 64 rows, 328 : 373 at 128, 474 : 386 at 192, 625 : 393 at 256
+//   D = 128, 256 rows: 41 : 67 at 1 x 2048 keys (2^14 of all heads), 123 : 96 at 8 x 2048 (2^17)
+// The codes' conversion takes as long for few rows as for many, and an item's start and end some 17 us.
+constexpr int WIDE_ROWS = 128;
+constexpr int64_t WIDE_KEYS = 1 << 17;
+
+inline bool wide_rows(int kind, int rows, int seqs, int heads, int64_t room) {
+  return kind != NOISE_KV_BF16 && rows > WIDE_ROWS && seqs <= 2048 && seqs * heads * room >= WIDE_KEYS;
 }
 
-// The row tile of a call: the least of 8, 16, 32 and 64 rows that holds all, or 64; W_ROWS on tcgen05.
-inline int tile_rows(int kind, int rows, int seqs) {
-  return wide_rows(kind, rows, seqs) ? W_ROWS : rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
-}
+// The row tile of a call on this file's kernel: the least of 8, 16, 32 and 64 rows that holds all, or 64.
+inline int narrow_tile(int rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 
 inline int sm_count() {
   int dev = 0, n = 0;
@@ -1044,7 +1047,8 @@ template <int KIND, int D>
 int by_rows(Params& p, size_t bytes, cudaStream_t s) {
   const int rows = p.nodes * p.group;
   if constexpr (KIND != NOISE_KV_BF16) {
-    if (wide_rows(KIND, rows, p.seqs)) return run_wide<KIND, D>(p, bytes, s);
+    if (wide_rows(KIND, rows, p.seqs, p.heads, static_cast<int64_t>(p.width) << p.page_shift))
+      return run_wide<KIND, D>(p, bytes, s);
   }
   if (rows <= 8) return run<KIND, D, 1, 1>(p, bytes, s);
   if (rows <= 16) return run<KIND, D, 2, 1>(p, bytes, s);
@@ -1065,13 +1069,13 @@ extern "C" {
 size_t noise_tree_attention_workspace_bytes(int seqs, int nodes, int q_heads, int heads, int dim) {
   if (seqs < 1 || nodes < 1 || heads < 1 || q_heads < heads || q_heads % heads || (dim != 64 && dim != 128)) return 0;
   using namespace noise::tree;
-  size_t rows = 0;  // of either kernel: the cache's kind is not known here
-  for (const int kind : {NOISE_KV_BF16, NOISE_KV_INT8}) {
-    const int tile = tile_rows(kind, nodes * (q_heads / heads), seqs);
-    const size_t need = static_cast<size_t>(2) * (tile == W_ROWS ? MAX_WIDE_GRID : max_grid(tile)) * tile;
-    if (need > rows) rows = need;
-  }
-  return rows * (dim + 2) * sizeof(float);
+  const int64_t rows = static_cast<int64_t>(nodes) * (q_heads / heads);
+  if (rows > 64 * 64) return 0;
+  const int tile = narrow_tile(static_cast<int>(rows));
+  size_t parts = static_cast<size_t>(2) * max_grid(tile) * tile;
+  // of either kernel: the cache's kind and the tables' width are not known here
+  if (rows > WIDE_ROWS && parts < static_cast<size_t>(2) * MAX_WIDE_GRID * W_ROWS) parts = 2 * MAX_WIDE_GRID * W_ROWS;
+  return parts * (dim + 2) * sizeof(float);
 }
 
 int noise_tree_attention(const noise_kv_cache_t* cache, int layer, const void* q, int64_t q_seq_stride,
@@ -1104,7 +1108,7 @@ int noise_tree_attention(const noise_kv_cache_t* cache, int layer, const void* q
   for (int64_t stride : {q_seq_stride, q_node_stride, q_head_stride, k_seq_stride, k_node_stride, k_head_stride,
                          v_seq_stride, v_node_stride, v_head_stride})
     if (stride % 8) return NOISE_ERR_ALIGN;
-  const int group = q_heads / cache->heads, tile = tile_rows(cache->kind, nodes * group, seqs);
+  const int group = q_heads / cache->heads, tile = narrow_tile(nodes * group);
   const int tiles = (nodes * group + tile - 1) / tile;
   if (static_cast<int64_t>(seqs) * cache->heads * tiles > 0x7fffffff) return NOISE_ERR_SHAPE;
   if (!workspace) return NOISE_ERR_WORKSPACE;

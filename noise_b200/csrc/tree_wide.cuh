@@ -1,16 +1,16 @@
 // Tree attention over an 8-bit cache with many query rows a key head, on tcgen05 (included by tree_attention.cu, whose
 // line of units, parts and join it shares).
 //
-// With more than 32 rows the products bound the call, not the cache's bytes: 4 D operations a row and key, on a dense
-// tile of 128 rows. A CTA takes up to 256 rows of one key head (groups A and B of 128) and walks 128 keys at a time:
-//   warps 0..3, 4..7  softmax of groups A and B, one row a thread: S from tensor memory, P = 2^(x - m) V's scale as fp16
-//                     pairs back into the first half of S's columns (the next product's A operand);
-//   warps 8..11       codes to fp16 in shared memory, in the swizzled rows that tcgen05.mma reads: K by keys, V by
-//                     dimensions with the keys along the row (its four-token quads are 8 bytes of such a row), and each
-//                     key's scales; the codes of the next two tiles are on their way (cp.async, each thread its own
-//                     pieces). K of a tile is made while the last tile's softmax runs, V while its own does, so one buffer
-//                     of each is enough;
-//   warp 12           tensor memory (512 columns: S / P and O of both groups) and the MMAs: S_g = Q_g K^T and
+// With more than 128 rows the products bound the call, not the cache's bytes: 4 D operations a row and key, on dense
+// tiles of 128 rows. A CTA takes up to 256 rows of one key head (groups A and B of 128) and walks 128 keys at a time:
+//   warps 0..3, 4..7  softmax of groups A and B, one row a thread: S from tensor memory, P = 2^(x - m) as fp16 pairs
+//                     back into the first half of S's columns (the next product's A operand);
+//   warps 8..11       K's codes to fp16 in the swizzled rows that tcgen05.mma reads, 12..15 V's, by dimensions with the
+//                     keys along the row (its four-token quads are 8 bytes of such a row); a code is multiplied by its
+//                     key's scale over the tile's largest, so S and O carry one power of two a tile. The codes of the next
+//                     two tiles are on their way (cp.async, each thread its own pieces). K of a tile is made while the
+//                     last tile's softmax runs, V while its own does, so one buffer of each is enough;
+//   warp 16           tensor memory (512 columns: S / P and O of both groups) and the MMAs: S_g = Q_g K^T and
 //                     O_g += P_g V, group B's while group A's softmax runs.
 // A row's maximum moves when a score passes it by 2^8, and O in tensor memory is rescaled then by its own warps: S_g of
 // a tile is only issued after P_g V of the last one, so O is still. The tree's own keys are the first tile, brought to
@@ -24,7 +24,7 @@
 namespace noise {
 namespace tree {
 
-constexpr int W_KEYS = 128, W_ROWS = 256, W_NT = 13 * 32;
+constexpr int W_KEYS = 128, W_ROWS = 256, W_NT = 17 * 32;
 
 __host__ __device__ constexpr uint32_t idesc_f16(int M, int N) {  // fp16 A and B, fp32 D
   return (1u << 4) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
@@ -35,9 +35,8 @@ struct Wide {
   static constexpr int Q_BYTES = 128 * D * 2;         // of a group
   static constexpr int K_BYTES = W_KEYS * D * 2;      // V's are as many
   static constexpr int K_AT = 2 * Q_BYTES, V_AT = K_AT + K_BYTES;
-  static constexpr int RAW_AT = V_AT + K_BYTES;       // two tiles' codes, K_BYTES each (of K, then of V)
-  static constexpr int SCALES_AT = RAW_AT + 2 * K_BYTES;  // of the tile and the next: kf, vf, 128 floats each
-  static constexpr int BAR_AT = SCALES_AT + 2 * 2 * W_KEYS * 4;
+  static constexpr int RAW_AT = V_AT + K_BYTES;       // two tiles' codes of K, two of V, K_BYTES / 2 each
+  static constexpr int BAR_AT = RAW_AT + 2 * K_BYTES;
   static constexpr int SMEM = BAR_AT + 128;           // then the line's ints, then depths
   static constexpr uint32_t S_COL = 0, O_COL = 256;   // S_A, S_B of 128 columns; O_A, O_B of D
 };
@@ -48,9 +47,22 @@ __device__ __forceinline__ void copy16_or_0(uint32_t dst, const void* src, bool 
 }
 
 struct TileInfo {
-  float unit;  // what O is to be multiplied by before this tile: 2^(old reference - new)
-  int nan_v;   // some key's V reads as NaN
+  float k_scale;  // of the tile's keys
+  float unit;     // what O is to be multiplied by before this tile: 2^(V's old reference - its new one)
+  int nan_v;      // some key's V reads as NaN
 };
+
+// 2^(byte - ref) in fp16, twice (byte <= ref).
+__device__ __forceinline__ __half2 relative(int byte, int ref) {
+  const int e = 15 + byte - ref;
+  const unsigned short h = e > 0 ? e << 10 : e > -10 ? 1 << (9 + e) : 0;
+  return __half2half2(__ushort_as_half(h));
+}
+
+__device__ __forceinline__ uint32_t times(uint32_t codes, __half2 f) {
+  const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&codes), f);
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
 
 template <int KIND, int D>
 __global__ void __launch_bounds__(W_NT, 1) wide_kernel(const Params p) {
@@ -58,21 +70,25 @@ __global__ void __launch_bounds__(W_NT, 1) wide_kernel(const Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* const bar = reinterpret_cast<uint64_t*>(smem + W::BAR_AT);
-  // k_full has two barriers, of even and odd tiles: a softmax warp that is late would miss a phase of a single one
-  uint64_t *const k_full = bar, *const k_empty = bar + 2, *const v_full = bar + 3, *const v_empty = bar + 4;
-  uint64_t *const s_full = bar + 5, *const p_full = bar + 7, *const o_full = bar + 9, *const told = bar + 10;
-  uint32_t* const tmem_at = reinterpret_cast<uint32_t*>(bar + 11);
+  // two barriers, of even and odd tiles, where a softmax warp that is late would miss a phase of a single one
+  uint64_t *const k_full = bar, *const v_known = bar + 2, *const k_empty = bar + 4, *const v_full = bar + 5;
+  uint64_t *const v_empty = bar + 6, *const s_full = bar + 7, *const p_full = bar + 9, *const o_full = bar + 11;
+  uint64_t* const told = bar + 12;  // of K's warps, of V's
+  uint32_t* const tmem_at = reinterpret_cast<uint32_t*>(bar + 14);
   int* const before = reinterpret_cast<int*>(smem + W::SMEM);
   int* const lens = before + p.seqs + 1;
   int* const depths = lens + p.seqs;
   __shared__ TileInfo info[2];
-  __shared__ int gave_up, lost[2], last_ref, tops[2][4];  // lost: a page of this (or the next) item out of range
+  __shared__ int gave_up, lost[2], last_ref, tops[2][2][4];  // lost: a page of this (or the next) item out of range
+  __shared__ __align__(16) uint8_t bytes[2][2][W_KEYS];      // scales of K, of V; of even and odd tiles
   __shared__ unsigned special[2];  // nodes whose V is not finite
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   cudaTriggerProgrammaticLaunchCompletion();
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&k_full[i], 4);
+      mbar_init(&v_known[i], 4);
+      mbar_init(&told[i], 4);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
     }
@@ -80,11 +96,10 @@ __global__ void __launch_bounds__(W_NT, 1) wide_kernel(const Params p) {
     mbar_init(v_full, 4);
     mbar_init(v_empty, 1);
     mbar_init(o_full, 1);
-    mbar_init(told, 4);
     fence_barrier_init();
     gave_up = lost[0] = lost[1] = 0;
   }
-  if (warp == 12) {
+  if (warp == 16) {
     tmem_alloc(tmem_at, 512);
     tmem_relinquish();
   }
@@ -161,11 +176,11 @@ __global__ void __launch_bounds__(W_NT, 1) wide_kernel(const Params p) {
         bool ok = true;
         for (int i = 0; i < tiles && ok; ++i) {
           const int n = done + i, st = n & 1;
-          ok = mbar_wait_warp(&k_full[st], n >> 1 & 1, &gave_up) && mbar_wait_warp(&s_full[g], mine + i & 1, &gave_up);
+          ok = mbar_wait_warp(&k_full[st], n >> 1 & 1, &gave_up) && mbar_wait_warp(&v_known[st], n >> 1 & 1, &gave_up) &&
+               mbar_wait_warp(&s_full[g], mine + i & 1, &gave_up);
           if (!ok) break;
           tc_fence_after();
-          const float4* kf = reinterpret_cast<const float4*>(smem + W::SCALES_AT + st * 2 * W_KEYS * 4);
-          const float4* vf = kf + W_KEYS / 4;
+          const float rt = rf * info[st].k_scale;
           const bool own = tree && i == 0;
           const int key0 = key_lo + (i - (tree ? 1 : 0)) * W_KEYS;
           const bool edge = own || key0 + W_KEYS > len || (p.window >= 0 && key0 < len + p.nodes - p.window);
@@ -186,12 +201,11 @@ __global__ void __launch_bounds__(W_NT, 1) wide_kernel(const Params p) {
               see[j] = up_to & from;
             }
           }
-          if (info[st].nan_v) {  // keys whose V reads as NaN have factor 0 in the product: their rows' sums say it
+          if (info[st].nan_v) {  // keys whose V reads as NaN are 0 in the product: their rows' sums say it
 #pragma unroll 1
             for (int c = 0; c < W_KEYS; ++c)
-              if (reinterpret_cast<const float*>(vf)[c] != reinterpret_cast<const float*>(vf)[c] &&
-                  (see[c >> 5] >> (c & 31) & 1))
-                l = __int_as_float(0x7fc00000);
+              if (bytes[1][st][c] == 255 && (see[c >> 5] >> (c & 31) & 1)) l = __int_as_float(0x7fc00000);
+            __syncwarp();
           }
           // Probabilities of the tile as packed pairs, their sum, and how far the largest passes the maximum.
           uint32_t pk[W_KEYS / 2];
@@ -208,37 +222,22 @@ __global__ void __launch_bounds__(W_NT, 1) wide_kernel(const Params p) {
               reg_fence<16>(s);
               const uint32_t bits = see[c >> 1] >> (c & 1) * 16;
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const float4 k4 = kf[c * 4 + j], v4 = vf[c * 4 + j];
-                float2 a = __fmul2_rn(make_float2(s[4 * j], s[4 * j + 1]), make_float2(k4.x, k4.y));
-                float2 z = __fmul2_rn(make_float2(s[4 * j + 2], s[4 * j + 3]), make_float2(k4.z, k4.w));
+              for (int j = 0; j < 8; ++j) {
+                float2 a = make_float2(s[2 * j], s[2 * j + 1]);
                 if constexpr (decltype(masked)::value) {
-                  if (!(bits >> (4 * j) & 1)) a.x = NEG;
-                  if (!(bits >> (4 * j + 1) & 1)) a.y = NEG;
-                  if (!(bits >> (4 * j + 2) & 1)) z.x = NEG;
-                  if (!(bits >> (4 * j + 3) & 1)) z.y = NEG;
+                  if (!(bits >> (2 * j) & 1)) a.x = NEG;
+                  if (!(bits >> (2 * j + 1) & 1)) a.y = NEG;
                 }
-                a = __ffma2_rn(a, make_float2(rf, rf), make_float2(off, off));
-                z = __ffma2_rn(z, make_float2(rf, rf), make_float2(off, off));
-                most = fmaxf(fmaxf(most, fmaxf(a.x, a.y)), fmaxf(z.x, z.y));
+                a = __ffma2_rn(a, make_float2(rt, rt), make_float2(off, off));
+                most = fmaxf(most, fmaxf(a.x, a.y));
                 a = make_float2(ex2(a.x), ex2(a.y));
-                z = make_float2(ex2(z.x), ex2(z.y));
-                sums = __fadd2_rn(sums, __fadd2_rn(a, z));
-                float2 va = make_float2(v4.x, v4.y), vz = make_float2(v4.z, v4.w);
-                if constexpr (decltype(masked)::value) {  // (a masked key's factor may be NaN)
-                  va = make_float2(va.x == va.x ? va.x : 0.f, va.y == va.y ? va.y : 0.f);
-                  vz = make_float2(vz.x == vz.x ? vz.x : 0.f, vz.y == vz.y ? vz.y : 0.f);
-                }
-                a = __fmul2_rn(a, va);
-                z = __fmul2_rn(z, vz);
-                pk[c * 8 + 2 * j] = pack_f16(a.x, a.y);
-                pk[c * 8 + 2 * j + 1] = pack_f16(z.x, z.y);
+                sums = __fadd2_rn(sums, a);
+                pk[c * 8 + j] = pack_f16(a.x, a.y);
               }
             }
             sum = sums.x + sums.y;
           };
-          const bool careful = edge || info[st].nan_v;
-          if (careful) soften(std::true_type{});
+          if (edge) soften(std::true_type{});
           else soften(std::false_type{});
           const float unit = info[st].unit;
           if (__any_sync(0xffffffffu, most > SLACK || unit != 1.f)) {
@@ -252,11 +251,10 @@ __global__ void __launch_bounds__(W_NT, 1) wide_kernel(const Params p) {
               reg_fence<32>(s);
 #pragma unroll
               for (int j = 0; j < 32; ++j) {
-                const float v = s[j] * reinterpret_cast<const float*>(kf)[c * 32 + j];
-                if (see[c] >> j & 1) x = fmaxf(x, v);
+                if (see[c] >> j & 1) x = fmaxf(x, s[j]);
               }
             }
-            x *= rf;
+            x *= rt;
             float f = 1.f;
             if (most > SLACK && x > -off) {
               f = ex2(-off - x);
@@ -279,7 +277,7 @@ __global__ void __launch_bounds__(W_NT, 1) wide_kernel(const Params p) {
                 tmem_st16(o_at + c * 16, w);
               }
             }
-            if (careful) soften(std::true_type{});
+            if (edge) soften(std::true_type{});
             else soften(std::false_type{});
           }
           l += sum;
@@ -298,11 +296,10 @@ __global__ void __launch_bounds__(W_NT, 1) wide_kernel(const Params p) {
         const float to = tiles > 0 ? ex2(static_cast<float>(last_ref - 127)) : 0.f;
         if (lost[turn] || !ok) l = __int_as_float(0x7fc00000);
         const uint64_t odd = (mask & (static_cast<uint64_t>(special[1]) << 32 | special[0]));
+        // 32 rows by D in the tiles' memory, which no product reads any more: rows leave whole
+        float4* const stage = reinterpret_cast<float4*>(smem + W::K_AT + warp * 32 * D * 4);
         const bool pad = depth < 0;
         const float f = pad ? 0.f : !whole ? to : l == 0.f ? 0.f : to / l;
-        __nv_bfloat16* out =
-            p.out + ((static_cast<int64_t>(b) * p.nodes + node) * p.heads * p.group + h * p.group + r - node * p.group) * D;
-        float* po = p.partial + (static_cast<int64_t>(slot) * W_ROWS + g * 128 + in) * D;
         float* pm = p.partial + static_cast<int64_t>(2 * p.grid) * W_ROWS * D + static_cast<int64_t>(slot) * 2 * W_ROWS + g * 128 + in;
         if (real && !whole) {
           pm[0] = off;
@@ -328,36 +325,51 @@ __global__ void __launch_bounds__(W_NT, 1) wide_kernel(const Params p) {
               }
             }
           }
-          if (!real) continue;
-          if (whole) {
-            uint4* w = reinterpret_cast<uint4*>(out + c * 16);
-            w[0] = make_uint4(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]), pack_bf16(o[4], o[5]), pack_bf16(o[6], o[7]));
-            w[1] = make_uint4(pack_bf16(o[8], o[9]), pack_bf16(o[10], o[11]), pack_bf16(o[12], o[13]), pack_bf16(o[14], o[15]));
-          } else {
 #pragma unroll
-            for (int j = 0; j < 16; j += 4)
-              *reinterpret_cast<float4*>(po + c * 16 + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+          for (int j = 0; j < 4; ++j)
+            stage[lane * (D / 4) + ((c * 4 + j) ^ (lane & (D / 4 - 1)))] =
+                make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+        }
+        __syncwarp();
+#pragma unroll 4
+        for (int i = lane; i < 32 * (D / 4); i += 32) {
+          const int k = i / (D / 4), c = i % (D / 4), rk = row0 + warp * 32 + k;
+          if (rk >= rows) continue;
+          const float4 o = stage[k * (D / 4) + (c ^ (k & (D / 4 - 1)))];
+          if (whole) {
+            const int nk = rk / p.group;
+            __nv_bfloat16* const out =
+                p.out + ((static_cast<int64_t>(b) * p.nodes + nk) * p.heads * p.group + h * p.group + rk - nk * p.group) * D;
+            *reinterpret_cast<uint2*>(out + c * 4) = make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
+          } else {
+            *reinterpret_cast<float4*>(p.partial + (static_cast<int64_t>(slot) * W_ROWS + warp * 32 + k) * D + c * 4) = o;
           }
         }
         tc_fence_before();
       }
-    } else if (warp < 12) {
-      // ---- codes to fp16
-      const int t = threadIdx.x - 256, w = t >> 5;
-      constexpr int PIECES = D / 16;  // 16-byte loads a thread of K, and of V, for 128 keys
-      uint32_t scales = 0, next_scales = 0;  // of key t: K's byte, V's byte
+    } else if (warp < 16) {
+      // ---- codes to fp16: four warps K's, four V's
+      const int t = threadIdx.x & 127, w = t >> 5, side = warp < 12 ? 0 : 1;
+      constexpr int PIECES = D / 16;         // 16-byte loads a thread for 128 keys
+      uint32_t scale = 0, next_scale = 0;    // of key t
       int ahead = 0;                         // cached tiles asked for
       const int cshift = p.page_shift - 4;
       const int* table = p.table + static_cast<int64_t>(b) * p.width;
+      const uint8_t* const from = static_cast<const uint8_t*>(side == 0 ? p.c.k : p.c.v);
+      const uint8_t* const scales = side == 0 ? p.c.k_scale : p.c.v_scale;
+      const uint32_t raw_at = W::RAW_AT + side * W::K_BYTES + t * 16;
       int next_page = 0;  // of the tile to be asked for next, looked up one tile before
-      const auto look_up = [&](int key0) {
+      const auto look_up = [&](int key0) {  // lane i: of keys 16 i on
         next_page = lane < 8 && key0 + 16 * lane < key_hi ? __ldg(table + ((key0 >> 4) + lane >> cshift)) : 0;
       };
       look_up(key_lo);
+      // keys that no row sees, before every window, past the end or of padding, have no part in the references
+      const int seen_from = p.window < 0 ? 0 : len - p.window;
       const auto fetch = [&] {
         const int key0 = key_lo + ahead++ * W_KEYS;
+        scale = next_scale;
         if (key0 >= key_hi) return;
-        int page = next_page;  // lane i: of keys 16 i on
+        int page = next_page;
         if (page < 0 || page >= p.c.pages) {
           lost[turn] = 1;
           record_error(p.c.status, NOISE_DEV_BAD_INDEX);
@@ -369,196 +381,208 @@ __global__ void __launch_bounds__(W_NT, 1) wide_kernel(const Params p) {
           return (((p.layer_cell + pg) * p.heads + h) << p.page_shift) +
                  ((((key0 >> 4) + block) & ((1 << cshift) - 1)) << 4);
         };
-        const uint32_t to = sbase + W::RAW_AT + (ahead - 1 & 1) * W::K_BYTES + t * 16;
-        // piece j of K: 16 codes of key (j * 128 + t) / PIECES, which is key `in16` of a block that follows from j
-        constexpr int STEP16 = 128 / PIECES / 16;  // blocks of 16 keys from one j to the next
-        const int in16 = t / PIECES & 15, block0 = t / PIECES >> 4;
-        const bool tail = key0 + W_KEYS > len;
-        const uint8_t* const k_from = static_cast<const uint8_t*>(p.c.k) + in16 * D + t % PIECES * 16;
+        const uint32_t to = sbase + raw_at + (ahead - 1 & 1) * (W::K_BYTES / 2);
+        if (side == 0) {
+          // piece j: 16 codes of key (j * 128 + t) / PIECES, which is key `in16` of a block that follows from j
+          constexpr int STEP16 = 128 / PIECES / 16;  // blocks of 16 keys from one j to the next
+          const int in16 = t / PIECES & 15, block0 = t / PIECES >> 4;
+          const uint8_t* const at16 = from + in16 * D + t % PIECES * 16;
 #pragma unroll
-        for (int j = 0; j < PIECES; ++j) {
-          const int block = j * STEP16 + block0;
-          copy16_or_0(to + j * 2048, k_from + cell(block) * D, !tail || key0 + block * 16 + in16 < len);
+          for (int j = 0; j < PIECES; ++j) {
+            const int block = j * STEP16 + block0;
+            copy16_or_0(to + j * 2048, at16 + cell(block) * D, key0 + block * 16 + in16 < len);
+          }
+        } else {
+          // piece j: quad lane % 16 of 64 keys (the second half of j: the other 64), dimensions 4 x .. 4 x + 3
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int quad = half * 16 + (lane & 15);
+            const uint8_t* const at16 = from + (cell(quad >> 2) + (quad & 3) * 4) * D + (w * PIECES + (lane >> 4)) * 16;
+            const bool there = key0 + quad * 4 < len;
+#pragma unroll
+            for (int j = 0; j < PIECES / 2; ++j)
+              copy16_or_0(to + (half * (PIECES / 2) + j) * 2048, at16 + j * 32, there);
+          }
         }
-        // piece j of V: quad lane % 16 of 64 keys (the second half of j: the other 64), dimensions 4 x .. 4 x + 3
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int quad = half * 16 + (lane & 15);
-          const uint8_t* const v_from = static_cast<const uint8_t*>(p.c.v) + (cell(quad >> 2) + (quad & 3) * 4) * D +
-                                        (w * PIECES + (lane >> 4)) * 16;
-          const bool there = key0 + quad * 4 < len;
-#pragma unroll
-          for (int j = 0; j < PIECES / 2; ++j)
-            copy16_or_0(to + (PIECES + half * (PIECES / 2) + j) * 2048, v_from + j * 32, there);
-        }
-        const int64_t at16 = cell(t >> 4);
-        next_scales = 1 | 1 << 8;
-        if (key0 + t < len)
-          next_scales =
-              __ldg(p.c.k_scale + at16 + (t & 15)) | static_cast<uint32_t>(__ldg(p.c.v_scale + at16 + (t & 15))) << 8;
+        const int64_t at = cell(t >> 4) + (t & 15);
+        next_scale = key0 + t >= seen_from && key0 + t < len ? __ldg(scales + at) : 1;
       };
       fetch();
       cp_async_commit();
-      scales = next_scales;
-      fetch();
-      cp_async_commit();
+      // the nodes' own keys or values: thread t has half the dimensions of node t / 2
+      const int node = t >> 1, d0 = (t & 1) * (D / 2);
+      uint64_t seen = 0;  // nodes that some row sees
+      if (tree) {
+        for (int i = lane; i < p.nodes; i += 32)
+          if (__ldg(p.depth + b * p.nodes + i) >= 0) seen |= __ldg(p.mask + b * p.nodes + i);
+        seen = static_cast<uint64_t>(__reduce_or_sync(0xffffffffu, static_cast<uint32_t>(seen >> 32))) << 32 |
+               __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(seen));
+      }
+      const bool here = tree && node < p.nodes && (seen >> node & 1);
+      uint4 x[D / 16];
+      {
+        const __nv_bfloat16* src = side == 0 ? p.k + b * p.k_seq + node * p.k_node + h * p.k_head + d0
+                                             : p.v + b * p.v_seq + node * p.v_node + h * p.v_head + d0;
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c)
+          x[c] = here ? __ldg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0, 0, 0, 0);
+      }
       __syncthreads();
       bool ok = true;
-      int ref = 0;  // the largest scale byte of V so far
-      uint8_t* const k_at = smem + W::K_AT;
-      uint8_t* const v_at = smem + W::V_AT;
-      // The scales of key `key` of tile n, V's relative to the largest so far; false if a wait gave up.
-      const auto put_scales = [&](int i, uint32_t mine, int key) {
+      int ref = 0;  // V: the largest scale byte so far; K: this tile's
+      uint8_t* const out = smem + (side == 0 ? W::K_AT : W::V_AT);
+      // Key `key`'s scale byte told to the other warps of the side and theirs heard: ref; false if a wait gave up.
+      const auto hear = [&](int i, uint32_t byte, int key) {
         const int n = done + i, st = n & 1;
-        float* const kf = reinterpret_cast<float*>(smem + W::SCALES_AT + st * 2 * W_KEYS * 4);
-        float* const vf = kf + W_KEYS;
-        const uint32_t kb = mine & 0xffu, vb = mine >> 8 & 0xffu;
-        const uint32_t top = __reduce_max_sync(0xffffffffu, vb == 255 ? 0u : vb);
-        const bool nan_here = __any_sync(0xffffffffu, vb == 255);
-        if (lane == 0) {
-          tops[st][w] = static_cast<int>(top) | (nan_here ? 256 : 0);
-          mbar_arrive(told);
-        }
-        if (!mbar_wait_warp(told, n & 1, &gave_up)) return false;
-        const int t0 = tops[st][0], t1 = tops[st][1], t2 = tops[st][2], t3 = tops[st][3];
-        const int new_ref = max(ref, max(max(t0 & 255, t1 & 255), max(t2 & 255, t3 & 255)));
-        kf[key] = kb == 255 ? __int_as_float(0x7fc00000) : kv::power(kb);
-        vf[key] = vb == 255 ? __int_as_float(0x7fc00000) : kv::power(max(static_cast<int>(vb) - new_ref + 127, 0));
-        if (t == 0) {
-          info[st].nan_v = (t0 | t1 | t2 | t3) >> 8;
-          info[st].unit = i == 0 ? 1.f : ex2(static_cast<float>(ref - new_ref));
-          last_ref = new_ref;
-        }
-        ref = new_ref;
-        return true;
-      };
-      const auto codes_of = [&](int i) {
-        return reinterpret_cast<const uint4*>(smem + W::RAW_AT + (i - (tree ? 1 : 0) & 1) * W::K_BYTES) + t;
-      };
-      const auto make_k = [&](int i) {  // K and the scales of tile i
-        const int n = done + i;
-        if (!mbar_wait_warp(k_empty, (n & 1) ^ 1, &gave_up)) return false;
-        cp_async_wait<0>();  // the tile's codes are there (each thread copied its own)
-        const uint4* const codes = codes_of(i);
-#pragma unroll 4
-        for (int j = 0; j < PIECES; ++j) {
-          const int piece = j * 128 + t, row_key = piece / PIECES, c = piece % PIECES;
-          const uint4 u = codes[j * 128];
-          const uint32_t v[4] = {u.x, u.y, u.z, u.w};
-          uint32_t y[8];
-#pragma unroll
-          for (int x = 0; x < 4; ++x) kv::decode4<KIND>(v[x], y[2 * x], y[2 * x + 1]);
-          uint8_t* row = k_at + (c >> 2) * 16384 + row_key * 128;
-          const int chunk = (c & 3) * 2, swap = c >> 2 & 1;  // the two halves' lanes store in turn: no shared banks
-          const uint4 y0 = make_uint4(y[0], y[1], y[2], y[3]), y1 = make_uint4(y[4], y[5], y[6], y[7]);
-          *reinterpret_cast<uint4*>(row + ((chunk + swap) ^ (row_key & 7)) * 16) = swap ? y1 : y0;
-          *reinterpret_cast<uint4*>(row + ((chunk + 1 - swap) ^ (row_key & 7)) * 16) = swap ? y0 : y1;
-        }
-        if (!put_scales(i, scales, t)) return false;
-        fence_proxy_async_smem();
+        const uint32_t top = __reduce_max_sync(0xffffffffu, byte == 255 ? 0u : byte);
+        const bool nan_here = __any_sync(0xffffffffu, byte == 255);
+        bytes[side][st][key] = static_cast<uint8_t>(byte);
         __syncwarp();
-        if (lane == 0) mbar_arrive(&k_full[n & 1]);
+        if (lane == 0) {
+          tops[side][st][w] = static_cast<int>(top) | (nan_here ? 256 : 0);
+          mbar_arrive(&told[side]);
+        }
+        if (!mbar_wait_warp(&told[side], n & 1, &gave_up)) return false;
+        const int t0 = tops[side][st][0], t1 = tops[side][st][1], t2 = tops[side][st][2], t3 = tops[side][st][3];
+        const int most = max(max(t0 & 255, t1 & 255), max(t2 & 255, t3 & 255));
+        const int old = ref;
+        ref = side == 0 ? most : max(ref, most);
+        if (t == 0) {
+          if (side == 0) {
+            info[st].k_scale = kv::power(ref);
+          } else {
+            info[st].nan_v = (t0 | t1 | t2 | t3) >> 8;
+            info[st].unit = i == 0 ? 1.f : ex2(static_cast<float>(old - ref));
+            last_ref = ref;
+          }
+        }
+        if (side == 1) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&v_known[st]);
+        }
         return true;
       };
-      if (tree) {  // the first tile: the nodes' own keys and values
-        ok = mbar_wait_warp(k_empty, (done & 1) ^ 1, &gave_up) && mbar_wait_warp(v_empty, (done & 1) ^ 1, &gave_up);
-        if (ok) {
-          uint32_t mine;
-          int key;
-          // thread t: half the dimensions of node t / 2; a row's largest is brought to [64, 128), the codes' range
-          const int node = t >> 1, d0 = (t & 1) * (D / 2);
-          const bool here = node < p.nodes;
-          uint32_t bytes[2];
+      for (int i = 0; i < tiles && ok; ++i) {
+        const int n = done + i, st = n & 1, cached = i - (tree ? 1 : 0);
+        if (cached < 0) {
+          uint32_t top = 0;
 #pragma unroll
-          for (int kv = 0; kv < 2; ++kv) {
-            const __nv_bfloat16* from = kv == 0 ? p.k + b * p.k_seq + node * p.k_node + h * p.k_head + d0
-                                                : p.v + b * p.v_seq + node * p.v_node + h * p.v_head + d0;
-            uint4 x[D / 16];
-            uint32_t top = 0;
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t v[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
 #pragma unroll
-            for (int c = 0; c < D / 16; ++c) {
-              x[c] = here ? __ldg(reinterpret_cast<const uint4*>(from) + c) : make_uint4(0, 0, 0, 0);
-              uint32_t* v = reinterpret_cast<uint32_t*>(&x[c]);
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < 4; ++j) {
+              if (side == 1) {  // V: what is not finite is left out here and put in at the end
 #pragma unroll
                 for (int sh = 0; sh < 32; sh += 16)
-                  if ((v[j] >> sh & 0x7f80u) == 0x7f80u && kv == 1) {  // V: left out here, put in at the end
+                  if ((v[j] >> sh & 0x7f80u) == 0x7f80u) {
                     v[j] &= ~(0xffffu << sh);
                     atomicOr(&special[node >> 5], 1u << (node & 31));
                   }
-#pragma unroll
-              for (int j = 0; j < 4; ++j) top = max(top, max(v[j] & 0x7fffu, v[j] >> 16 & 0x7fffu));
+              }
+              top = max(top, max(v[j] & 0x7fffu, v[j] >> 16 & 0x7fffu));
             }
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            int e = static_cast<int>(top >> 7);
-            e = e == 255 || e < 1 ? 127 : e < 67 ? 67 : e > 247 ? 247 : e;
-            const float f = kv::power(254 - e + 6);
-            bytes[kv] = e - 6;
+            x[c] = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+          top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          int e = static_cast<int>(top >> 7);
+          e = e == 255 || e < 1 ? 127 : e < 67 ? 67 : e > 247 ? 247 : e;
+          // the largest of all is brought to [64, 128), the codes' range; a node's first thread tells its scale, the
+          // second that of an empty key past the nodes
+          ok = hear(i, t & 1 || !here ? 1 : e - 6, node + (t & 1) * 64);
+          ok = ok && mbar_wait_warp(side == 0 ? k_empty : v_empty, (n & 1) ^ 1, &gave_up);
+          if (!ok) break;
+          const float f = kv::power(254 - ref);
 #pragma unroll
-            for (int c = 0; c < D / 16; ++c) {
-              const uint32_t v[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
-              uint32_t y[4];
+          for (int c = 0; c < D / 16; ++c) {
+            const uint32_t v[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+            uint32_t y[4];
 #pragma unroll
-              for (int j = 0; j < 4; ++j) y[j] = pack_f16(low_f(v[j]) * f, high_f(v[j]) * f);
-              const int d = d0 + c * 8;
-              if (kv == 0) {
-                const int at16 = (d >> 6) * 16384 + ((d >> 3 & 7) ^ (node & 7)) * 16;
-                *reinterpret_cast<uint4*>(k_at + at16 + node * 128) = make_uint4(y[0], y[1], y[2], y[3]);
-                *reinterpret_cast<uint4*>(k_at + at16 + (node + 64) * 128) = make_uint4(0, 0, 0, 0);
-              } else {
+            for (int j = 0; j < 4; ++j) y[j] = pack_f16(low_f(v[j]) * f, high_f(v[j]) * f);
+            const int d = d0 + c * 8;
+            if (side == 0) {
+              uint8_t* const at = out + (d >> 6) * 16384 + ((d >> 3 & 7) ^ (node & 7)) * 16;
+              *reinterpret_cast<uint4*>(at + node * 128) = make_uint4(y[0], y[1], y[2], y[3]);
+              *reinterpret_cast<uint4*>(at + (node + 64) * 128) = make_uint4(0, 0, 0, 0);
+            } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                  const int row = d + j, chunk = (node >> 3) ^ (row & 7);
-                  *reinterpret_cast<unsigned short*>(v_at + row * 128 + chunk * 16 + (node & 7) * 2) =
-                      static_cast<unsigned short>(y[j >> 1] >> (16 * (j & 1)));
+              for (int j = 0; j < 8; ++j) {
+                const int row = d + j, chunk = (node >> 3) ^ (row & 7);
+                *reinterpret_cast<unsigned short*>(out + row * 128 + chunk * 16 + (node & 7) * 2) =
+                    static_cast<unsigned short>(y[j >> 1] >> (16 * (j & 1)));
+              }
+              *reinterpret_cast<uint4*>(out + D * 128 + (t * (D / 16) + c) * 16) = make_uint4(0, 0, 0, 0);  // keys 64 on
+            }
+          }
+        } else {
+          if (cached == 0) {  // (the second tile's copies follow the first's)
+            fetch();
+            cp_async_commit();
+          }
+          ok = hear(i, scale, t);
+          ok = ok && mbar_wait_warp(side == 0 ? k_empty : v_empty, (n & 1) ^ 1, &gave_up);
+          if (!ok) break;
+          cp_async_wait<1>();  // the tile's codes are there (each thread copied its own)
+          const uint4* const codes =
+              reinterpret_cast<const uint4*>(smem + raw_at + (cached & 1) * (W::K_BYTES / 2));
+          if (side == 0) {
+#pragma unroll 4
+            for (int j = 0; j < PIECES; ++j) {
+              const int piece = j * 128 + t, key = piece / PIECES, c = piece % PIECES;
+              const int byte = bytes[0][st][key];
+              const __half2 f = byte == 255 ? __half2half2(__ushort_as_half(0x7e00)) : relative(byte, ref);  // (NaN)
+              const uint4 u = codes[j * 128];
+              const uint32_t v[4] = {u.x, u.y, u.z, u.w};
+              uint32_t y[8];
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                kv::decode4<KIND>(v[x], y[2 * x], y[2 * x + 1]);
+                y[2 * x] = times(y[2 * x], f), y[2 * x + 1] = times(y[2 * x + 1], f);
+              }
+              uint8_t* const row = out + (c >> 2) * 16384 + key * 128;
+              const int chunk = (c & 3) * 2, swap = c >> 2 & 1;  // the two halves' lanes store in turn: no shared banks
+              const uint4 y0 = make_uint4(y[0], y[1], y[2], y[3]), y1 = make_uint4(y[4], y[5], y[6], y[7]);
+              *reinterpret_cast<uint4*>(row + ((chunk + swap) ^ (key & 7)) * 16) = swap ? y1 : y0;
+              *reinterpret_cast<uint4*>(row + ((chunk + 1 - swap) ^ (key & 7)) * 16) = swap ? y0 : y1;
+            }
+          } else {
+            const int key0 = key_lo + cached * W_KEYS, quad = lane & 15;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const int left = len - key0 - (half * 16 + quad) * 4;  // keys of the quad that are there
+              const uint32_t keep = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : 0xffffffffu >> (32 - 8 * left);
+              const uint32_t four = *reinterpret_cast<const uint32_t*>(&bytes[1][st][half * 64 + quad * 4]);
+              __half2 f[2];
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const int b0 = four >> (16 * j) & 255, b1 = four >> (16 * j + 8) & 255;
+                const __half2 f0 = relative(b0 == 255 ? 0 : b0, ref), f1 = relative(b1 == 255 ? 0 : b1, ref);
+                f[j] = __halves2half2(b0 == 255 ? __ushort_as_half(0) : __low2half(f0),
+                                      b1 == 255 ? __ushort_as_half(0) : __low2half(f1));
+              }
+#pragma unroll 4
+              for (int j = 0; j < PIECES / 2; ++j) {
+                const int x = 2 * (w * (PIECES / 2) + j) + (lane >> 4);
+                const uint4 u = codes[(half * (PIECES / 2) + j) * 128];
+                const uint32_t v[4] = {u.x & keep, u.y & keep, u.z & keep, u.w & keep};
+#pragma unroll
+                for (int d4 = 0; d4 < 4; ++d4) {
+                  const int d = x * 4 + d4;
+                  uint2 y;
+                  kv::decode4<KIND>(v[d4], y.x, y.y);
+                  y.x = times(y.x, f[0]), y.y = times(y.y, f[1]);
+                  *reinterpret_cast<uint2*>(out + half * D * 128 + d * 128 + ((quad >> 1) ^ (d & 7)) * 16 + (quad & 1) * 8) = y;
                 }
-                *reinterpret_cast<uint4*>(v_at + D * 128 + (t * (D / 16) + c) * 16) = make_uint4(0, 0, 0, 0);  // keys 64 on
               }
             }
-          }
-          // a node's first thread has its scales, the second those of an empty key past the nodes
-          mine = t & 1 || !here ? 1 | 1 << 8 : bytes[0] | bytes[1] << 8;
-          key = node + (t & 1) * 64;
-          ok = put_scales(0, mine, key);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (ok && lane == 0) {
-            mbar_arrive(&k_full[done & 1]);
-            mbar_arrive(v_full);
-          }
-        }
-      }
-      if (ok && tiles > (tree ? 1 : 0)) ok = make_k(tree ? 1 : 0);
-      scales = next_scales;
-      for (int i = tree ? 1 : 0; i < tiles && ok; ++i) {
-        const int n = done + i, key0 = key_lo + (i - (tree ? 1 : 0)) * W_KEYS;
-        ok = mbar_wait_warp(v_empty, (n & 1) ^ 1, &gave_up);
-        if (!ok) break;
-        const uint4* const codes = codes_of(i);
-#pragma unroll 4
-        for (int j = 0; j < PIECES; ++j) {
-          const int half = j / (PIECES / 2), quad = lane & 15;
-          const int x = 2 * (w * (PIECES / 2) + j % (PIECES / 2)) + (lane >> 4);
-          const int left = len - key0 - (half * 16 + quad) * 4;  // keys of the quad that are there
-          const uint32_t keep = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : 0xffffffffu >> (32 - 8 * left);
-          const uint4 u = codes[(PIECES + j) * 128];
-          const uint32_t v[4] = {u.x & keep, u.y & keep, u.z & keep, u.w & keep};
-#pragma unroll
-          for (int d4 = 0; d4 < 4; ++d4) {
-            const int d = x * 4 + d4;
-            uint2 y;
-            kv::decode4<KIND>(v[d4], y.x, y.y);
-            *reinterpret_cast<uint2*>(v_at + half * D * 128 + d * 128 + ((quad >> 1) ^ (d & 7)) * 16 + (quad & 1) * 8) = y;
           }
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(v_full);
-        if (i + 1 < tiles) ok = make_k(i + 1);  // before the next copies: S waits for it
-        fetch();
-        cp_async_commit();
-        scales = next_scales;
+        if (lane == 0) mbar_arrive(side == 0 ? &k_full[st] : v_full);
+        if (cached >= 0) {
+          fetch();
+          cp_async_commit();
+        }
       }
       cp_async_wait<0>();
     } else {
@@ -620,7 +644,7 @@ __global__ void __launch_bounds__(W_NT, 1) wide_kernel(const Params p) {
     if (gave_up) break;
   }
   if (gave_up) {  // products may still be under way: their memory is freed after a bounded wait for them
-    if (warp == 12) {
+    if (warp == 16) {
       if (elect_one()) tc_commit(o_full);
       const uint64_t from = global_ns();
       while (global_ns() - from < 1000000) {
@@ -631,7 +655,7 @@ __global__ void __launch_bounds__(W_NT, 1) wide_kernel(const Params p) {
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 12) tmem_dealloc(tmem, 512);
+  if (warp == 16) tmem_dealloc(tmem, 512);
 }
 
 }  // namespace tree

@@ -276,11 +276,13 @@ def _random_tree(n, g):
     return parents
 
 
-def _check(got, q, k, v, past, plan, window=-1, scale=None):
+def _check(got, q, k, v, past, plan, window=-1, scale=None, lost=None):
     for b, (mask, depth) in enumerate(plan):
         ref, a = oracle.tree_attention(q[b].cpu(), k[b].cpu(), v[b].cpu(), *past[b], mask, depth, window, scale)
         err = (got[b].cpu().double() - ref).abs()
         assert torch.isfinite(got[b]).all()
+        if lost is not None:
+            err -= lost[b]
         assert (err <= 2.0 ** -8 * ref.abs() + (2.0 ** -8 + 2.0 ** -12) * a).all(), (b, (err / (a + 1e-30)).max().item())
 
 
@@ -624,3 +626,184 @@ def test_refusals():
         with pytest.raises(kind):
             call()
     cache.check()
+
+
+# ---- tree attention with more than 128 rows a key head (8-bit caches whose tables have room) --------------------
+
+
+def _roomy(table, page, heads):
+    """The table with room for 2^17 keys of all heads; its new entries name no page."""
+    width = -(-2 ** 17 // (len(table) * page * heads))
+    return torch.nn.functional.pad(table, (0, max(0, width - table.shape[1])), value=-7)
+
+
+@pytest.mark.parametrize('kind', ['e4m3', 'int8'])
+@pytest.mark.parametrize('dim', [64, 128])
+@pytest.mark.parametrize('nodes,heads,group,page,window', [
+    (64, 1, 4, 16, -1), (33, 1, 8, 64, 64), (3, 2, 64, 128, 0), (43, 1, 3, 32, 30), (64, 2, 64, 64, 5),
+    (17, 1, 8, 16, 200)])
+def test_wide_tree_attention(kind, dim, nodes, heads, group, page, window):
+    """From 129 rows to 16 tiles of them, several items a CTA, lengths from none to several tiles of keys."""
+    from noise_b200 import decode
+    g = _gen(nodes * dim + group + 1)
+    lens = [0, 1, 15, 127, 128, 129, 255, 256, 257, 383, 700]
+    cache, table = _cache(kind, dim, heads, page, len(lens), 768, seed=nodes)
+    past, table = _fill(cache, table, lens, g), _roomy(table, page, heads)
+    parents = torch.tensor([_random_tree(nodes, g) for _ in lens], dtype=torch.int32, device=DEV)
+    mask, depth = decode.tree_plan(parents)
+    plan = [oracle.tree_plan(p) for p in parents.tolist()]
+    qkv = torch.randn(len(lens), nodes, heads * (group + 2), dim, generator=g).to(torch.bfloat16).to(DEV)
+    q, k, v = qkv[:, :, :heads * group] * 2, qkv[:, :, heads * group:-heads], qkv[:, :, -heads:]
+    lengths = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    got = decode.tree_attention(q, k, v, cache, table, lengths, mask, depth, window=window)
+    _check(got, q, k, v, past, plan, window)
+    assert torch.equal(got, decode.tree_attention(q, k, v, cache, table, lengths, mask, depth, window=window))
+    cache.check()
+
+
+@pytest.mark.parametrize('dim', [64, 128])
+def test_wide_tree_attention_long(dim):
+    """Items split over many CTAs and joined, in the last layer, on another stream; a scale that leaves one key."""
+    from noise_b200 import decode
+    g = _gen(dim)
+    cache, table = _cache('int8', dim, 2, 64, 3, 9000, layers=2)
+    lens = [8999, 0, 4500]
+    last = decode.KVCache.of(cache.k[1:], cache.v[1:], cache.k_scale[1:], cache.v_scale[1:])
+    past, table = _fill(last, table, lens, g), _roomy(table, 64, 2)
+    q, k, v = (torch.randn(3, 3, h, dim, generator=g).to(torch.bfloat16).to(DEV) for h in (128, 2, 2))
+    parents = [[-1, 0, 0]] * 3
+    mask, depth = decode.tree_plan(torch.tensor(parents, dtype=torch.int32, device=DEV))
+    lengths = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    plan = [oracle.tree_plan(p) for p in parents]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for scale in (None, 4.0):
+            got = decode.tree_attention(q, k, v, cache, table, lengths, mask, depth, layer=1, scale=scale)
+            side.synchronize()
+            # what fp16 probabilities cannot hold: below 2^-24 of the largest they round to 2^-25 or are lost
+            lost = []
+            for b in range(3):
+                kk, vv = (torch.cat([x, y[b].cpu().float()]).double() for x, y in zip(past[b], (k, v)))
+                s = torch.einsum('nhgd,khd->nhgk', q[b].cpu().double().view(3, 2, 64, dim), kk)
+                s *= dim ** -0.5 if scale is None else scale
+                if lens[b]:  # of no less than the row's own sum: all keys over that of the cached ones
+                    p = (s - s[..., :lens[b]].logsumexp(-1, keepdim=True)).exp().clamp(max=2.0 ** -25)
+                    lost.append(torch.einsum('nhgk,khd->nhgd', p, vv.abs()).reshape(3, 128, dim))
+                else:
+                    lost.append(torch.zeros(3, 128, dim, dtype=torch.float64))
+            _check(got, q, k, v, past, plan, scale=scale, lost=lost)
+
+
+@pytest.mark.parametrize('kind', ['e4m3', 'int8'])
+def test_wide_tree_attention_ignores_what_is_masked(kind):
+    """NaN and infinities past the end, before the window, in padding nodes and in branches not seen."""
+    from noise_b200 import decode
+    g = _gen(12)
+    cache, table = _cache(kind, 64, 1, 16, 3, 400)
+    lens, window = [333, 190, 7], 140
+    past = _fill(cache, table, lens, g)
+    every = torch.arange(400, dtype=torch.int32, device=DEV)
+    for b, n in enumerate(lens):
+        at = torch.cat([every[n:], every[:max(0, n - window - 1)]])
+        junk = torch.full((len(at), 1, 64), math.nan, device=DEV)
+        junk[::2] = math.inf
+        cache.write(junk, junk, torch.full_like(at, b), at, table)
+    page = table[2, 1]
+    cache.k.view(torch.uint8)[:, page] = 0x7f
+    cache.v.view(torch.uint8)[:, page] = 0xff
+    cache.v_scale[:, page] = 254
+    room = _roomy(table, 16, 1)
+    parents = [[-1, 0, 0, 1, -2, 2, 5, 6]] * 3
+    plan = [oracle.tree_plan(p) for p in parents]
+    mask, depth = decode.tree_plan(torch.tensor(parents, dtype=torch.int32, device=DEV))
+    q, k, v = (torch.randn(3, 8, h, 64, generator=g).to(torch.bfloat16) for h in (32, 1, 1))
+    k[:, 4], v[:, 4] = math.nan, math.inf
+    lengths = torch.tensor(lens, dtype=torch.int32, device=DEV)
+
+    def attend(values):
+        return decode.tree_attention(q.to(DEV), k.to(DEV), values.to(DEV), cache, room, lengths, mask, depth,
+                                     window=window)
+    got = attend(v)
+    _check(got, q, k, v, past, plan, window)
+    v2 = v.clone()
+    v2[:, 1, 0, 5], v2[:, 3, 0, 9] = math.nan, -math.inf
+    got2 = attend(v2)
+    same = torch.ones_like(got, dtype=torch.bool)
+    same[:, [1, 3], :, 5] = same[:, 3, :, 9] = False
+    # (fp16 steps are relative to the largest scale among a tile's keys: a last place may move)
+    assert torch.allclose(got[same].float(), got2[same].float(), rtol=2.0 ** -7, atol=2.0 ** -9)
+    assert torch.isnan(got2[:, [1, 3], :, 5]).all() and (got2[:, 3, :, 9] == -math.inf).all()
+    at = torch.tensor([lens[0] - window], dtype=torch.int32, device=DEV)  # the root sees it, its children do not
+    bad = torch.full((1, 1, 64), math.nan, device=DEV)
+    cache.write(torch.zeros_like(bad), bad, torch.zeros_like(at), at, table)
+    got3 = attend(v)
+    assert torch.isnan(got3[0, 0]).all() and torch.equal(got3[1:], got[1:])
+    assert torch.allclose(got3[0, 1:].float(), got[0, 1:].float(), rtol=2.0 ** -7, atol=2.0 ** -9)
+
+
+def test_wide_tree_attention_rows_that_see_nothing():
+    from noise_b200 import decode
+    cache, table = _cache('e4m3', 64, 1, 16, 2, 32)
+    q, k, v = (torch.randn(2, 3, h, 64, generator=_gen(h)).to(torch.bfloat16).to(DEV) for h in (64, 1, 1))
+    mask = torch.tensor([[0, 2, 0], [1, 0, 4]], device=DEV)
+    depth = torch.tensor([[0, 0, -1], [0, 0, -1]], dtype=torch.int32, device=DEV)
+    got = decode.tree_attention(q, k, v, cache, _roomy(table, 16, 1),
+                                torch.tensor([0, -5], dtype=torch.int32, device=DEV), mask, depth)
+    assert (got[0, 0] == 0).all() and (got[1, 1] == 0).all() and (got[:, 2] == 0).all()
+    assert torch.equal(got[0, 1], v[0, 1].expand(64, 64)) and torch.equal(got[1, 0], v[1, 0].expand(64, 64))
+
+
+def test_wide_tree_attention_bad_page():
+    from noise_b200 import decode
+    from noise_b200._lib import NoiseError
+    cache, table = _cache('int8', 64, 1, 16, 3, 512)
+    q, k, v = (torch.randn(3, 3, h, 64, generator=_gen(h)).to(torch.bfloat16).to(DEV) for h in (64, 1, 1))
+    mask, depth = decode.tree_plan(torch.tensor([[-1, 0, 1]] * 3, dtype=torch.int32, device=DEV))
+    table[1, 20] = cache.k.shape[1]
+    lengths = torch.tensor([512] * 3, dtype=torch.int32, device=DEV)
+    got = decode.tree_attention(q, k, v, cache, _roomy(table, 16, 1), lengths, mask, depth)
+    assert torch.isfinite(got[[0, 2]]).all() and torch.isnan(got[1]).all()
+    with pytest.raises(NoiseError, match='out of range'):
+        cache.check()
+
+
+@pytest.mark.parametrize('kind', ['e4m3', 'int8'])
+@pytest.mark.parametrize('size', [2.0 ** -60, 2.0 ** 60])
+def test_wide_tree_attention_sizes_of_values(kind, size):
+    from noise_b200 import decode
+    g = _gen(3)
+    cache, table = _cache(kind, 64, 1, 16, 1, 320)
+    k, v = (torch.randn(300, 1, 64, generator=g).to(torch.bfloat16).to(DEV) for _ in range(2))
+    seq, pos = torch.zeros(300, dtype=torch.int32, device=DEV), torch.arange(300, dtype=torch.int32, device=DEV)
+    qt, kt, vt = (torch.randn(1, 3, h, 64, generator=g).to(torch.bfloat16).to(DEV) for h in (64, 1, 1))
+    mask, depth = decode.tree_plan(torch.tensor([[-1, 0, 0]], dtype=torch.int32, device=DEV))
+    lengths, room = torch.tensor([300], dtype=torch.int32, device=DEV), _roomy(table, 16, 1)
+    for vs, qs in ((max(size, 2.0 ** -12), 1.0), (1.0, min(size, 2.0 ** 40))):
+        cache.write(k / qs, v * vs, seq, pos, table)
+        past = [x.cpu() for x in cache.read(seq, pos, table, dtype=torch.float32)]
+        got = decode.tree_attention(qt * qs, kt / qs, vt * vs, cache, room, lengths, mask, depth)
+        _check(got, qt * qs, kt / qs, vt * vs, [past], [oracle.tree_plan([-1, 0, 0])])
+
+
+@pytest.mark.parametrize('kind', ['bf16', 'e4m3', 'int8'])
+@pytest.mark.parametrize('group', [2, 40])
+def test_large_values_where_no_row_looks(kind, group):
+    """Keys and values of 1e30 past the end, before every window and in padding cost the others no precision."""
+    from noise_b200 import decode
+    g = _gen(group)
+    cache, table = _cache(kind, 64, 1, 16, 3, 400)
+    lens, window = [333, 190, 7], 140
+    past = _fill(cache, table, lens, g)
+    every = torch.arange(400, dtype=torch.int32, device=DEV)
+    for b, n in enumerate(lens):
+        at = torch.cat([every[n:], every[:max(0, n - window)]])
+        junk = torch.full((len(at), 1, 64), 1e30, device=DEV)
+        cache.write(junk, junk, torch.full_like(at, b), at, table)
+    parents = [[-1, 0, -2, 1, 0]] * 3
+    mask, depth = decode.tree_plan(torch.tensor(parents, dtype=torch.int32, device=DEV))
+    q, k, v = (torch.randn(3, 5, h, 64, generator=g).to(torch.bfloat16).to(DEV) for h in (group, 1, 1))
+    k[:, 2] = v[:, 2] = 1e30
+    got = decode.tree_attention(q, k, v, cache, _roomy(table, 16, 1),
+                                torch.tensor(lens, dtype=torch.int32, device=DEV), mask, depth, window=window)
+    _check(got, q, k, v, past, [oracle.tree_plan(p) for p in parents], window)
