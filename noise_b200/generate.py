@@ -1,0 +1,195 @@
+"""Text from the trained GPT, several tokens a step: the operators of noise_b200.decode run together.
+
+The reference's model is only ever trained (GPT.forward, utils/model.py:193-209); ``Generator`` runs the same blocks on
+a paged cache. A prompt goes in as chains of up to 64 tokens. Then each step takes the last token and a tree of drafts
+under it (by default what followed the same two tokens earlier in the sequence) through the blocks once, and
+``verify_tree`` keeps the drafts that the model itself would have sampled, so the text is distributed as if it were
+made token by token.
+
+    gen = Generator(params, kind='int8')  # params: name -> tensor, as noise_b200.eggroll.make_params
+    tokens = gen.generate([[1, 2, 3], [4, 5]], new_tokens=100, temperature=0.8)
+
+``python -m noise_b200.generate`` runs it on fresh weights with and without drafts.
+"""
+import argparse
+import time
+
+import torch
+from torch.nn import functional as F
+
+from . import _lib
+from .decode import KVCache, head_norm_rope, tree_attention, tree_plan, verify_tree
+from .population import HEAD_DIM, N_EMBD, N_HEAD, N_LAYER, VOCAB, WINDOWS, has_ve, param_shapes, rotary_tables
+
+SOFTCAP = 15.0  # utils/model.py:205
+CHAIN = 64      # tokens of a prompt a pass
+
+
+def repeated(history, length, branches=4, back=1024):
+    """What followed the last two tokens where they stood before in ``history``: up to ``branches`` continuations of up
+    to ``length`` tokens, the latest first."""
+    out = []
+    for i in range(len(history) - 3, max(-1, len(history) - back), -1):
+        if history[i:i + 2] == history[-2:]:
+            out.append(history[i + 2:i + 2 + length])
+            if len(out) == branches:
+                break
+    return out
+
+
+def grow(root, drafts, nodes):
+    """(tokens, parents) of ``nodes`` nodes: continuations merged into one tree under ``root``, padded with -2."""
+    tokens, parents, child = [root], [-1], {}
+    for draft in drafts:
+        at = 0
+        for t in draft:
+            if (at, t) not in child:
+                if len(tokens) == nodes:
+                    break
+                child[at, t] = len(tokens)
+                tokens.append(t)
+                parents.append(at)
+            at = child[at, t]
+    pad = nodes - len(tokens)
+    return tokens + [0] * pad, parents + [-2] * pad
+
+
+class Generator:
+    """The GPT of ``params`` (name -> tensor, utils/model.py's names) with its weights in bf16, as autocast has them."""
+
+    def __init__(self, params, kind='int8', page_size=64, device='cuda'):
+        for name, shape in param_shapes():
+            if name not in params or tuple(params[name].shape) != shape:
+                raise ValueError(f'{name}: a tensor {shape}')
+        w = {n: t.detach().to(device) for n, t in params.items()}
+        self.device, self.kind, self.page_size = torch.device(device), kind, page_size
+        self.lambdas = list(zip(w['resid_lambdas'].tolist(), w['x0_lambdas'].tolist()))
+        self.wte, self.head = w['transformer.wte.weight'].float(), w['lm_head.weight'].bfloat16()
+        self.blocks = []
+        for i in range(N_LAYER):
+            pre = f'transformer.h.{i}.'
+            qkv = torch.cat([w[pre + f'attn.{n}.weight'] for n in ('c_q', 'c_k', 'c_v')]).bfloat16()
+            rest = [w[pre + f'{n}.weight'].bfloat16() for n in ('attn.c_proj', 'mlp.c_fc', 'mlp.c_proj')]
+            values = (w[f'value_embeds.{i}.weight'].bfloat16(),
+                      w[pre + 'attn.ve_gate.weight'].bfloat16()) if has_ve(i) else None
+            self.blocks.append((qkv, *rest, values))
+
+    def _forward(self, tokens, parents, lengths, table, cache, cos, sin):
+        """Logits fp32 [B, N, V] (before the softcap) at every node, and the nodes' keys and values of all layers."""
+        b, n = tokens.shape
+        mask, depth = tree_plan(parents)
+        positions = (lengths[:, None] + depth).clamp_(min=0).view(-1)
+        tokens = tokens.view(-1)
+        x = x0 = F.rms_norm(self.wte[tokens], (N_EMBD,))
+        keys = torch.empty(N_LAYER, b * n, N_HEAD, HEAD_DIM, dtype=torch.bfloat16, device=self.device)
+        values = torch.empty_like(keys)
+        for i, (qkv, c_proj, c_fc, m_proj, ve) in enumerate(self.blocks):
+            x = self.lambdas[i][0] * x + self.lambdas[i][1] * x0
+            h = F.rms_norm(x, (N_EMBD,)).bfloat16()
+            q, k, v = _lib.gemm_bf16_tn(h, qkv).bfloat16().view(b * n, 3, N_HEAD, HEAD_DIM).unbind(1)
+            if ve is not None:  # utils/model.py:87-90
+                gate = 2 * torch.sigmoid((h[:, None, :ve[1].shape[1]].float() * ve[1].float()).sum(-1))
+                v = v + (gate[..., None] * ve[0][tokens].view(b * n, N_HEAD, HEAD_DIM)).bfloat16()
+            q, k = head_norm_rope(q, k, cos, sin, positions)
+            keys[i], values[i] = k, v
+            y = tree_attention(q.view(b, n, N_HEAD, HEAD_DIM), k.view(b, n, N_HEAD, HEAD_DIM),
+                               values[i].view(b, n, N_HEAD, HEAD_DIM), cache, table, lengths, mask, depth, layer=i,
+                               window=WINDOWS[i])
+            x = x + _lib.gemm_bf16_tn(y.view(b * n, N_EMBD), c_proj)
+            h = _lib.gemm_bf16_tn(F.rms_norm(x, (N_EMBD,)).bfloat16(), c_fc)
+            x = x + _lib.gemm_bf16_tn(F.relu(h).square().bfloat16(), m_proj)
+        logits = _lib.gemm_bf16_tn(F.rms_norm(x, (N_EMBD,)).bfloat16(), self.head)
+        return logits.view(b, n, VOCAB), keys, values
+
+    def _keep(self, cache, keys, values, path, lengths, table):
+        """The keys and values of the nodes in ``path`` [B, N] (-1: none) written at lengths[b] on, in all layers."""
+        b, n = path.shape
+        seq = torch.arange(b, dtype=torch.int32, device=self.device)[:, None].expand(b, n)
+        pos = lengths[:, None] + torch.arange(n, dtype=torch.int32, device=self.device)
+        rows = torch.where(path < 0, -1, path + seq * n)
+        cache.write(keys, values, seq.contiguous().view(-1), pos.view(-1), table, layer=None, rows=rows.view(-1))
+
+    @torch.no_grad()
+    def generate(self, prompts, new_tokens, temperature=0.0, nodes=16, draft=repeated, seed=0):
+        """``new_tokens`` tokens after each of ``prompts`` (lists of ids, none empty) as lists. nodes: of a step's tree,
+        the last token among them (1: token by token, at most 64); draft(history, length): lists of tokens that may
+        come next. Afterwards ``steps`` is the number of steps and ``accepted`` that of the drafts they kept."""
+        if not 1 <= nodes <= 64:
+            raise ValueError(f'nodes: 1 to 64, got {nodes}')
+        if new_tokens < 0:
+            raise ValueError(f'new_tokens: 0 or more, got {new_tokens}')
+        for p in prompts:
+            if len(p) == 0 or min(p) < 0 or max(p) >= VOCAB:
+                raise ValueError(f'prompts: one or more ids from 0 to {VOCAB - 1} each')
+        self.steps = self.accepted = 0
+        if not prompts or new_tokens == 0:
+            return [[] for _ in prompts]
+        b, dev = len(prompts), self.device
+        room = max(map(len, prompts)) + new_tokens + max(nodes, CHAIN)
+        width = -(-room // self.page_size)
+        cache = KVCache(N_LAYER, b * width, N_HEAD, HEAD_DIM, self.kind, self.page_size, dev)
+        table = torch.arange(b * width, dtype=torch.int32, device=dev).view(b, width)
+        cos, sin = rotary_tables(room, dev)
+        lengths = torch.zeros(b, dtype=torch.int32, device=dev)
+        for at in range(0, max(map(len, prompts)) - 1, CHAIN):  # all but the last token, which is the first root
+            part = [p[at:min(at + CHAIN, len(p) - 1)] for p in prompts]
+            n = max(map(len, part))
+            tokens = torch.tensor([p + [0] * (n - len(p)) for p in part], device=dev)
+            parents = torch.tensor([[i - 1 if i < len(p) else -2 for i in range(n)] for p in part], dtype=torch.int32,
+                                   device=dev)
+            _, keys, values = self._forward(tokens, parents, lengths, table, cache, cos, sin)
+            path = torch.tensor([[i if i < len(p) else -1 for i in range(n)] for p in part], dtype=torch.int32,
+                                device=dev)
+            self._keep(cache, keys, values, path, lengths, table)
+            lengths += torch.tensor([len(p) for p in part], dtype=torch.int32, device=dev)
+        history, want = [list(p) for p in prompts], [len(p) + new_tokens for p in prompts]
+        g = torch.Generator(dev).manual_seed(seed)
+        while True:
+            busy = [len(h) < w for h, w in zip(history, want)]
+            if not any(busy):
+                break
+            trees = [grow(h[-1], draft(h, nodes - 1) if nodes > 1 and go else [], nodes)
+                     for h, go in zip(history, busy)]
+            tokens = torch.tensor([t for t, _ in trees], device=dev)
+            parents = torch.tensor([p for _, p in trees], dtype=torch.int32, device=dev)
+            logits, keys, values = self._forward(tokens, parents, lengths, table, cache, cos, sin)
+            u = torch.rand(b, nodes, device=dev, generator=g)
+            race = torch.empty(b, VOCAB, device=dev).exponential_(generator=g)
+            count, path, token = verify_tree(logits, tokens, parents, u, race, temperature=temperature, softcap=SOFTCAP)
+            go = torch.tensor(busy, device=dev)
+            self._keep(cache, keys, values, torch.where(go[:, None], path, -1), lengths, table)
+            lengths += torch.where(go, count + 1, 0)
+            self.steps += 1
+            for i, (c, p, t) in enumerate(zip(count.tolist(), path.tolist(), token.tolist())):
+                if busy[i]:
+                    if t < 0:
+                        raise FloatingPointError(f'sequence {i}: the logits name no token')
+                    history[i] += [trees[i][0][j] for j in p[1:c + 1]] + [t]
+                    self.accepted += c
+        cache.check()
+        return [h[len(p):w] for h, p, w in zip(history, prompts, want)]
+
+
+def main():
+    from .eggroll import make_params
+    parser = argparse.ArgumentParser(description=__doc__.split('\n')[0])
+    parser.add_argument('--kind', default='int8', choices=['bf16', 'e4m3', 'int8'], help='of the cache')
+    parser.add_argument('--sequences', type=int, default=8)
+    parser.add_argument('--prompt', type=int, default=512, help='tokens of each prompt')
+    parser.add_argument('--tokens', type=int, default=256, help='to be made for each')
+    parser.add_argument('--temperature', type=float, default=0.0)
+    args = parser.parse_args()
+    gen = Generator(make_params('cuda'), args.kind)
+    g = torch.Generator().manual_seed(0)
+    prompts = torch.randint(0, VOCAB, (args.sequences, args.prompt), generator=g).tolist()
+    for nodes in (1, 16):
+        gen.generate(prompts, 2, args.temperature, nodes)
+        start = time.perf_counter()
+        gen.generate(prompts, args.tokens, args.temperature, nodes)
+        seconds = time.perf_counter() - start
+        print(f'{nodes:2d} nodes a step: {gen.steps} steps, {gen.accepted} drafts accepted, '
+              f'{args.sequences * args.tokens / seconds:.0f} tokens/s with the prompts')
+
+
+if __name__ == '__main__':
+    main()

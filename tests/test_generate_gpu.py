@@ -1,0 +1,75 @@
+"""The GPT's text on the paged cache: every greedy token is the full forward's, drafts change nothing but the steps."""
+import pytest
+import torch
+
+from oracle import gpt as oracle
+
+pytestmark = pytest.mark.gpu
+
+
+def _prompts():
+    rows = oracle.zipf_tokens(3, 150, seed=3).tolist()
+    return [rows[0], rows[1][:1], rows[2][:65]]
+
+
+def _check_greedy(w, prompts, texts):
+    """Each token's logit in the oracle's fp32 forward is within 0.17 of the row's spread of the largest.
+
+    Some 48 roundings to bf16 (relative 2^-9 each, 6 a block) move a logit by about sqrt(48) 2^-9 = 1.4% of the spread,
+    an int8 cache by 2^-7 of its rows' largest, about 2%: 5 sigma of the difference of two such logits is
+    5 sqrt(2) 2.4% = 17% at most. A token that owes nothing to the model stands 3.5 spreads below."""
+    for p, t in zip(prompts, texts):
+        logits = oracle.forward(w, torch.tensor([p + t[:-1]]))[0, len(p) - 1:]
+        behind = logits.amax(-1) - logits.gather(1, torch.tensor(t)[:, None])[:, 0]
+        assert (behind <= 0.17 * logits.std(-1)).all(), (behind / logits.std(-1)).max()
+
+
+@pytest.mark.parametrize('kind', ['bf16', 'int8'])
+def test_greedy_text(kind):
+    from noise_b200.generate import Generator
+    w, prompts, new = oracle.informative_weights(1), _prompts(), 24
+    gen = Generator(w, kind)
+    plain = gen.generate(prompts, new, nodes=1)
+    assert gen.steps == new and gen.accepted == 0 and [len(t) for t in plain] == [new] * 3
+    _check_greedy(w, prompts, plain)
+    # drafts: the right text behind a wrong one that shares its start
+    known = {len(p): p + t for p, t in zip(prompts, plain)}
+
+    def draft(history, length):
+        full = next(f for n, f in known.items() if history[:n] == f[:n] and len(history) >= n)
+        ahead = full[len(history):len(history) + 5]
+        return [ahead[:2] + [0, 1], ahead]
+    text = gen.generate(prompts, new, nodes=12, draft=draft)
+    assert gen.steps <= new // 2 and gen.accepted >= 3 * new // 2
+    _check_greedy(w, prompts, text)
+
+
+def test_long_text_passes_the_windows():
+    """A text that outgrows the short windows of 1024."""
+    from noise_b200.generate import Generator
+    w = oracle.informative_weights(2)
+    prompt = oracle.zipf_tokens(1, 1100, seed=5).tolist()
+    text = Generator(w, 'bf16').generate(prompt, 4, nodes=4)
+    _check_greedy(w, prompt, text)
+
+
+def test_sampled_text():
+    from noise_b200.generate import Generator
+    gen = Generator(oracle.informative_weights(1), 'e4m3')
+    first = gen.generate([[5, 6, 5, 6, 5], [7]], 10, temperature=1.0, nodes=8, seed=1)
+    assert [len(t) for t in first] == [10, 10] and all(0 <= x < oracle.VOCAB for t in first for x in t)
+    assert first == gen.generate([[5, 6, 5, 6, 5], [7]], 10, temperature=1.0, nodes=8, seed=1)
+    assert first != gen.generate([[5, 6, 5, 6, 5], [7]], 10, temperature=1.0, nodes=8, seed=2)
+
+
+def test_refusals():
+    from noise_b200.generate import Generator
+    w = oracle.informative_weights(1)
+    gen = Generator(w)
+    for prompts, kw in (([[]], {}), ([[oracle.VOCAB]], {}), ([[-1]], {}), ([[1]], {'nodes': 65}),
+                        ([[1]], {'nodes': 0})):
+        with pytest.raises(ValueError):
+            gen.generate(prompts, 3, **kw)
+    assert gen.generate([], 3) == [] and gen.generate([[1]], 0) == [[]]
+    with pytest.raises(ValueError, match='lm_head'):
+        Generator({**w, 'lm_head.weight': w['lm_head.weight'][1:]})
