@@ -15,6 +15,8 @@
 #include <cstdint>
 
 #include "noise_b200.h"
+#include "ptx.cuh"
+#include "warp_mma.cuh"
 
 namespace noise {
 namespace headnorm {
@@ -71,6 +73,16 @@ struct Raw {
     } else {
       static_assert(N == 1 && sizeof(T) == 2, "one 16-bit value");
       w[0] = __ldg(reinterpret_cast<const unsigned short*>(p));
+    }
+  }
+  __device__ __forceinline__ void load_shared(const uint8_t* p) {  // 8 or 16 bytes
+    if constexpr (BYTES == 8) {
+      const uint2 u = *reinterpret_cast<const uint2*>(p);
+      w[0] = u.x, w[1] = u.y;
+    } else {
+      static_assert(BYTES == 16, "a lane's piece");
+      const uint4 u = *reinterpret_cast<const uint4*>(p);
+      w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
     }
   }
   __device__ __forceinline__ float operator[](int e) const {
@@ -229,11 +241,55 @@ __global__ void __launch_bounds__(32 * WARPS) forward_kernel(const Args a) {
   }
 }
 
+template <int BYTES>
+__device__ __forceinline__ void copy_in(uint32_t to, const void* from) {
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
+}
+
+// Blocks of the gradient on an SM. Without weights a lane holds little between items: 32 warps an SM with plain loads
+// keep the memory busy (12,287 tokens of 40 bf16 heads of 128: 62 us, 93% of the copy rate; 66 with the ring below,
+// 78 with the next item in registers and 24 warps). The weights and their sums take 120 registers, so 16 warps, and the
+// next items have to be on their way in shared memory (79 us; 91 with plain loads, 88 with 24 warps that spill).
+constexpr int grad_per_sm(bool weights) { return weights ? 2 : 4; }
+constexpr int GRAD_BLOCKS = 148 * grad_per_sm(false);
+
+// A warp's stage: x's halves, dy's, then cos and sin, each lane's 16 bytes beside the next lane's (tables: 8, 16 or two
+// times 16).
+template <typename T, typename TT, int VEC>
+struct GradRing {
+  static constexpr int PIECE = VEC * sizeof(TT), TABLE = 32 * PIECE, STAGE = 4 * 512 + 2 * TABLE;
+  static constexpr int STAGES = 3, SMEM = WARPS * STAGES * STAGE;
+  // to, from: of the lane's 16 bytes
+  static __device__ __forceinline__ void copy_table(uint32_t to, int lane, const TT* from) {
+    if constexpr (PIECE == 8) {
+      copy_in<8>(to - lane * 8, from);
+    } else {
+      copy_in<16>(to, from);
+      if constexpr (PIECE == 32) copy_in<16>(to + 512, from + VEC / 2);
+    }
+  }
+  static __device__ __forceinline__ void read_table(Raw<VEC, TT>& r, const uint8_t* from, int lane) {
+    if constexpr (PIECE == 8) {
+      r.load_shared(from - lane * 8);
+    } else {
+      const uint4 u = *reinterpret_cast<const uint4*>(from);
+      r.w[0] = u.x, r.w[1] = u.y, r.w[2] = u.z, r.w[3] = u.w;
+      if constexpr (PIECE == 32) {
+        const uint4 t = *reinterpret_cast<const uint4*>(from + 512);
+        r.w[4] = t.x, r.w[5] = t.y, r.w[6] = t.z, r.w[7] = t.w;
+      }
+    }
+  }
+};
+
 // Blocks [0, q_blocks) take the queries, the others the keys, so a lane sums one weight's gradient over all its rows;
 // a block's sums go to partial[block] (no atomics: the order is the same from call to call). A warp walks over its
-// (token, heads) items with the next one's rows on their way while it computes.
+// (token, heads) items; with weights its lanes copy their own pieces of the next two items to shared memory meanwhile.
 template <typename T, typename TT, int VEC, int LPR, int ITER, bool W>
-__global__ void __launch_bounds__(32 * WARPS) backward_kernel(const Args a) {
+__global__ void __launch_bounds__(32 * WARPS, VEC > 1 ? grad_per_sm(W) : 2) backward_kernel(const Args a) {
   __shared__ float sums[W ? WARPS : 1][2 * LPR * VEC * ITER];
   constexpr int P = (VEC + 1) / 2;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % LPR, grp = lane / LPR;
@@ -260,55 +316,101 @@ __global__ void __launch_bounds__(32 * WARPS) backward_kernel(const Args a) {
       }
     }
   }
-  struct Item {
-    Raw<VEC, T> x[ITER][2], g[ITER][2];
-    int token, h, pos;
-  };
-  const auto fetch = [&](Item& n, unsigned item) {
-    n.token = static_cast<int>(item / chunks);
-    n.h = static_cast<int>(item - n.token * chunks) * (32 / LPR) + grp;
-    if (item >= items) n.h = r.heads;
-    n.pos = item < items ? __ldg(a.positions + n.token) : -1;
+  constexpr bool RING = VEC > 1 && W;
+  using G = GradRing<T, TT, VEC>;
+  extern __shared__ __align__(16) uint8_t ring[];
+  const uint32_t mine = smem_u32(ring) + warp * (G::STAGES * G::STAGE) + lane * 16;
+  const unsigned first = block * WARPS + warp;
+  cudaTriggerProgrammaticLaunchCompletion();
+  unsigned known_at = 0;  // bit: whether the stage's position is in the tables
+  int next_pos = -1;      // of the item to be asked for next
+  const auto pos_of = [&](unsigned item) { return item < items ? __ldg(a.positions + item / chunks) : -1; };
+  const auto fetch = [&](unsigned item, int stage) {
+    const int pos = next_pos;
+    next_pos = pos_of(item + step);
+    const bool known = pos >= 0 && pos < a.table_rows;
+    known_at = (known_at & ~(1u << stage)) | static_cast<unsigned>(known) << stage;
+    if (item < items) {
+      const int token = static_cast<int>(item / chunks);
+      const int h = static_cast<int>(item - token * chunks) * (32 / LPR) + grp, i = sub * VEC;
+      const uint32_t to = mine + stage * G::STAGE;
+      if (i < half && h < r.heads) {
 #pragma unroll
-    for (int it = 0; it < ITER; ++it) {
-      const int i = (it * LPR + sub) * VEC;
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        n.x[it][p].zero();
-        n.g[it][p].zero();
-        if (n.h < r.heads && i < half) {
-          n.x[it][p].load(static_cast<const T*>(r.x) + n.token * r.token + n.h * r.head + p * half + i);
-          n.g[it][p].load(static_cast<const T*>(r.dy) + n.token * r.dy_token + n.h * r.dy_head + p * half + i);
+        for (int p = 0; p < 2; ++p) {
+          copy_in<16>(to + p * 512, static_cast<const T*>(r.x) + token * r.token + h * r.head + p * half + i);
+          copy_in<16>(to + 1024 + p * 512,
+                      static_cast<const T*>(r.dy) + token * r.dy_token + h * r.dy_head + p * half + i);
         }
       }
+      if (i < half && known) {
+        const int64_t at = static_cast<int64_t>(pos) * half + i;
+        G::copy_table(to + 2048, lane, static_cast<const TT*>(a.cos) + at);
+        G::copy_table(to + 2048 + G::TABLE, lane, static_cast<const TT*>(a.sin) + at);
+      }
     }
+    cp_async_commit();
   };
-  const unsigned first = block * WARPS + warp;
-  Item cur;
-  if (first < items) fetch(cur, first);
+  int stage = 0;
+  if constexpr (RING) {
+    next_pos = pos_of(first);
+    for (int i = 0; i < G::STAGES - 1; ++i) fetch(first + i * step, i);  // (tokens * chunks + 4 step stays below 2^32)
+  }
   for (unsigned item = first; item < items; item += step) {
-    const bool known = cur.pos >= 0 && cur.pos < a.table_rows, here = cur.h < r.heads;
+    const int token = static_cast<int>(item / chunks);
+    const int head = static_cast<int>(item - token * chunks) * (32 / LPR) + grp;
+    const bool here = head < r.heads;
+    bool known;
+    Raw<VEC, T> x[ITER][2], dy[ITER][2];
     Raw<VEC, TT> c[ITER], s[ITER];
 #pragma unroll
     for (int it = 0; it < ITER; ++it) {
-      const int i = (it * LPR + sub) * VEC;
-      c[it].zero();
-      s[it].zero();
-      if (known && i < half) {
-        c[it].load(static_cast<const TT*>(a.cos) + static_cast<int64_t>(cur.pos) * half + i);
-        s[it].load(static_cast<const TT*>(a.sin) + static_cast<int64_t>(cur.pos) * half + i);
+      x[it][0].zero(), x[it][1].zero(), dy[it][0].zero(), dy[it][1].zero();
+      c[it].zero(), s[it].zero();
+    }
+    if constexpr (RING) {
+      cp_async_wait<G::STAGES - 2>();  // this lane's own copies
+      fetch(item + (G::STAGES - 1) * step, stage == 0 ? G::STAGES - 1 : stage - 1);
+      const uint8_t* const from = ring + warp * (G::STAGES * G::STAGE) + stage * G::STAGE + lane * 16;
+      known = known_at >> stage & 1;
+      if (here && sub * VEC < half) {
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          x[0][p].load_shared(from + p * 512);
+          dy[0][p].load_shared(from + 1024 + p * 512);
+        }
+      }
+      if (known && sub * VEC < half) {
+        G::read_table(c[0], from + 2048, lane);
+        G::read_table(s[0], from + 2048 + G::TABLE, lane);
+      }
+      stage = stage == G::STAGES - 1 ? 0 : stage + 1;
+    } else {
+      const int pos = __ldg(a.positions + token);
+      known = pos >= 0 && pos < a.table_rows;
+#pragma unroll
+      for (int it = 0; it < ITER; ++it) {
+        const int i = (it * LPR + sub) * VEC;
+        if (i >= half) continue;
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          if (!here) continue;
+          x[it][p].load(static_cast<const T*>(r.x) + token * r.token + head * r.head + p * half + i);
+          dy[it][p].load(static_cast<const T*>(r.dy) + token * r.dy_token + head * r.dy_head + p * half + i);
+        }
+        if (known) {
+          c[it].load(static_cast<const TT*>(a.cos) + static_cast<int64_t>(pos) * half + i);
+          s[it].load(static_cast<const TT*>(a.sin) + static_cast<int64_t>(pos) * half + i);
+        }
       }
     }
-    Item next;
-    fetch(next, item + step);  // (tokens * chunks + step stays below 2^32)
     F2 g[ITER][2][P];
     F2 sq = both(0.f), dot = both(0.f);  // dot: sum h x
 #pragma unroll
     for (int it = 0; it < ITER; ++it)
 #pragma unroll
       for (int e = 0; e < P; ++e) {
-        const F2 d1 = get2(cur.g[it][0], e), d2 = get2(cur.g[it][1], e);
-        const F2 x1 = get2(cur.x[it][0], e), x2 = get2(cur.x[it][1], e);
+        const F2 d1 = get2(dy[it][0], e), d2 = get2(dy[it][1], e);
+        const F2 x1 = get2(x[it][0], e), x2 = get2(x[it][1], e);
         const F2 cc = get2(c[it], e), ss = get2(s[it], e);
         g[it][0][e] = fma2(d1, cc, negative(d2) * ss);
         g[it][1][e] = fma2(d1, ss, d2 * cc);
@@ -322,7 +424,7 @@ __global__ void __launch_bounds__(32 * WARPS) backward_kernel(const Args a) {
     float rr = rsqrtf(row_sum<LPR>(sums_sq.x + sums_sq.y) / a.dim + a.eps);
     if (!known) rr = __int_as_float(0x7fc00000);
     const float m = row_sum<LPR>(sums_dot.x + sums_dot.y) * rr / a.dim;  // mean(h xh)
-    T* dst = static_cast<T*>(r.out) + (static_cast<int64_t>(cur.token) * r.heads + cur.h) * a.dim;
+    T* dst = static_cast<T*>(r.out) + (static_cast<int64_t>(token) * r.heads + head) * a.dim;
     const F2 r2 = both(rr), m2 = both(-m * rr);
 #pragma unroll
     for (int it = 0; it < ITER; ++it) {
@@ -332,7 +434,7 @@ __global__ void __launch_bounds__(32 * WARPS) backward_kernel(const Args a) {
         F2 o[P];
 #pragma unroll
         for (int e = 0; e < P; ++e) {
-          const F2 xh = get2(cur.x[it][p], e) * r2;
+          const F2 xh = get2(x[it][p], e) * r2;
           F2 h = g[it][p][e];
           if constexpr (W) {
             if (here) dw[it][p][e] = fma2(h, xh, dw[it][p][e]);
@@ -343,7 +445,6 @@ __global__ void __launch_bounds__(32 * WARPS) backward_kernel(const Args a) {
         if (here && i < half) store<VEC>(dst + p * half + i, o);
       }
     }
-    cur = next;
   }
   if constexpr (W) {
     if (!a.partial) return;
@@ -392,7 +493,6 @@ __global__ void __launch_bounds__(1024) weight_kernel(const float* partial, int 
   }
 }
 
-constexpr int GRAD_BLOCKS = 148 * 4;
 
 inline int lanes_of(int half, int vec) {
   int l = 1;
@@ -416,12 +516,17 @@ cudaError_t run(Args a, bool backward, float* q_dw, float* k_dw, cudaStream_t s)
   a.k_chunks = (a.k.heads + HEADS - 1) / HEADS;
   const int64_t q_need = (static_cast<int64_t>(a.tokens) * a.q_chunks + WARPS - 1) / WARPS;
   const int64_t k_need = (static_cast<int64_t>(a.tokens) * a.k_chunks + WARPS - 1) / WARPS;
-  int64_t q_most = static_cast<int64_t>(GRAD_BLOCKS) * a.q_chunks / (a.q_chunks + a.k_chunks);
+  const int most = 148 * grad_per_sm(W);  // as many as are resident
+  int64_t q_most = static_cast<int64_t>(most) * a.q_chunks / (a.q_chunks + a.k_chunks);
   if (q_most < 1) q_most = 1;
-  const int64_t k_most = GRAD_BLOCKS - q_most > 1 ? GRAD_BLOCKS - q_most : 1;
+  const int64_t k_most = most - q_most > 1 ? most - q_most : 1;
   a.q_blocks = static_cast<int>(q_need < q_most ? q_need : q_most);
   const int blocks = a.q_blocks + static_cast<int>(k_need < k_most ? k_need : k_most);
-  backward_kernel<T, TT, VEC, LPR, ITER, W><<<blocks, 32 * WARPS, 0, s>>>(a);
+  const int smem = VEC > 1 && W ? GradRing<T, TT, VEC>::SMEM : 0;
+  if (smem && cudaFuncSetAttribute(backward_kernel<T, TT, VEC, LPR, ITER, W>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   smem) != cudaSuccess)
+    return cudaErrorInvalidValue;
+  backward_kernel<T, TT, VEC, LPR, ITER, W><<<blocks, 32 * WARPS, smem, s>>>(a);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || (!q_dw && !k_dw)) return e;
   cudaLaunchConfig_t cfg = {};
