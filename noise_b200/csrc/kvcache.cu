@@ -63,6 +63,19 @@ struct Row8 {  // 8 values as they lie in memory
 #pragma unroll
     for (int i = 0; i < static_cast<int>(sizeof(T)) * 2; ++i) w[i] = 0;
   }
+  __device__ __forceinline__ uint32_t top() const {  // the largest of the bits of |x|, or some NaN's
+    if constexpr (sizeof(T) == 4) {
+      uint32_t t = w[0] & 0x7fffffffu;
+#pragma unroll
+      for (int i = 1; i < 8; ++i) t = max(t, w[i] & 0x7fffffffu);
+      return t;
+    } else {
+      const auto two = [&](int i) { return __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[i])); };
+      const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(two(0), two(1)), __hmax2_nan(two(2), two(3)));
+      const uint32_t t = *reinterpret_cast<const uint32_t*>(&m);
+      return max(t << 16, t & 0xffff0000u);
+    }
+  }
   __device__ __forceinline__ float operator[](int i) const {
     if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
     else return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
@@ -92,9 +105,7 @@ __device__ __forceinline__ uint32_t quantise(const R& x, uint32_t (&code)[KIND =
     for (int i = 0; i < 4; ++i) code[i] = pack2(x[2 * i], x[2 * i + 1]);
     return 0;
   } else {
-    uint32_t top = 0;  // of the bits of |x|: orders NaN above infinity above the finite
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+    uint32_t top = x.top();  // the bits of the largest |x|: orders NaN above infinity above the finite
 #pragma unroll
     for (int o = LPR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (top >= 0x7f800000u) {
