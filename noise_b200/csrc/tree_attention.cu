@@ -8,7 +8,7 @@
 //
 // A cached key costs D codes of K and of V and 4 D operations a row: with up to some 64 rows of 8-bit codes the
 // kernel is bound by the cache's bytes. So it is built to stream them:
-//  - Each warp walks the keys 16 or 32 at a time and keeps a running maximum, sum and output (32 bits) for its rows. It
+//  - Each warp walks the keys 16 at a time and keeps a running maximum, sum and output (32 bits) for its rows. It
 //    copies its own steps (cp.async, a ring of STAGES of them), no other warp waits for it, and the next steps stay
 //    in flight while one computes.
 //  - Keys are the products' 16 rows (S^T = K Q^T, O^T = V^T P^T) and query rows their 8 columns, so a decoding step of
@@ -18,8 +18,11 @@
 //    consecutive bytes of a key's row, for V^T P^T four neighbouring keys of one dimension, which lie in one word of V's
 //    layout; codes become fp16 in registers.
 //  - The running maximum moves only when a score passes it by 2^8: a vote a step instead of a reduction over its keys.
-//  - The keys of all sequences, heads and row tiles form one line of units of 64 or 128 keys, cut into equal spans, one a
-//    CTA, whatever the lengths are. Parts of an item are joined by a second kernel.
+//  - The keys of all sequences, heads and row tiles form one line of units of 64 keys, cut into equal spans, one a CTA,
+//    whatever the lengths are. Parts of an item are joined by a second kernel, launched while the first still runs.
+// Measured: one token of 32 heads over 8 sequences of 8,193 to 65,536 e4m3 keys of 8 heads of 128: 100 us, 93% of the
+// bytes' time at the rate of a copy. A tree of 16 nodes, 8 heads of 64, over 8 sequences of 2,048 keys and fewer: 26 us
+// against 8 for the bytes, of which some 10 are the launches, the tree's own keys and the joining, the same for any length.
 // Roundings: Q to fp16 under a power of two per row (an element loses bits only below 2^-14 of the row's largest),
 // P 2^(scale of V) to fp16 relative to the largest scale seen; for a bf16 cache and for the nodes' own bf16 keys, P
 // to bf16, the type of V. All sums are in fp32.
@@ -36,8 +39,10 @@ namespace noise {
 namespace tree {
 
 constexpr int KW = 4;            // warps that share a row tile's keys: a unit is one step of each
-constexpr int LEAST = 2;         // units a CTA takes at least: a shorter span is all overhead
-constexpr int HEAD = 3;          // what an item costs beside its cached keys, in units
+// Units a CTA takes at least (a shorter span is all overhead), and what an item costs beside its cached keys, in units.
+// Measured at 1 / 2 and at 1 / 3 / 6: within 4% of one another; an item's cost of 0 leaves a CTA the outputs of many.
+constexpr int LEAST = 2;
+constexpr int HEAD = 3;
 constexpr int MAX_SEQS = 4096;  // two words each in shared memory
 constexpr int VREF = 127 - 20;   // the output's first unit is 2^-20: V rows with less than that as a scale lose bits
 constexpr float NEG = -INFINITY;
@@ -176,12 +181,12 @@ struct Shape {
   static constexpr int NL = BF ? D / 16 : D / 32;    // 16-byte loads a lane of K, and of V
   static constexpr int NT = 32 * KW * RW;
   static constexpr int RT = 8 * NTL * RW;
-  static constexpr int G = BF || NTL > 2 || D == 128 ? 1 : 2;  // groups of 16 keys a step: about 4 KB
-  static constexpr int CHAINS = NTL * G == 1 ? 2 : 1;  // sums of K Q^T side by side: one alone waits on itself
-  static constexpr int BLOCK = 2 * NL * 512 + (BF ? 0 : 256);  // bytes of 16 keys
-  static constexpr int STEP = G * BLOCK;
+  static constexpr int STEP = 2 * NL * 512 + (BF ? 0 : 256);  // bytes of a step: 16 keys
+  // 3 stages cost 3% of a call of 8 x 4096 int8 keys of 64; more do not fit beside 4 tiles of rows of bf16 keys of 128
   static constexpr int STAGES = STEP <= 2500 ? 4 : BF && NTL == 4 && D == 128 ? 2 : 3;
-  static constexpr bool QREG = NTL * KS <= 16;       // Q's fragments in registers, else in shared memory
+  // Q's fragments in registers, else (more than 64 a lane) in shared memory: 100 us against 108 for one token of
+  // 32 heads over 8 sequences of 8,193 to 65,536 e4m3 keys of 8 heads of 128
+  static constexpr bool QREG = NTL * KS <= 16;
   static constexpr int RING = STAGES * STEP;
   static constexpr int JOIN = 32 * (4 * NTL * MB + 4 * NTL) * 4;  // a warp's output, maxima and sums
   static constexpr int QBYTES = QREG ? 0 : RW * NTL * KS * 256;
@@ -228,16 +233,14 @@ struct Part {
   int vref;                     // acc holds the output in units of 2^(vref - 127) (8-bit kinds)
 
   // The maximum and the output's unit moved; every lane of the warp calls it.
-  __device__ __forceinline__ void move(const float (&s)[S::G][NTL][4], int new_ref) {
+  __device__ __forceinline__ void move(const float (&s)[NTL][4], int new_ref) {
     const float unit = ex2(static_cast<float>(vref - new_ref));
     vref = new_ref;
 #pragma unroll
     for (int nt = 0; nt < NTL; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float x = NEG;
-#pragma unroll
-        for (int j = 0; j < S::G; ++j) x = fmaxf(x, fmaxf(s[j][nt][e], s[j][nt][2 + e]));
+        float x = fmaxf(s[nt][e], s[nt][2 + e]);
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16)) * rf[nt][e];
@@ -257,14 +260,12 @@ struct Part {
   }
 
   // Scores s (masked: -inf) to probabilities, their sums, and the running maximum; ref: the largest V scale there is.
-  __device__ __forceinline__ void soften(float (&s)[S::G][NTL][4], int ref) {
+  __device__ __forceinline__ void soften(float (&s)[NTL][4], int ref) {
     bool up = ref > vref;
 #pragma unroll
-    for (int j = 0; j < S::G; ++j)
+    for (int nt = 0; nt < NTL; ++nt)
 #pragma unroll
-      for (int nt = 0; nt < NTL; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) up |= fmaf(s[j][nt][e], rf[nt][e & 1], off[nt][e & 1]) > SLACK;
+      for (int e = 0; e < 4; ++e) up |= fmaf(s[nt][e], rf[nt][e & 1], off[nt][e & 1]) > SLACK;
     if (__any_sync(0xffffffffu, up)) {
       ref = max(ref, __shfl_xor_sync(0xffffffffu, ref, 4));
       ref = max(ref, __shfl_xor_sync(0xffffffffu, ref, 8));
@@ -272,14 +273,12 @@ struct Part {
       move(s, max(ref, vref));
     }
 #pragma unroll
-    for (int j = 0; j < S::G; ++j)
+    for (int nt = 0; nt < NTL; ++nt)
 #pragma unroll
-      for (int nt = 0; nt < NTL; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[j][nt][e] = ex2(fmaf(s[j][nt][e], rf[nt][e & 1], off[nt][e & 1]));
-          l[nt][e & 1] += s[j][nt][e];
-        }
+      for (int e = 0; e < 4; ++e) {
+        s[nt][e] = ex2(fmaf(s[nt][e], rf[nt][e & 1], off[nt][e & 1]));
+        l[nt][e & 1] += s[nt][e];
+      }
   }
 };
 
@@ -351,7 +350,7 @@ __global__ void __launch_bounds__(Shape<KIND, D, NTL, RW>::NT)
     attend_kernel(const Params p) {
   using S = Shape<KIND, D, NTL, RW>;
   constexpr bool BF = S::BF;
-  constexpr int NL = S::NL, KS = S::KS, MB = S::MB, G = S::G;
+  constexpr int NL = S::NL, KS = S::KS, MB = S::MB;
   extern __shared__ __align__(16) uint8_t smem[];
   uint2* const qs = reinterpret_cast<uint2*>(smem + S::WORK);
   int* const before = reinterpret_cast<int*>(smem + S::SMEM);
@@ -430,42 +429,37 @@ __global__ void __launch_bounds__(Shape<KIND, D, NTL, RW>::NT)
     // ---- then the cached keys' first copies
     const int* table = p.table + static_cast<int64_t>(b) * p.width;
     const int cshift = p.page_shift - 4;
-    int chunk = (unit0 + max(u0, HEAD)) * KW + kw;  // of 16 G keys
-    const int chunk_end = min((unit0 + u1) * KW, (len + 16 * G - 1) / (16 * G));
+    int chunk = (unit0 + max(u0, HEAD)) * KW + kw;  // of 16 keys
+    const int chunk_end = min((unit0 + u1) * KW, (len + 15) / 16);
     int ahead = chunk, page0 = -64, pages = 0;
     bool lost = false;
     const uint8_t* const k_lane = static_cast<const uint8_t*>(p.c.k) + lane * 16;
     const uint8_t* const v_lane = static_cast<const uint8_t*>(p.c.v) + lane * 16;
     const auto fetch = [&](int stage) {
       if (ahead < chunk_end) {
+        const int pi = ahead >> cshift;  // 16 keys are in one page
+        if (pi >= page0 + 32) {  // the next 32 entries of the table, one a lane
+          page0 = pi;
+          pages = page0 + lane < p.width ? table[page0 + lane] : 0;
+        }
+        int page = __shfl_sync(0xffffffffu, pages, pi - page0);
+        if (page < 0 || page >= p.c.pages) {
+          lost = true;
+          page = 0;
+        }
+        const int64_t cell =
+            (((p.layer_cell + page) * p.heads + h) << p.page_shift) + ((ahead & ((1 << cshift) - 1)) << 4);
+        const uint32_t to = smem_u32(ring) + stage * S::STEP;
+        const uint8_t* k = k_lane + cell * (D * (BF ? 2 : 1));
+        const uint8_t* v = v_lane + cell * (D * (BF ? 2 : 1));
 #pragma unroll
-        for (int j = 0; j < G; ++j) {
-          const int block = ahead * G + j;  // of 16 keys: in one page
-          if (j > 0 && block << 4 >= len) break;  // (stays as it is: masked)
-          const int pi = block >> cshift;
-          if (pi >= page0 + 32) {  // the next 32 entries of the table, one a lane
-            page0 = pi;
-            pages = page0 + lane < p.width ? table[page0 + lane] : 0;
-          }
-          int page = __shfl_sync(0xffffffffu, pages, pi - page0);
-          if (page < 0 || page >= p.c.pages) {
-            lost = true;
-            page = 0;
-          }
-          const int64_t cell =
-              (((p.layer_cell + page) * p.heads + h) << p.page_shift) + ((block & ((1 << cshift) - 1)) << 4);
-          const uint32_t to = smem_u32(ring) + stage * S::STEP + j * S::BLOCK;
-          const uint8_t* k = k_lane + cell * (D * (BF ? 2 : 1));
-          const uint8_t* v = v_lane + cell * (D * (BF ? 2 : 1));
+        for (int c = 0; c < NL; ++c) copy16(to + S::k_place(c * 32 + lane) * 16, k + c * 512);
 #pragma unroll
-          for (int c = 0; c < NL; ++c) copy16(to + S::k_place(c * 32 + lane) * 16, k + c * 512);
-#pragma unroll
-          for (int c = 0; c < NL; ++c) copy16(to + S::v_place(c * 32 + lane) * 16, v + c * 512);
-          if constexpr (!BF) {
-            const uint32_t s4 = to + lane * 4 + 2 * NL * 512;
-            copy4(s4, p.c.k_scale + cell + (g & 6) * 2);
-            copy4(s4 + 128, p.c.v_scale + cell + (g & 6) * 2);
-          }
+        for (int c = 0; c < NL; ++c) copy16(to + S::v_place(c * 32 + lane) * 16, v + c * 512);
+        if constexpr (!BF) {
+          const uint32_t s4 = to + lane * 4 + 2 * NL * 512;
+          copy4(s4, p.c.k_scale + cell + (g & 6) * 2);
+          copy4(s4 + 128, p.c.v_scale + cell + (g & 6) * 2);
         }
       }
       cp_async_commit();
@@ -527,15 +521,11 @@ __global__ void __launch_bounds__(Shape<KIND, D, NTL, RW>::NT)
     cp_async_wait<S::STAGES - 1>();
     __syncthreads();  // depths, the tree's rows and masks, Q in shared memory
     if (u0 == 0 && kw * 16 < p.nodes) {
-      float both[G][NTL][4];  // the second group of 16: none
-      float(&s)[NTL][4] = both[0];
+      float s[NTL][4];
 #pragma unroll
       for (int nt = 0; nt < NTL; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[nt][e] = 0.f;
-          if constexpr (G == 2) both[1][nt][e] = NEG;
-        }
+        for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
       int node2[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) node2[j] = kw * 16 + key_of(g) + 2 * j;
@@ -577,7 +567,7 @@ __global__ void __launch_bounds__(Shape<KIND, D, NTL, RW>::NT)
         }
       uint32_t vis[NTL][2], pf[NTL][2];
       visible<NTL>(s, vis);
-      part.soften(both, part.vref);
+      part.soften(s, part.vref);
       constexpr float UNITS = BF ? 1.f : 1048576.f;  // 1 in units of 2^(VREF - 127)
 #pragma unroll
       for (int nt = 0; nt < NTL; ++nt) p_fragment<true>(s[nt], UNITS, UNITS, pf[nt]);
@@ -605,146 +595,126 @@ __global__ void __launch_bounds__(Shape<KIND, D, NTL, RW>::NT)
       __syncwarp();  // every lane's copies of this step are there, and the step read last is read
       fetch(stage == 0 ? S::STAGES - 1 : stage - 1);
       const uint8_t* step = ring + stage * S::STEP;
-      const int key0 = chunk * 16 * G;
+      const int key0 = chunk * 16;
       // some key is past the end, or before the window of the deepest node there could be
-      const bool edge = key0 + 16 * G > len || (p.window >= 0 && key0 < len + p.nodes - p.window);
-      float s[G][NTL][4];
-      uint32_t vb[G][2];  // V's scale bytes of keys g and g + 8
-      uint32_t keep[G];   // a byte for each of quad t's keys that exist
+      const bool edge = key0 + 16 > len || (p.window >= 0 && key0 < len + p.nodes - p.window);
+      float s[NTL][4];
+      uint32_t vb[2];   // V's scale bytes of keys g and g + 8
+      uint32_t keep = 0xffffffffu;  // a byte for each of quad t's keys that exist
+      const uint4* own = reinterpret_cast<const uint4*>(step);
 #pragma unroll
-      for (int j = 0; j < G; ++j) {
-        const uint4* own = reinterpret_cast<const uint4*>(step + j * S::BLOCK);
-        float chain[S::CHAINS][NTL][4];
+      for (int nt = 0; nt < NTL; ++nt)
 #pragma unroll
-        for (int x = 0; x < S::CHAINS; ++x)
+        for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
 #pragma unroll
-          for (int nt = 0; nt < NTL; ++nt)
+      for (int c = 0; c < NL / 2; ++c) {
+        constexpr int PER = BF ? 2 : 4;  // steps in 16 bytes
+        uint32_t w[2][4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) chain[x][nt][e] = 0.f;
+        for (int i = 0; i < 2; ++i) {
+          const uint4 u = own[S::k_read(i, c, g, t)];
+          w[i][0] = u.x, w[i][1] = u.y, w[i][2] = u.z, w[i][3] = u.w;
+        }
 #pragma unroll
-        for (int c = 0; c < NL / 2; ++c) {
-          constexpr int PER = BF ? 2 : 4;  // steps in 16 bytes
-          uint32_t w[2][4];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint4 u = own[S::k_read(i, c, g, t)];
-            w[i][0] = u.x, w[i][1] = u.y, w[i][2] = u.z, w[i][3] = u.w;
+        for (int i = 0; i < PER; ++i) {
+          const int ks = c * PER + i;
+          uint32_t a[4];
+          if constexpr (BF) {
+            a[0] = w[0][2 * i], a[1] = w[1][2 * i], a[2] = w[0][2 * i + 1], a[3] = w[1][2 * i + 1];
+          } else {
+            kv::decode4<KIND>(w[0][i], a[0], a[2]);
+            kv::decode4<KIND>(w[1][i], a[1], a[3]);
           }
 #pragma unroll
-          for (int i = 0; i < PER; ++i) {
-            const int ks = c * PER + i;
-            uint32_t a[4];
-            if constexpr (BF) {
-              a[0] = w[0][2 * i], a[1] = w[1][2 * i], a[2] = w[0][2 * i + 1], a[3] = w[1][2 * i + 1];
+          for (int nt = 0; nt < NTL; ++nt) {
+            if constexpr (S::QREG) {
+              mma<BF>(s[nt], a, qr[nt][ks][0], qr[nt][ks][1]);
             } else {
-              kv::decode4<KIND>(w[0][i], a[0], a[2]);
-              kv::decode4<KIND>(w[1][i], a[1], a[3]);
-            }
-#pragma unroll
-            for (int nt = 0; nt < NTL; ++nt) {
-              if constexpr (S::QREG) {
-                mma<BF>(chain[ks % S::CHAINS][nt], a, qr[nt][ks][0], qr[nt][ks][1]);
-              } else {
-                const uint2 x = qs[((rw * NTL + nt) * KS + ks) * 32 + lane];
-                mma<BF>(chain[ks % S::CHAINS][nt], a, x.x, x.y);
-              }
+              const uint2 x = qs[((rw * NTL + nt) * KS + ks) * 32 + lane];
+              mma<BF>(s[nt], a, x.x, x.y);
             }
           }
         }
+      }
+      vb[0] = vb[1] = 0;
+      if constexpr (!BF) {
+        const uint32_t* sc = reinterpret_cast<const uint32_t*>(step + 2 * NL * 512) + lane;
+        const uint32_t kb = sc[0] >> (8 * (g & 1)), v2 = sc[32] >> (8 * (g & 1));
+        vb[0] = v2 & 0xffu, vb[1] = v2 >> 16 & 0xffu;
+        // byte 255 gives infinity, times the row's zero codes NaN
+        const float f0 = __uint_as_float((kb & 0xffu) << 23), f1 = __uint_as_float((kb & 0xff0000u) << 7);
+#pragma unroll
+        for (int nt = 0; nt < NTL; ++nt) s[nt][0] *= f0, s[nt][1] *= f0, s[nt][2] *= f1, s[nt][3] *= f1;
+      }
+      if (edge) {
+        const int left4 = len - key0 - 4 * t, k0 = key0 + key_of(g);
+        keep = left4 >= 4 ? 0xffffffffu : left4 <= 0 ? 0u : 0xffffffffu >> (32 - 8 * left4);
+        const int seen = p.window < 0 ? 0 : len - p.window;  // no row sees a key before: its scale counts for nothing
+        if (k0 >= len || k0 < seen) vb[0] = 0;
+        if (k0 + 2 >= len || k0 + 2 < seen) vb[1] = 0;
 #pragma unroll
         for (int nt = 0; nt < NTL; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            s[j][nt][e] = S::CHAINS == 2 ? chain[0][nt][e] + chain[S::CHAINS - 1][nt][e] : chain[0][nt][e];
-        vb[j][0] = vb[j][1] = 0;
-        if constexpr (!BF) {
-          const uint32_t* sc = reinterpret_cast<const uint32_t*>(step + j * S::BLOCK + 2 * NL * 512) + lane;
-          const uint32_t kb = sc[0] >> (8 * (g & 1)), v2 = sc[32] >> (8 * (g & 1));
-          vb[j][0] = v2 & 0xffu, vb[j][1] = v2 >> 16 & 0xffu;
-          // byte 255 gives infinity, times the row's zero codes NaN
-          const float f0 = __uint_as_float((kb & 0xffu) << 23), f1 = __uint_as_float((kb & 0xff0000u) << 7);
-#pragma unroll
-          for (int nt = 0; nt < NTL; ++nt) s[j][nt][0] *= f0, s[j][nt][1] *= f0, s[j][nt][2] *= f1, s[j][nt][3] *= f1;
-        }
-        keep[j] = 0xffffffffu;
-        if (edge) {
-          const int k16 = key0 + 16 * j, left4 = len - k16 - 4 * t, k0 = k16 + key_of(g);
-          keep[j] = left4 >= 4 ? 0xffffffffu : left4 <= 0 ? 0u : 0xffffffffu >> (32 - 8 * left4);
-          const int seen = p.window < 0 ? 0 : len - p.window;  // no row sees a key before: its scale counts for nothing
-          if (k0 >= len || k0 < seen) vb[j][0] = 0;
-          if (k0 + 2 >= len || k0 + 2 < seen) vb[j][1] = 0;
-#pragma unroll
-          for (int nt = 0; nt < NTL; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int low = p.window < 0 ? 0 : len + depth_of(nt, e) - p.window;
-              if (k0 >= len || k0 < low) s[j][nt][e] = NEG;
-              if (k0 + 2 >= len || k0 + 2 < low) s[j][nt][2 + e] = NEG;
-            }
-        }
+          for (int e = 0; e < 2; ++e) {
+            const int low = p.window < 0 ? 0 : len + depth_of(nt, e) - p.window;
+            if (k0 >= len || k0 < low) s[nt][e] = NEG;
+            if (k0 + 2 >= len || k0 + 2 < low) s[nt][2 + e] = NEG;
+          }
       }
       uint32_t vis[BF ? NTL : 1][2];
       if constexpr (BF) {
-        if (edge) visible<NTL>(s[0], vis);
+        if (edge) visible<NTL>(s, vis);
         part.soften(s, part.vref);
       } else {
-        uint32_t top = 0;
-#pragma unroll
-        for (int j = 0; j < G; ++j) top = max(top, max(vb[j][0], vb[j][1]));
+        uint32_t top = max(vb[0], vb[1]);
         if (__any_sync(0xffffffffu, top == 255)) {
           // rows of V that read as NaN: taken out of the product (codes 0, factor 0) and put into the sums
           top = 0;
 #pragma unroll
-          for (int j = 0; j < G; ++j)
+          for (int i = 0; i < 2; ++i) {
+            if (vb[i] == 255) {
+              vb[i] = 0;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              if (vb[j][i] == 255) {
-                vb[j][i] = 0;
+              for (int nt = 0; nt < NTL; ++nt)
 #pragma unroll
-                for (int nt = 0; nt < NTL; ++nt)
-#pragma unroll
-                  for (int e = 0; e < 2; ++e)
-                    if (s[j][nt][2 * i + e] != NEG) part.l[nt][e] = __int_as_float(0x7fc00000);
-              }
-              top = max(top, vb[j][i]);
+                for (int e = 0; e < 2; ++e)
+                  if (s[nt][2 * i + e] != NEG) part.l[nt][e] = __int_as_float(0x7fc00000);
             }
+            top = max(top, vb[i]);
+          }
         }
         part.soften(s, static_cast<int>(top));
       }
+      float f0 = 1.f, f1 = 1.f;
+      if constexpr (!BF) {
+        f0 = kv::power(max(static_cast<int>(vb[0]) - part.vref + 127, 0));
+        f1 = kv::power(max(static_cast<int>(vb[1]) - part.vref + 127, 0));
+      }
+      uint32_t pf[NTL][2];
 #pragma unroll
-      for (int j = 0; j < G; ++j) {
-        const uint4* own = reinterpret_cast<const uint4*>(step + j * S::BLOCK);
-        float f0 = 1.f, f1 = 1.f;
-        if constexpr (!BF) {
-          f0 = kv::power(max(static_cast<int>(vb[j][0]) - part.vref + 127, 0));
-          f1 = kv::power(max(static_cast<int>(vb[j][1]) - part.vref + 127, 0));
-        }
-        uint32_t pf[NTL][2];
+      for (int nt = 0; nt < NTL; ++nt) p_fragment<BF>(s[nt], f0, f1, pf[nt]);
 #pragma unroll
-        for (int nt = 0; nt < NTL; ++nt) p_fragment<BF>(s[j][nt], f0, f1, pf[nt]);
+      for (int c = 0; c < NL; ++c) {
+        const uint4 u = own[S::v_read(c, g, t)];
+        uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        if constexpr (BF) {  // dimensions 2g, 2g + 1 of 16: words keys 01, 23 of the one, then of the other
+          const uint32_t a[4] = {w[0], w[2], w[1], w[3]};
+          if (edge) {
+            const uint32_t lo = __byte_perm(keep, 0, 0x1100), hi = __byte_perm(keep, 0, 0x3322);
+            const uint32_t a2[4] = {a[0] & lo, a[1] & lo, a[2] & hi, a[3] & hi};
+            pv_special<NTL, MB>(part.acc, c, a2, pf, vis);
+          } else {
 #pragma unroll
-        for (int c = 0; c < NL; ++c) {
-          const uint4 u = own[S::v_read(c, g, t)];
-          uint32_t w[4] = {u.x, u.y, u.z, u.w};
-          if constexpr (BF) {  // dimensions 2g, 2g + 1 of 16: words keys 01, 23 of the one, then of the other
-            const uint32_t a[4] = {w[0], w[2], w[1], w[3]};
-            if (edge) {
-              const uint32_t lo = __byte_perm(keep[j], 0, 0x1100), hi = __byte_perm(keep[j], 0, 0x3322);
-              const uint32_t a2[4] = {a[0] & lo, a[1] & lo, a[2] & hi, a[3] & hi};
-              pv_special<NTL, MB>(part.acc, c, a2, pf, vis);
-            } else {
+            for (int nt = 0; nt < NTL; ++nt) mma<true>(part.acc[nt][c], a, pf[nt][0], pf[nt][1]);
+          }
+        } else {  // dimensions 4g .. 4g + 3 of 32
 #pragma unroll
-              for (int nt = 0; nt < NTL; ++nt) mma<true>(part.acc[nt][c], a, pf[nt][0], pf[nt][1]);
-            }
-          } else {  // dimensions 4g .. 4g + 3 of 32
+          for (int i = 0; i < 2; ++i) {
+            uint32_t a[4];
+            kv::decode4<KIND>(w[2 * i] & keep, a[0], a[2]);
+            kv::decode4<KIND>(w[2 * i + 1] & keep, a[1], a[3]);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              uint32_t a[4];
-              kv::decode4<KIND>(w[2 * i] & keep[j], a[0], a[2]);
-              kv::decode4<KIND>(w[2 * i + 1] & keep[j], a[1], a[3]);
-#pragma unroll
-              for (int nt = 0; nt < NTL; ++nt) mma<false>(part.acc[nt][2 * c + i], a, pf[nt][0], pf[nt][1]);
-            }
+            for (int nt = 0; nt < NTL; ++nt) mma<false>(part.acc[nt][2 * c + i], a, pf[nt][0], pf[nt][1]);
           }
         }
       }
@@ -978,7 +948,8 @@ inline int sm_count() {
 // Joins the items' parts after the kernel that makes them.
 inline int launch_join(const Params& p, int rt, int dim, cudaStream_t s) {
   // parts an item may have: with few, a thread goes through them all; with many (a few long rows over the whole GPU) 16
-  // threads share them
+  // threads share them (one token over 60,000 int8 keys of 8 heads of 64: 20 us, 30 with one thread; 8 sequences of
+  // 32-row trees over 4,096 keys: 52 and 50)
   const int items = p.seqs * p.heads * p.tiles, shares = p.grid / items >= 8 ? 16 : p.grid / items >= 3 ? 4 : 1;
   const int groups = rt * dim / 4;
   cudaLaunchConfig_t cfg = {};
@@ -1012,8 +983,8 @@ int run(Params& p, size_t workspace_bytes, cudaStream_t s) {
   p.grid = sms * per_sm;
   if (p.grid > max_grid(S::RT)) p.grid = max_grid(S::RT);
   const int64_t room = static_cast<int64_t>(p.width) << p.page_shift;
-  p.unit_shift = S::G == 2 ? 7 : 6;
-  static_assert(16 * KW == 64, "a unit is KW steps of 16 G keys");
+  p.unit_shift = 6;
+  static_assert(16 * KW == 64, "a unit is KW steps of 16 keys");
   const int64_t units = static_cast<int64_t>(p.seqs) * p.heads * p.tiles * (HEAD + 1 + (room >> p.unit_shift));
   if (units > 0x7fffffff) return NOISE_ERR_SHAPE;
   if (units / LEAST < p.grid) p.grid = units < 2 * LEAST ? 1 : static_cast<int>(units / LEAST);

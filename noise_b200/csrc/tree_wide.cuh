@@ -15,6 +15,15 @@
 // A row's maximum moves when a score passes it by 2^8, and O in tensor memory is rescaled then by its own warps: S_g of
 // a tile is only issued after P_g V of the last one, so O is still. The tree's own keys are the first tile, brought to
 // fp16 under a power of two per key like the codes.
+//
+// Measured: trees of 64 nodes, 32 heads on 8 key heads of 128, over 8 sequences of 4,000 to 8,192 int8 keys: 188 us (265 on
+// the warp products), six times the products' time at the rate of a large matrix product. A tile of 128 keys takes 4.6
+// us: 2.2 of softmax on a group's four warps (128 scores a thread: exponentials, packing, the row's maximum), and the
+// groups, the conversions (2 us each of K and V) and the MMAs (1.3) overlap only in part, since S and P share columns and
+// P V has to be issued before the next S. An item's start and end, its Q in and its O out, take 10 to 17 us of a CTA.
+// Roundings: as on the warp products, and K's and V's codes, as fp16, to 2^-24 of the largest scale of their tile (V: of
+// the tiles so far) among the keys that some row sees; a key's codes are whole numbers, so they lose bits only 2^24 (int8)
+// or 2^15 (e4m3) below it.
 #pragma once
 
 #include "kv.cuh"
